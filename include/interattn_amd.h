@@ -506,6 +506,62 @@ IA_API int64_t ia_set_wait_limit(int64_t ticks);
  */
 IA_API int64_t ia_wait_fallbacks(int32_t reset);
 
+/*
+ * Packed prompts: n_seq sequences of different lengths one behind the other in n_tokens
+ * rows.  q[t, h, :] at q + t * q_token_stride + h * q_head_stride (elements, 16-byte
+ * multiples; rows of head_dim contiguous elements).  The query heads of a kv head are
+ * neighbours, any number up to 64 of them.
+ */
+typedef struct ia_prompt_shape {
+  int32_t n_seq;
+  int32_t n_tokens;
+  int32_t n_q_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim; /* 64 or 128 */
+  int32_t q_dtype;  /* IA_F32 or IA_BF16 */
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+} ia_prompt_shape;
+
+/* K and V rows of packed prompts (strides in elements, 16-byte multiples). */
+typedef struct ia_packed_kv {
+  const void* k;
+  const void* v;
+  int32_t dtype; /* IA_F32 or IA_BF16 */
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+} ia_packed_kv;
+
+/*
+ * Causal attention over packed prompts: sequence b is the tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (a device array [n_seq + 1], not decreasing, within [0,
+ * n_tokens]; values outside are clipped), and token i of it attends tokens 0..i of it:
+ * out[t, h] = softmax(q[t, h] . k^T * scale) v, float32 sums, written to out [n_tokens,
+ * n_q_heads, head_dim] (contiguous, out_dtype).  Rows of no sequence are left as they
+ * were.  Replaces the reference's SDPA prefill (_sdpa_prefill_attention_forward,
+ * CBT/core.py:1180-1200) for a batch of prompts without padding.
+ *
+ * ia_paged_prompt_attention is the same with K and V in a paged pool, into which the new
+ * tokens' rows have been written already: q holds the last cu_seqlens[b + 1] -
+ * cu_seqlens[b] tokens of sequence b, which has seq_lens[b] tokens (a device array
+ * [n_seq]) in the pool, and a query at position i attends positions 0..i.  A chunk of a
+ * long prompt, a prompt behind a cached prefix and a single new token are all this call.
+ * Pages outside [0, n_pages) and positions the block table cannot hold contribute
+ * nothing; a row that sees no key is zeros.
+ *
+ * Few rows over many keys are cut along the keys and merged in a second launch, for which
+ * the workspace holds partials: ia_prompt_attention_workspace_size bytes (0 where nothing
+ * is cut, else one size per device, kv_dtype and head_dim) with max_keys the keys a sequence can have (n_tokens for packed K/V, else what
+ * the pool's table can hold).  Its contents need no initialisation.
+ */
+IA_API size_t ia_prompt_attention_workspace_size(const ia_prompt_shape* shape, int32_t kv_dtype, int64_t max_keys);
+IA_API int ia_prompt_attention(const ia_prompt_shape* shape, const void* q, const ia_packed_kv* kv,
+                               const int32_t* cu_seqlens, float scale, void* out, int32_t out_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+IA_API int ia_paged_prompt_attention(const ia_prompt_shape* shape, const void* q, const ia_paged_kv* kv,
+                                     const int32_t* seq_lens, const int32_t* cu_seqlens, float scale, void* out,
+                                     int32_t out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Most split-K items per (b, h) the two decode entry points use for the given
  * workload (the stride of the partials); size the decode workspace with it.
  * Tokens of ia_paged_decode past max_seq_len (rounded up to a 128-token tile) are

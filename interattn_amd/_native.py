@@ -119,6 +119,31 @@ class SuffixKV(ctypes.Structure):
     ]
 
 
+class PromptShape(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("q_dtype", ctypes.c_int32),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+    ]
+
+
+class PackedKV(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -201,6 +226,13 @@ SIGNATURES = {
         [ctypes.POINTER(DecodeShape), _P, ctypes.POINTER(BlockSummaries), _P, ctypes.POINTER(PagedKV),
          ctypes.POINTER(SuffixKV), _F, _P, _I32, _P, _SZ, _P]),
     "ia_topk_block_mask": (ctypes.c_int, [_P, _P, _I32, _I32, _I32, _I32, _P, _P]),
+    "ia_prompt_attention_workspace_size": (_SZ, [ctypes.POINTER(PromptShape), _I32, _I64]),
+    "ia_prompt_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(PromptShape), _P, ctypes.POINTER(PackedKV), _P, _F, _P, _I32, _P, _SZ, _P]),
+    "ia_paged_prompt_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(PromptShape), _P, ctypes.POINTER(PagedKV), _P, _P, _F, _P, _I32, _P, _SZ, _P]),
     "ia_sparse_max_items": (_I32, [_I32, _I32, _I32]),
     "ia_dense_max_items": (_I32, [_I32, _I32, _I32]),
 }

@@ -1,0 +1,120 @@
+// Causal attention of packed prompts: parameters shared by the host side and the per-type
+// kernel instances.
+#pragma once
+
+#include "attend_rows.hpp"
+
+namespace ia {
+
+struct PromptParams {
+  ArParams ar;
+  const int32_t* cu;        // [n_seq + 1] first token of each sequence in q
+  const int32_t* seq_lens;  // paged: [n_seq] keys of each sequence; null: its own tokens
+  int64_t kv_cap;           // paged: keys a block-table row can hold
+  int32_t n_seq, n_tokens;
+  int32_t tile_tokens;      // tokens of a row tile (128 / group)
+  int32_t n_tiles;          // bound over all sequences
+  int32_t slices;           // most key slices of a row tile
+  float* part_ml;
+  float* part_acc;
+};
+
+constexpr int kPromptSliceTiles = 8;  // fewest key tiles a slice is worth (512 keys)
+
+// slices the keys of a row tile are cut into, and the key tiles of each
+__host__ __device__ inline int prompt_slices(int key_tiles, int most) {
+  int n = (key_tiles + kPromptSliceTiles - 1) / kPromptSliceTiles;
+  return n < 1 ? 1 : n > most ? most : n;
+}
+
+int launch_prompt_bf16(const PromptParams& p, int d, hipStream_t st);
+int launch_prompt_f32(const PromptParams& p, int d, hipStream_t st);
+int launch_prompt_fp8(const PromptParams& p, int d, hipStream_t st);
+
+// A row tile of the packed batch.  Sequence b's tiles are numbered from cu[b] / T + b
+// (T tokens a tile): floor sums leave every sequence room for its own, so a workgroup
+// finds its sequence from cu alone, 64 candidates at a time, with no scan over the batch.
+struct PromptTile {
+  int b, tok0, n_tok;  // sequence, first token (of q), tokens; n_tok 0: no tile
+  int first, count;    // the sequence's first token and token count
+};
+
+__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int tile, int lane) {
+  PromptTile r{};
+  int lo = 0, len = p.n_seq;
+  auto cu = [&](int i) {
+    const int x = p.cu[i];
+    return x < 0 ? 0 : x > p.n_tokens ? p.n_tokens : x;
+  };
+  while (len > 1) {
+    const int step = (len + 63) / 64, i = lo + lane * step;
+    const bool in = lane * step < len;
+    const unsigned long long at = __ballot(in && cu(i) / p.tile_tokens + i <= tile);
+    const int n = at ? 64 - __builtin_clzll(at) : 1;  // the last candidate that starts at or before the tile
+    len = len - (n - 1) * step < step ? len - (n - 1) * step : step;
+    lo += (n - 1) * step;
+  }
+  const int c0 = cu(lo), c1 = cu(lo + 1);
+  r.b = lo;
+  r.first = c0;
+  r.count = c1 > c0 ? c1 - c0 : 0;
+  const int local = tile - (c0 / p.tile_tokens + lo);
+  const int64_t t0 = (int64_t)local * p.tile_tokens;
+  if (local < 0 || t0 >= r.count) return r;
+  r.tok0 = c0 + (int)t0;
+  r.n_tok = r.count - (int)t0 < p.tile_tokens ? r.count - (int)t0 : p.tile_tokens;
+  return r;
+}
+
+// keys the tile's last row sees, and the first row's limit
+__device__ __forceinline__ void prompt_keys(const PromptParams& p, const PromptTile& t, int* limit0, int* k_hi) {
+  int64_t total = t.count;
+  if (p.seq_lens) total = p.seq_lens[t.b];
+  const int64_t first = total - t.count + (t.tok0 - t.first) + 1;  // keys the tile's first token sees
+  *limit0 = (int)first;
+  int64_t hi = first + t.n_tok - 1;
+  if (p.seq_lens && hi > p.kv_cap) hi = p.kv_cap;
+  *k_hi = hi < 0 ? 0 : (int)hi;
+}
+
+template <int KV, int D>
+__global__ __launch_bounds__(kArThreads, KV == kArF32 ? 1 : 2) void ia_prompt_attention(PromptParams p) {
+  __shared__ __align__(1024) char smem[ArShape<KV, D>::kSmem];
+  // heads fastest, so that with 2^n heads a head's tiles share XCDs (their L2 holds its
+  // K/V); later tiles of the batch, which see more keys, first
+  int id = blockIdx.x;
+  const int head = id % p.ar.n_kv_heads;
+  id /= p.ar.n_kv_heads;
+  const int slice = id % p.slices, tile = p.n_tiles - 1 - id / p.slices;
+  const PromptTile t = prompt_tile(p, tile, threadIdx.x & 63);
+  if (t.n_tok == 0) return;
+  ArItem it{};
+  int k_end = 0;
+  prompt_keys(p, t, &it.limit0, &k_end);
+  const int key_tiles = (k_end + kArTile - 1) / kArTile;
+  const int n = prompt_slices(key_tiles, p.slices);
+  if (slice >= n) return;
+  const int per = (key_tiles + n - 1) / n;
+  it.k_lo = slice * per * kArTile;
+  it.k_hi = (slice + 1) * per * kArTile < k_end ? (slice + 1) * per * kArTile : k_end;
+  it.table = p.ar.kv.table ? p.ar.kv.table + (int64_t)t.b * p.ar.kv.bt_stride : nullptr;
+  it.row0 = p.seq_lens ? 0 : t.first;
+  it.head = head;
+  it.tok0 = t.tok0;
+  it.n_rows = t.n_tok * p.ar.group;
+  if (n > 1) {
+    const int64_t slot = ((int64_t)tile * p.ar.n_kv_heads + head) * p.slices + slice;
+    it.part_ml = p.part_ml + slot * (2 * kArRows);
+    it.part_acc = p.part_acc + slot * (kArRows * (int64_t)D);
+  }
+  ar_attend<KV, D>(p.ar, it, smem);
+}
+
+template <int KV, int D>
+int launch_prompt(const PromptParams& p, hipStream_t st) {
+  const unsigned tiles = (unsigned)p.n_tiles * p.ar.n_kv_heads;
+  hipLaunchKernelGGL((ia_prompt_attention<KV, D>), dim3(tiles * p.slices), dim3(kArThreads), 0, st, p);
+  return check_launch("prompt attention");
+}
+
+}  // namespace ia
