@@ -562,6 +562,28 @@ IA_API int ia_paged_prompt_attention(const ia_prompt_shape* shape, const void* q
                                      const int32_t* seq_lens, const int32_t* cu_seqlens, float scale, void* out,
                                      int32_t out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Dense paged decode of a batch whose sequences share long prefixes (continuations of one
+ * prompt, requests behind one system prompt): ia_paged_decode's result, with each shared
+ * prefix's K/V read once for all sequences of its group.  Group g is the sequences
+ * group_starts[g] .. group_starts[g + 1] - 1 (a device array [n_groups + 1], not
+ * decreasing, values outside [0, batch] clipped; sequences of no group share nothing), and
+ * the first shared_lens[g] tokens (a device array [n_groups], any number) of all of them
+ * are the same: the call reads them through the block-table row of the group's first
+ * sequence, the rest of a sequence through its own row.  A sequence shorter than its
+ * group's prefix attends its own tokens only; where the first sequence is shorter, the
+ * prefix ends there.  Query heads as in ia_prompt_shape: any number up to 64 per kv head.
+ * out: [batch, n_q_heads, D] contiguous, out_dtype; a sequence of no tokens gives zeros.
+ * Three launches: a plan from the device's lengths, the items, the merge.  The workspace
+ * (ia_shared_prefix_workspace_size bytes) needs no initialisation.  No counterpart in the
+ * reference, whose K/V is per sequence.
+ */
+IA_API size_t ia_shared_prefix_workspace_size(const ia_decode_shape* shape, int32_t kv_dtype, int32_t n_groups);
+IA_API int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, const ia_paged_kv* kv,
+                                   const int32_t* seq_lens, const int32_t* group_starts, const int32_t* shared_lens,
+                                   int32_t n_groups, float scale, void* out, int32_t out_dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 /* Most split-K items per (b, h) the two decode entry points use for the given
  * workload (the stride of the partials); size the decode workspace with it.
  * Tokens of ia_paged_decode past max_seq_len (rounded up to a 128-token tile) are

@@ -19,6 +19,6 @@ from .ops import (  # noqa: F401
     wait_fallbacks,
     workspace_tensor,
 )
-from .prompt import paged_prompt_attention, prompt_attention  # noqa: F401
+from .prompt import paged_prompt_attention, prompt_attention, shared_prefix_decode  # noqa: F401
 
 __version__ = "0.1.0"

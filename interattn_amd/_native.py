@@ -233,6 +233,10 @@ SIGNATURES = {
     "ia_paged_prompt_attention": (
         ctypes.c_int,
         [ctypes.POINTER(PromptShape), _P, ctypes.POINTER(PagedKV), _P, _P, _F, _P, _I32, _P, _SZ, _P]),
+    "ia_shared_prefix_workspace_size": (_SZ, [ctypes.POINTER(DecodeShape), _I32, _I32]),
+    "ia_shared_prefix_decode": (
+        ctypes.c_int,
+        [ctypes.POINTER(DecodeShape), _P, ctypes.POINTER(PagedKV), _P, _P, _P, _I32, _F, _P, _I32, _P, _SZ, _P]),
     "ia_sparse_max_items": (_I32, [_I32, _I32, _I32]),
     "ia_dense_max_items": (_I32, [_I32, _I32, _I32]),
 }

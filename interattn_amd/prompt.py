@@ -137,3 +137,45 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
            *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())))
     del keep
     return out
+
+
+def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *, scale=None,
+                         scales=None, out=None, out_dtype=None, workspace=None):
+    """Dense decode of a batch whose sequences share long prefixes: the result of
+    ``paged_decode``, each shared prefix's K/V read once for all sequences of its group.
+
+    ``q [batch, Hq, D]``; group g is the neighbouring sequences ``group_starts[g] ..
+    group_starts[g + 1] - 1`` (``[n_groups + 1] int32``, on the device), whose first
+    ``shared_lens[g]`` tokens (``[n_groups] int32``, any number, no multiple of a page
+    needed) are the same; sequences of no group share nothing.  The shared tokens are read
+    through the block-table row of the group's first sequence, the rest through each
+    sequence's own row, so forked tables (``fork_sequences``) and tables that repeat the
+    prefix in pages of their own give the same.  Any group of query heads up to 64; bf16,
+    float32 and fp8 pools."""
+    kv, keep = paged_kv(pool_k, pool_v, block_table, scales)
+    same_device(q, pool_k=pool_k, pool_v=pool_v, block_table=block_table, seq_lens=seq_lens,
+                group_starts=group_starts, shared_lens=shared_lens)
+    hkv, d = int(pool_k.shape[1]), int(pool_k.shape[3])
+    if q.dim() != 3 or q.stride(2) != 1 or q.dtype not in (_F32, _BF16) or q.shape[2] != d:
+        raise ValueError("q must be [batch, n_q_heads, D] float32 or bfloat16 with contiguous rows of the pool's D")
+    b, hq, _ = q.shape
+    if hkv <= 0 or hq <= 0 or hq % hkv:
+        raise ValueError("n_q_heads must be a multiple of n_kv_heads (grouped query attention)")
+    check_ints(seq_lens, "seq_lens", b)
+    check_ints(shared_lens, "shared_lens")
+    n_groups = int(shared_lens.shape[0])
+    check_ints(group_starts, "group_starts", n_groups + 1)
+    if block_table is not None and block_table.shape[0] != b:
+        raise ValueError("block_table rows must match the batch")
+    out = output(q, out, out_dtype, workspace, "attention_output")
+    shape = N.DecodeShape(b, hq, hkv, d, *_strides(q), _DTYPE_CODE[q.dtype])
+    key = ("shared_prefix_scratch", b, n_groups, hkv, hq, d, kv.dtype)
+    ws = None if workspace is None else workspace.get(key)
+    if ws is None or ws.device != q.device:
+        need = N.lib().ia_shared_prefix_workspace_size(shape, kv.dtype, n_groups)
+        ws = workspace_tensor(workspace, key, (max(need, 1),), device=q.device, dtype=torch.uint8)
+    launch(N.lib().ia_shared_prefix_decode, q, shape, q.data_ptr(), kv, seq_lens.data_ptr(), group_starts.data_ptr(),
+           shared_lens.data_ptr(), n_groups, d ** -0.5 if scale is None else float(scale), out.data_ptr(),
+           _DTYPE_CODE[out.dtype], ws.data_ptr(), ws.numel())
+    del keep
+    return out
