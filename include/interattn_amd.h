@@ -584,6 +584,97 @@ IA_API int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, 
                                    int32_t n_groups, float scale, void* out, int32_t out_dtype, void* workspace,
                                    size_t workspace_bytes, void* stream);
 
+/*
+ * The K/V rows of packed prompts into the paged pool: sequence b's rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (a device array [n_seq + 1] as for ia_prompt_attention) are
+ * written at positions seq_lens[b], seq_lens[b] + 1, ... through the block table, and
+ * new_seq_lens[b] (another array than seq_lens, so that ia_update_block_summaries can
+ * have both) receives the length after them.  The many-token form of ia_append_kv: bf16
+ * and f32 pools; a position whose page is not mapped (or past the table) is skipped, and
+ * the length counts up to the first such position.
+ */
+IA_API int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* rows, const int32_t* cu_seqlens,
+                               const int32_t* seq_lens, int32_t* new_seq_lens, int32_t n_seq, int32_t n_tokens,
+                               int32_t n_kv_heads, int32_t head_dim, void* stream);
+
+/*
+ * Pages of one tensor: page p starts at data + p * page_stride and holds n_outer x n_inner
+ * runs of run_bytes at the given strides (all in bytes, multiples of word_bytes: 16, or 4
+ * for small rows such as fp8 scales).  A K or V pool, or a scale array, of one layer.
+ */
+typedef struct ia_page_tensor {
+  void* data;
+  int64_t page_stride, outer_stride, inner_stride;
+  int32_t n_outer, n_inner, run_bytes, word_bytes;
+} ia_page_tensor;
+
+/*
+ * Who holds the pages of a cache, on the device: block_table [rows, cols] (row stride
+ * bt_stride, -1: no page), seq_lens [rows] and refs [n_pages], the number of table
+ * entries that hold each page (0: free; 16-byte aligned).  The calls below keep the three
+ * consistent; they allocate the lowest free pages, so the state after a call depends on
+ * the state before it alone.  One state's calls must be ordered (one stream).  No
+ * counterpart in the reference, which has no page pool.
+ */
+typedef struct ia_page_state {
+  int32_t* block_table;
+  int64_t bt_stride;
+  int32_t rows, cols;
+  int32_t* seq_lens;
+  int32_t* refs;
+  int64_t n_pages;
+  int32_t page_size;
+} ia_page_state;
+
+/*
+ * Page src[i] of every tensor copied to page dst[i] (device arrays [n]).  Pages outside
+ * [0, n_pages) are skipped.  No page may be in dst twice, or in src and dst.
+ */
+IA_API int ia_copy_pages(const ia_page_tensor* tensors, int32_t n_tensors, const int32_t* src, const int32_t* dst,
+                         int32_t n, int64_t n_pages, void* stream);
+
+/*
+ * Row dst[i] becomes a continuation of row src[i] (device arrays [n], n <= 8192): the
+ * source's whole pages are shared (their refs rise), the page its last tokens partly fill
+ * is copied, in every tensor, to the lowest free page, and the length is taken over, so
+ * both rows can be appended to.  Pages the source has reserved past its length stay its
+ * own.  ok[i] is 1, or 0 and row dst[i] as it was: where a row does not exist, dst[i] is
+ * not empty (length 0 and no page: ia_free_sequences) or listed before, src[i] is
+ * somewhere in dst or longer than its row, its last page is not mapped, or no page is
+ * free.  workspace: ia_fork_workspace_size bytes.
+ */
+IA_API size_t ia_fork_workspace_size(int32_t n);
+IA_API int ia_fork_sequences(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,
+                             const int32_t* src, const int32_t* dst, int32_t n, int32_t* ok, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Rows (device array [n]; a row listed twice is freed once, rows that do not exist are
+ * skipped) give up their pages: refs fall, entries become -1, lengths 0.
+ */
+IA_API int ia_free_sequences(const ia_page_state* state, const int32_t* rows, int32_t n, void* stream);
+
+/*
+ * Pages for the next new_tokens[row] tokens of every row (device array [rows]; 0 or less:
+ * none): each entry without a page in the pages they reach gets the lowest free page, rows
+ * in order.  ok[row] is 1, or 0 and the row as it was where its table row is too short or
+ * the pages left do not cover it (later rows are still served).  workspace:
+ * ia_reserve_workspace_size bytes.
+ */
+IA_API size_t ia_reserve_workspace_size(int32_t rows, int64_t n_pages);
+IA_API int ia_reserve_pages(const ia_page_state* state, const int32_t* new_tokens, int32_t* ok, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
+ * Live pages moved to the front of the pools: with n_live pages held, those at or past
+ * n_live move, in ascending order, to the free pages before it (in every tensor), and
+ * table and refs follow.  n_live (device, one entry) receives the count: pages past it are
+ * free afterwards.  seq_lens is not read (may be null).  workspace: ia_compact_workspace_size bytes.
+ */
+IA_API size_t ia_compact_workspace_size(int64_t n_pages);
+IA_API int ia_compact_pages(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,
+                            int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Most split-K items per (b, h) the two decode entry points use for the given
  * workload (the stride of the partials); size the decode workspace with it.
  * Tokens of ia_paged_decode past max_seq_len (rounded up to a 128-token tile) are

@@ -19,6 +19,12 @@ from .ops import (  # noqa: F401
     wait_fallbacks,
     workspace_tensor,
 )
-from .prompt import paged_prompt_attention, prompt_attention, shared_prefix_decode  # noqa: F401
+from .pages import copy_pages, compact_pages, fork_sequences, free_sequences, reserve_pages  # noqa: F401
+from .prompt import (  # noqa: F401
+    append_prompt_kv,
+    paged_prompt_attention,
+    prompt_attention,
+    shared_prefix_decode,
+)
 
 __version__ = "0.1.0"

@@ -144,6 +144,32 @@ class PackedKV(ctypes.Structure):
     ]
 
 
+class PageTensor(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64),
+        ("inner_stride", ctypes.c_int64),
+        ("n_outer", ctypes.c_int32),
+        ("n_inner", ctypes.c_int32),
+        ("run_bytes", ctypes.c_int32),
+        ("word_bytes", ctypes.c_int32),
+    ]
+
+
+class PageState(ctypes.Structure):
+    _fields_ = [
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("cols", ctypes.c_int32),
+        ("seq_lens", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -237,6 +263,20 @@ SIGNATURES = {
     "ia_shared_prefix_decode": (
         ctypes.c_int,
         [ctypes.POINTER(DecodeShape), _P, ctypes.POINTER(PagedKV), _P, _P, _P, _I32, _F, _P, _I32, _P, _SZ, _P]),
+    "ia_append_prompt_kv": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagedKV), ctypes.POINTER(PackedKV), _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "ia_copy_pages": (ctypes.c_int, [ctypes.POINTER(PageTensor), _I32, _P, _P, _I32, _I64, _P]),
+    "ia_fork_workspace_size": (_SZ, [_I32]),
+    "ia_fork_sequences": (
+        ctypes.c_int,
+        [ctypes.POINTER(PageState), ctypes.POINTER(PageTensor), _I32, _P, _P, _I32, _P, _P, _SZ, _P]),
+    "ia_free_sequences": (ctypes.c_int, [ctypes.POINTER(PageState), _P, _I32, _P]),
+    "ia_reserve_workspace_size": (_SZ, [_I32, _I64]),
+    "ia_reserve_pages": (ctypes.c_int, [ctypes.POINTER(PageState), _P, _P, _P, _SZ, _P]),
+    "ia_compact_workspace_size": (_SZ, [_I64]),
+    "ia_compact_pages": (
+        ctypes.c_int, [ctypes.POINTER(PageState), ctypes.POINTER(PageTensor), _I32, _P, _P, _SZ, _P]),
     "ia_sparse_max_items": (_I32, [_I32, _I32, _I32]),
     "ia_dense_max_items": (_I32, [_I32, _I32, _I32]),
 }

@@ -11,7 +11,7 @@ namespace ia {
 template <int D>
 __global__ __launch_bounds__(kArThreads) void ia_prompt_merge(PromptParams p) {
   const int head = blockIdx.x % p.ar.n_kv_heads, tile = blockIdx.x / p.ar.n_kv_heads;
-  const PromptTile t = prompt_tile(p, tile, threadIdx.x & 63);
+  const PackedTile t = prompt_tile(p, tile, threadIdx.x & 63);
   if (t.n_tok == 0) return;
   int limit0, k_end;
   prompt_keys(p, t, &limit0, &k_end);

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "attend_rows.hpp"
+#include "packed_rows.hpp"
 
 namespace ia {
 
@@ -31,43 +32,12 @@ int launch_prompt_bf16(const PromptParams& p, int d, hipStream_t st);
 int launch_prompt_f32(const PromptParams& p, int d, hipStream_t st);
 int launch_prompt_fp8(const PromptParams& p, int d, hipStream_t st);
 
-// A row tile of the packed batch.  Sequence b's tiles are numbered from cu[b] / T + b
-// (T tokens a tile): floor sums leave every sequence room for its own, so a workgroup
-// finds its sequence from cu alone, 64 candidates at a time, with no scan over the batch.
-struct PromptTile {
-  int b, tok0, n_tok;  // sequence, first token (of q), tokens; n_tok 0: no tile
-  int first, count;    // the sequence's first token and token count
-};
-
-__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int tile, int lane) {
-  PromptTile r{};
-  int lo = 0, len = p.n_seq;
-  auto cu = [&](int i) {
-    const int x = p.cu[i];
-    return x < 0 ? 0 : x > p.n_tokens ? p.n_tokens : x;
-  };
-  while (len > 1) {
-    const int step = (len + 63) / 64, i = lo + lane * step;
-    const bool in = lane * step < len;
-    const unsigned long long at = __ballot(in && cu(i) / p.tile_tokens + i <= tile);
-    const int n = at ? 64 - __builtin_clzll(at) : 1;  // the last candidate that starts at or before the tile
-    len = len - (n - 1) * step < step ? len - (n - 1) * step : step;
-    lo += (n - 1) * step;
-  }
-  const int c0 = cu(lo), c1 = cu(lo + 1);
-  r.b = lo;
-  r.first = c0;
-  r.count = c1 > c0 ? c1 - c0 : 0;
-  const int local = tile - (c0 / p.tile_tokens + lo);
-  const int64_t t0 = (int64_t)local * p.tile_tokens;
-  if (local < 0 || t0 >= r.count) return r;
-  r.tok0 = c0 + (int)t0;
-  r.n_tok = r.count - (int)t0 < p.tile_tokens ? r.count - (int)t0 : p.tile_tokens;
-  return r;
+__device__ __forceinline__ PackedTile prompt_tile(const PromptParams& p, int tile, int lane) {
+  return packed_tile(p.cu, p.n_seq, p.n_tokens, p.tile_tokens, tile, lane);
 }
 
 // keys the tile's last row sees, and the first row's limit
-__device__ __forceinline__ void prompt_keys(const PromptParams& p, const PromptTile& t, int* limit0, int* k_hi) {
+__device__ __forceinline__ void prompt_keys(const PromptParams& p, const PackedTile& t, int* limit0, int* k_hi) {
   int64_t total = t.count;
   if (p.seq_lens) total = p.seq_lens[t.b];
   const int64_t first = total - t.count + (t.tok0 - t.first) + 1;  // keys the tile's first token sees
@@ -86,7 +56,7 @@ __global__ __launch_bounds__(kArThreads, KV == kArF32 ? 1 : 2) void ia_prompt_at
   const int head = id % p.ar.n_kv_heads;
   id /= p.ar.n_kv_heads;
   const int slice = id % p.slices, tile = p.n_tiles - 1 - id / p.slices;
-  const PromptTile t = prompt_tile(p, tile, threadIdx.x & 63);
+  const PackedTile t = prompt_tile(p, tile, threadIdx.x & 63);
   if (t.n_tok == 0) return;
   ArItem it{};
   int k_end = 0;

@@ -139,6 +139,42 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     return out
 
 
+def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, *, new_seq_lens=None):
+    """Write the K/V rows of packed prompts (``k_new, v_new [tokens, Hkv, D]`` of the pool's
+    dtype, any token and head strides) into the pool: sequence b's rows go to positions
+    ``seq_lens[b], seq_lens[b] + 1, ...`` through the block table.  Returns the lengths
+    after it, ``[n_seq] int32`` (``new_seq_lens`` when given; never ``seq_lens`` itself, so
+    ``update_block_summaries`` can have both).  A position without a page is skipped and the
+    length counts up to the first of them.  The many-token form of ``append_kv``: bf16 and
+    float32 pools, capturable."""
+    kv, keep = paged_kv(pool_k, pool_v, block_table)
+    same_device(pool_k, pool_v=pool_v, block_table=block_table, seq_lens=seq_lens, k_new=k_new, v_new=v_new,
+                cu_seqlens=cu_seqlens, new_seq_lens=new_seq_lens)
+    check_ints(cu_seqlens, "cu_seqlens")
+    n_seq = int(cu_seqlens.shape[0]) - 1
+    if n_seq < 0:
+        raise ValueError("cu_seqlens must have n_seq + 1 entries")
+    check_ints(seq_lens, "seq_lens", n_seq)
+    hkv, d = int(pool_k.shape[1]), int(pool_k.shape[3])
+    for t in (k_new, v_new):
+        if t.dim() != 3 or tuple(t.shape[1:]) != (hkv, d) or t.stride(2) != 1 or t.dtype != pool_k.dtype:
+            raise ValueError("k_new/v_new must be [tokens, Hkv, D] of the pool dtype with contiguous rows")
+    if k_new.shape[0] != v_new.shape[0]:
+        raise ValueError("k_new and v_new must have the same tokens")
+    if block_table is not None and block_table.shape[0] != n_seq:
+        raise ValueError("block_table rows must match the sequences")
+    if new_seq_lens is None:
+        new_seq_lens = torch.empty_like(seq_lens)
+    check_ints(new_seq_lens, "new_seq_lens", n_seq)
+    if n_seq and abs(new_seq_lens.data_ptr() - seq_lens.data_ptr()) < 4 * n_seq:
+        raise ValueError("new_seq_lens must not overlap seq_lens")
+    rows = N.PackedKV(k_new.data_ptr(), v_new.data_ptr(), kv.dtype, *_strides(k_new), *_strides(v_new))
+    launch(N.lib().ia_append_prompt_kv, pool_k, kv, rows, cu_seqlens.data_ptr(), seq_lens.data_ptr(),
+           new_seq_lens.data_ptr(), n_seq, int(k_new.shape[0]), hkv, d)
+    del keep
+    return new_seq_lens
+
+
 def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *, scale=None,
                          scales=None, out=None, out_dtype=None, workspace=None):
     """Dense decode of a batch whose sequences share long prefixes: the result of
