@@ -574,9 +574,9 @@ IA_API int ia_paged_prompt_attention(const ia_prompt_shape* shape, const void* q
  * group's prefix attends its own tokens only; where the first sequence is shorter, the
  * prefix ends there.  Query heads as in ia_prompt_shape: any number up to 64 per kv head.
  * out: [batch, n_q_heads, D] contiguous, out_dtype; a sequence of no tokens gives zeros.
- * Three launches: a plan from the device's lengths, the items, the merge.  The workspace
- * (ia_shared_prefix_workspace_size bytes) needs no initialisation.  No counterpart in the
- * reference, whose K/V is per sequence.
+ * Two launches: the items, planned from the device's lengths, and their merge.  The
+ * workspace (ia_shared_prefix_workspace_size bytes) needs no initialisation.  No counterpart in
+ * the reference, whose K/V is per sequence.
  */
 IA_API size_t ia_shared_prefix_workspace_size(const ia_decode_shape* shape, int32_t kv_dtype, int32_t n_groups);
 IA_API int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, const ia_paged_kv* kv,

@@ -1,5 +1,5 @@
-// Shared-prefix decode, host side: argument checks, the plan that cuts the ranges into
-// items, dispatch to the per-type instances (shared_prefix_{bf16,f32,fp8}.hip), the merge.
+// Shared-prefix decode, host side: argument checks, dispatch to the per-type instances
+// (shared_prefix_{bf16,f32,fp8}.hip), and the merge.
 #include <algorithm>
 
 #include "shared_prefix.hpp"
@@ -7,177 +7,70 @@
 namespace ia {
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kMergeThreads = 512;
 
-__device__ __forceinline__ int group_start(const PrefixParams& p, int g) {
-  const int s = p.group_starts[g];
-  return s < 0 ? 0 : s > p.batch ? p.batch : s;
-}
-
-__device__ __forceinline__ int seq_len(const PrefixParams& p, int b) {
-  const int n = p.seq_lens[b];
-  return n < 0 ? 0 : n > p.kv_cap ? (int)p.kv_cap : n;
-}
-
-// tokens group g's prefix pass covers: as many as its first sequence, whose pages it reads,
-// has.  A group of one shares with nobody: its tokens are all its own range.
-__device__ __forceinline__ int group_shared(const PrefixParams& p, int g) {
-  const int s0 = group_start(p, g), s1 = group_start(p, g + 1);
-  if (s1 - s0 < 2) return 0;
-  const int n = p.shared_lens[g], have = seq_len(p, s0);
-  return n < 0 ? 0 : n < have ? n : have;
-}
-
-// the last group that starts at or before sequence b, where b lies in it; else -1
-__device__ __forceinline__ int group_of(const PrefixParams& p, int b) {
-  int lo = 0, hi = p.n_groups;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (group_start(p, mid) <= b) lo = mid + 1; else hi = mid;
-  }
-  const int g = lo - 1;
-  return g >= 0 && b < group_start(p, g + 1) ? g : -1;
-}
-
-struct Range {
-  int tok0, n_tok, k_lo, k_hi, table_seq;
-};
-
-// entry e: a row tile of a group's prefix (e < n_tiles) or a sequence's own tokens
-__device__ __forceinline__ Range plan_range(const PrefixParams& p, int e) {
-  Range r{};
-  if (e >= p.n_tiles) {
-    const int b = e - p.n_tiles, g = group_of(p, b);
-    r.tok0 = r.table_seq = b;
-    r.n_tok = 1;
-    r.k_lo = g < 0 ? 0 : group_shared(p, g);
-    r.k_hi = seq_len(p, b);
-    return r;
-  }
-  int lo = 0, hi = p.n_groups;  // the last group whose tiles start at or before e
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (group_start(p, mid) / p.tile_seqs + mid <= e) lo = mid + 1; else hi = mid;
-  }
-  const int g = lo - 1;
-  if (g < 0) return r;
-  const int s0 = group_start(p, g), s1 = group_start(p, g + 1);
-  const int64_t at = s0 + (int64_t)(e - (s0 / p.tile_seqs + g)) * p.tile_seqs;
-  if (at >= s1) return r;
-  r.tok0 = (int)at;
-  r.n_tok = s1 - (int)at < p.tile_seqs ? s1 - (int)at : p.tile_seqs;
-  r.k_hi = group_shared(p, g);
-  r.table_seq = s0;
-  return r;
-}
-
-__device__ __forceinline__ int range_tiles(const Range& r) {
-  return r.n_tok == 0 || r.k_hi <= r.k_lo ? 0 : (r.k_hi - (r.k_lo & ~15) + kArTile - 1) / kArTile;
-}
-
-// Cuts the ranges into items of at most `cut` key tiles, cut = all tiles over the items the
-// device runs at once.  One workgroup: a batch has few ranges.
-__global__ __launch_bounds__(kPlanThreads) void ia_shared_prefix_plan(PrefixParams p) {
-  __shared__ int wave_a[kPlanThreads / 64], wave_b[kPlanThreads / 64];
-  __shared__ long long total;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = p.n_tiles + p.batch;
-  if (tid == 0) total = 0;
-  __syncthreads();
-  long long mine = 0;
-  for (int e = tid; e < n; e += kPlanThreads) mine += range_tiles(plan_range(p, e));
-  for (int s = 32; s > 0; s >>= 1) mine += __shfl_xor(mine, s, 64);
-  if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&total), (unsigned long long)mine);
-  __syncthreads();
-  long long cut = (total + p.target - 1) / p.target;
-  if (cut < kPrefixMinTiles) cut = kPrefixMinTiles;
-  int base = 0, slot = 0;
-  for (int e0 = 0; e0 < n; e0 += kPlanThreads) {
-    const int e = e0 + tid;
-    Range r{};
-    int tiles = 0;
-    if (e < n) {
-      r = plan_range(p, e);
-      tiles = range_tiles(r);
-    }
-    const int items = (int)((tiles + cut - 1) / cut), rows = r.n_tok * p.ar.group;
-    const int ia = wave_inclusive_scan(items), ib = wave_inclusive_scan(items * rows);
-    if (lane == 63) {
-      wave_a[wave] = ia;
-      wave_b[wave] = ib;
-    }
-    __syncthreads();
-    int at = base + ia - items, row = slot + ib - items * rows;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wave) {
-        at += wave_a[w];
-        row += wave_b[w];
-      }
-      base += wave_a[w];
-      slot += wave_b[w];
-    }
-    if (e < n) {
-      p.entries[e] = PrefixEntry{row, items, rows, 0};
-      if (e >= p.n_tiles) {
-        const int b = e - p.n_tiles, g = group_of(p, b);
-        int t = -1;
-        if (g >= 0) {
-          const int s0 = group_start(p, g);
-          t = s0 / p.tile_seqs + g + (b - s0) / p.tile_seqs;
-        }
-        p.tile_of[b] = t < p.n_tiles ? t : -1;
-      }
-      const int per = items ? (tiles + items - 1) / items : 0, tb = r.k_lo & ~15;
-      for (int i = 0; i < items; ++i) {
-        const int lo = tb + i * per * kArTile, hi = lo + per * kArTile;
-        if (at + i < p.max_items)
-          p.items[at + i] = PrefixItem{r.tok0, r.n_tok, lo < r.k_lo ? r.k_lo : lo, hi < r.k_hi ? hi : r.k_hi,
-                                       r.table_seq, row + i * rows, 0, 0};
-      }
-    }
-    __syncthreads();
-  }
-  if (tid == 0) *p.n_items = base < p.max_items ? base : p.max_items;
-}
-
-// One workgroup per (sequence, kv head): its rows' partials, prefix first.
+// One workgroup per (sequence, kv head): its rows' partials, prefix first.  A row's partials
+// are dealt to the thread groups of D / 4 that share it, so a sequence of few heads still
+// has every partial's load in flight at once; the groups' sums meet in LDS in order.
 template <int D>
-__global__ __launch_bounds__(kArThreads) void ia_shared_prefix_merge(PrefixParams p) {
+__global__ __launch_bounds__(kMergeThreads) void ia_shared_prefix_merge(PrefixParams p) {
+  constexpr int kCols = D / 4, kGroups = kMergeThreads / kCols;
+  __shared__ f32x4_t acc[kGroups][kCols];
+  __shared__ float sum_l[kGroups];
   const int b = blockIdx.x / p.ar.n_kv_heads, head = blockIdx.x % p.ar.n_kv_heads;
-  const int tile = p.tile_of[b];
-  PrefixEntry pre{}, own = p.entries[p.n_tiles + b];
+  const PrefixGroups gr{p, nullptr, nullptr};
+  const PrefixEntry own = p.entries[p.n_tiles + b];
+  PrefixEntry pre{};
   int in_tile = 0;  // the sequence's first row in its tile's partials
-  if (tile >= 0) {
-    pre = p.entries[tile];
-    in_tile = (b - group_start(p, group_of(p, b))) % p.tile_seqs * p.ar.group;
+  const int g = p.n_groups ? gr.of(b) : -1;
+  if (g >= 0) {
+    const int s0 = gr.start(g), tile = s0 / p.tile_seqs + g + (b - s0) / p.tile_seqs;
+    if (tile < p.n_tiles) pre = p.entries[tile];
+    in_tile = (b - s0) % p.tile_seqs * p.ar.group;
     if (in_tile + p.ar.group > pre.rows) pre.n = 0;  // (starts that decrease)
   }
   const int64_t base = (int64_t)head * p.rows;
   ArItem it{};
   it.head = head;
   it.tok0 = b;
-  const int n = pre.n + own.n;
-  for (int i = threadIdx.x; i < p.ar.group * (D / 4); i += kArThreads) {
-    const int r = i / (D / 4), e = (i % (D / 4)) * 4;
+  const int n = pre.n + own.n, per_row = kGroups / p.ar.group > 0 ? kGroups / p.ar.group : 1;
+  const int grp = threadIdx.x / kCols, col = threadIdx.x % kCols, part = grp % per_row;
+  const int at_once = kGroups / per_row;
+  for (int r0 = 0; r0 < p.ar.group; r0 += at_once) {
+    const int r = r0 + grp / per_row;
+    const bool live = r < p.ar.group && grp < at_once * per_row;
     auto at = [&](int s) {
       return base + (s < pre.n ? pre.slot + s * pre.rows + in_tile + r : own.slot + (s - pre.n) * own.rows + r);
     };
-    float m = kNegInf;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[2 * at(s)]);
-    const float mu = m == kNegInf ? 0.f : m;
-    float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
-      const int64_t row = at(s);
-      const float a = __builtin_amdgcn_exp2f(p.part_ml[2 * row] - mu);
-      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + row * D + e);
-      l += a * p.part_ml[2 * row + 1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += a * y[j];
+    float m = kNegInf, l = 0.f;
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+#pragma unroll 8
+      for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[2 * at(s)]);
+      const float mu = m == kNegInf ? 0.f : m;
+#pragma unroll 4
+      for (int s = part; s < n; s += per_row) {
+        const int64_t row = at(s);
+        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(p.part_ml + 2 * row);
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + row * D + 4 * col);
+        const float a = __builtin_amdgcn_exp2f(ml[0] - mu);
+        l += a * ml[1];
+        x += a * y;
+      }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] *= inv;
-    ar_store4(p.ar, ar_out_row(p.ar, it, r, D) + e, x);
+    __syncthreads();  // (the last round's sums have been read)
+    acc[grp][col] = x;
+    if (col == 0) sum_l[grp] = l;
+    __syncthreads();
+    if (live && part == 0) {
+      for (int s = 1; s < per_row; ++s) {
+        x += acc[grp + s][col];
+        l += sum_l[grp + s];
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+      ar_store4(p.ar, ar_out_row(p.ar, it, r, D) + 4 * col, y);
+    }
   }
 }
 
@@ -190,7 +83,7 @@ int check_prefix_shape(const ia_decode_shape* s, int n_groups) {
   if (s->n_q_heads / s->n_kv_heads > kArMaxGroup)
     return fail(IA_ERR_UNSUPPORTED, "GQA group size must not exceed " + std::to_string(kArMaxGroup));
   if (s->head_dim != 64 && s->head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
-  if ((int64_t)s->batch + n_groups > 1 << 20) return fail(IA_ERR_UNSUPPORTED, "batch too large for one plan");
+  if ((int64_t)s->batch + n_groups > 1 << 20) return fail(IA_ERR_UNSUPPORTED, "batch too large");
   return check_ar_q(s->q_dtype, s->q_batch_stride, s->q_row_stride);
 }
 
@@ -212,10 +105,7 @@ size_t prefix_layout(const ia_decode_shape* s, int kv_dtype, int n_groups, Prefi
     at += align_up(bytes, 256);
     return x;
   };
-  p->n_items = reinterpret_cast<int32_t*>(take(4));
-  p->items = reinterpret_cast<PrefixItem*>(take(sizeof(PrefixItem) * p->max_items));
   p->entries = reinterpret_cast<PrefixEntry*>(take(sizeof(PrefixEntry) * (p->n_tiles + (size_t)s->batch)));
-  p->tile_of = reinterpret_cast<int32_t*>(take(4 * (size_t)s->batch));
   p->part_ml = reinterpret_cast<float*>(take(8 * (size_t)p->rows * s->n_kv_heads));
   p->part_acc = reinterpret_cast<float*>(take(4 * (size_t)p->rows * s->n_kv_heads * s->head_dim));
   return at;
@@ -259,18 +149,15 @@ int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, const i
   if ((int64_t)p.max_items * shape->n_kv_heads >= (int64_t)1 << 31 || p.rows >= (int64_t)1 << 31)
     return fail(IA_ERR_UNSUPPORTED, "batch too large for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(ia_shared_prefix_plan, dim3(1), dim3(kPlanThreads), 0, st, p);
-  rc = check_launch("shared-prefix plan");
-  if (rc) return rc;
   const int d = shape->head_dim;
   rc = kv->dtype == IA_BF16 ? launch_prefix_bf16(p, d, st)
                             : kv->dtype == IA_F32 ? launch_prefix_f32(p, d, st) : launch_prefix_fp8(p, d, st);
   if (rc) return rc;
   const dim3 grid((unsigned)shape->batch * shape->n_kv_heads);
   if (d == 128)
-    hipLaunchKernelGGL((ia_shared_prefix_merge<128>), grid, dim3(kArThreads), 0, st, p);
+    hipLaunchKernelGGL((ia_shared_prefix_merge<128>), grid, dim3(kMergeThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((ia_shared_prefix_merge<64>), grid, dim3(kArThreads), 0, st, p);
+    hipLaunchKernelGGL((ia_shared_prefix_merge<64>), grid, dim3(kMergeThreads), 0, st, p);
   return check_launch("shared-prefix merge");
 }
 
