@@ -32,6 +32,7 @@ constexpr int kArThreads = 256;   // four waves
 constexpr int kArRows = 128;      // rows of a wide workgroup
 constexpr int kArNarrow = 32;     // most rows of a narrow one
 constexpr int kArMaxGroup = 64;   // query heads per kv head: a row tile holds at least two tokens
+constexpr int64_t kArMaxGrid = 1 << 23;  // workgroups of a launch (work items are 32 bits)
 constexpr float kArSlack = 8.f;   // log2 units a row's maximum may rise before it is rescaled
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
@@ -131,10 +132,13 @@ struct ArLoader {
   using S = ArShape<KV, D>;
   const ArSource& kv;
   const ArItem& it;
-  const char* kb;
-  const char* vb;
   int lane, wave, tid;
-  int page, in_page;       // group lane & 3 of the tile to be loaded next
+  int page;                // group lane & 3 of the tile to be loaded next: its page, and
+  int64_t k_grp, v_grp;    // where its first rows are
+  // a lane's row and chunk within the 16 rows of a group (two forms where a round of loads
+  // covers half a group): the rest of an address is the same in every lane
+  static constexpr int kForms = S::kLoadRows < 16 ? 2 : 1;
+  int64_t k_lane[kForms], v_lane[kForms];
   float ks, vs;            // fp8: its scales, of the tile last issued
   u32x4_t kr[KV == kArFp8 ? S::kLoads : 1], vr[KV == kArFp8 ? S::kLoads : 1];
 
@@ -142,9 +146,14 @@ struct ArLoader {
     tid = threadIdx.x;
     lane = tid & 63;
     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    kb = kv.k + it.head * kv.k_head + it.row0 * kv.k_tok;
-    vb = kv.v + it.head * kv.v_head + it.row0 * kv.v_tok;
     ks = vs = 0.f;
+#pragma unroll
+    for (int f = 0; f < kForms; ++f) {
+      const int row = (tid / S::kSrcChunks + f * S::kLoadRows) & 15, slot = tid % S::kSrcChunks;
+      const int chunk = KV == kArFp8 ? slot : slot ^ ar_swizzle<KV, D>(row);
+      k_lane[f] = row * kv.k_tok + chunk * 16;
+      v_lane[f] = row * kv.v_tok + chunk * 16;
+    }
   }
 
   __device__ __forceinline__ void fetch_pages(int tb) {
@@ -158,7 +167,12 @@ struct ArLoader {
       if (pg >= kv.n_pages) pg = -1;
     }
     page = pg;
-    in_page = in;
+    k_grp = reinterpret_cast<int64_t>(kv.k) + it.head * kv.k_head + (it.row0 + in) * kv.k_tok + pg * kv.k_page;
+    v_grp = reinterpret_cast<int64_t>(kv.v) + it.head * kv.v_head + (it.row0 + in) * kv.v_tok + pg * kv.v_page;
+  }
+  static __device__ __forceinline__ int64_t lane_i64(int64_t x, int l) {
+    const u32 lo = __builtin_amdgcn_readlane((u32)x, l), hi = __builtin_amdgcn_readlane((u32)((unsigned long long)x >> 32), l);
+    return (int64_t)(((unsigned long long)hi << 32) | lo);
   }
 
   // keys of the tile at tb that exist: in range, on a valid page
@@ -166,35 +180,42 @@ struct ArLoader {
     return tb >= it.k_lo && tb + kArTile <= it.k_hi && __ballot(page < 0) == 0;
   }
 
-  // Start the loads of the tile at tb (its pages fetched) into stage `smem`.  Keys that do
-  // not exist get V rows of zeros: their P is 0, and 0 * garbage must not become NaN.
-  __device__ __forceinline__ void issue(int tb, char* smem) {
-    const bool all = whole(tb);
+  template <bool WHOLE>
+  __device__ __forceinline__ void issue_rows(int tb, char* smem) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
       const int row = i * S::kLoadRows + tid / S::kSrcChunks;
       const int grp = __builtin_amdgcn_readfirstlane(row >> 4);
+      // (lane reads before the lanes part ways)
       const int pg = __builtin_amdgcn_readlane(page, grp);
-      const int in = __builtin_amdgcn_readlane(in_page, grp) + (row & 15);
-      const int slot = tid % S::kSrcChunks;
-      const bool live = all || (pg >= 0 && tb + row >= it.k_lo && tb + row < it.k_hi);
+      const char* k_row = reinterpret_cast<const char*>(lane_i64(k_grp, grp) + k_lane[i % kForms]);
+      const char* v_row = reinterpret_cast<const char*>(lane_i64(v_grp, grp) + v_lane[i % kForms]);
+      const bool live = WHOLE || (pg >= 0 && tb + row >= it.k_lo && tb + row < it.k_hi);
       if constexpr (KV == kArFp8) {
         kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
         if (live) {
-          kr[i] = *reinterpret_cast<const u32x4_t*>(kb + (int64_t)pg * kv.k_page + (int64_t)in * kv.k_tok + slot * 16);
-          vr[i] = *reinterpret_cast<const u32x4_t*>(vb + (int64_t)pg * kv.v_page + (int64_t)in * kv.v_tok + slot * 16);
+          kr[i] = *reinterpret_cast<const u32x4_t*>(k_row);
+          vr[i] = *reinterpret_cast<const u32x4_t*>(v_row);
         }
       } else {
-        const int chunk = slot ^ ar_swizzle<KV, D>(row);
         const u32 dst = lds_addr(smem) + (i * 4 + wave) * 1024;
         if (live) {
-          ar_dma16(kb + (int64_t)pg * kv.k_page + (int64_t)in * kv.k_tok + chunk * 16, dst);
-          ar_dma16(vb + (int64_t)pg * kv.v_page + (int64_t)in * kv.v_tok + chunk * 16, dst + S::kTileBytes);
+          ar_dma16(k_row, dst);
+          ar_dma16(v_row, dst + S::kTileBytes);
         } else {
           *reinterpret_cast<u32x4_t*>(smem + S::kTileBytes + (i * kArThreads + tid) * 16) = u32x4_t{0, 0, 0, 0};
         }
       }
     }
+  }
+
+  // Start the loads of the tile at tb (its pages fetched) into stage `smem`.  Keys that do
+  // not exist get V rows of zeros: their P is 0, and 0 * garbage must not become NaN.
+  __device__ __forceinline__ void issue(int tb, char* smem) {
+    if (whole(tb))
+      issue_rows<true>(tb, smem);
+    else
+      issue_rows<false>(tb, smem);
     if constexpr (KV == kArFp8) {
       ks = vs = 0.f;
       if (page >= 0) {
@@ -459,20 +480,49 @@ __device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, cha
       const char* vt = cur + S::kTileBytes;
       f32x16_t s[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+      if constexpr (KV == kArF32) {
 #pragma unroll
-        for (int q = 0; q < kQ; ++q) {
-          const char* a = kt + kb * 32 * S::kRowBytes + k_off + (((2 * q) ^ fk) << 4);
-          if constexpr (KV == kArF32) {
-            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a);
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int q = 0; q < kQ; ++q) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(kt + kb * 32 * S::kRowBytes + k_off + (((2 * q) ^ fk) << 4));
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[q][e], s[kb], 0, 0, 0);
-          } else {
-            s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(a), qb[q], s[kb], 0, 0, 0);
           }
+      } else {
+        // The key operands of 32 keys are read before their products, the next 32 keys'
+        // behind them: left to itself the compiler reads, waits and multiplies one by one.
+        bf16x8_t ka[kQ], kc[kQ];
+        const char* a = kt + k_off;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) ka[q] = *reinterpret_cast<const bf16x8_t*>(a + (((2 * q) ^ fk) << 4));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q)
+          kc[q] = *reinterpret_cast<const bf16x8_t*>(a + 32 * S::kRowBytes + (((2 * q) ^ fk) << 4));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[q], qb[q], s[0], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kc[q], qb[q], s[1], 0, 0, 0);
+      }
+      // V operands, 16 keys at a time: the first are on their way during the softmax, the
+      // next during the products of the ones before
+      u32x2_t v[2][kDb][2];
+      auto read_v = [&](int g) {
+        const char* a = vt + v_off + 16 * g * S::kRowBytes;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d) {
+          v[g & 1][d][0] = ar_read_tr(a + (((4 * d) ^ vc0) << 4));
+          v[g & 1][d][1] = ar_read_tr(a + 8 * S::kRowBytes + (((4 * d) ^ 2 ^ vc0) << 4));
         }
+      };
+      if constexpr (KV != kArF32) {
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (KV == kArFp8) {
 #pragma unroll
@@ -554,16 +604,15 @@ __device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, cha
       } else {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
+          if (g < 3) read_v(g + 1);
           u32 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(s[g >> 1][8 * (g & 1) + 2 * j], s[g >> 1][8 * (g & 1) + 2 * j + 1]);
           const bf16x8_t pb = as_bf16x8(w);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int d = 0; d < kDb; ++d) {
-            const char* a = vt + v_off + 16 * g * S::kRowBytes;
-            const u32x2_t lo = ar_read_tr(a + (((4 * d) ^ vc0) << 4));
-            const u32x2_t hi = ar_read_tr(a + 8 * S::kRowBytes + (((4 * d) ^ 2 ^ vc0) << 4));
-            const u32 va[4] = {lo[0], lo[1], hi[0], hi[1]};
+            const u32 va[4] = {v[g & 1][d][0][0], v[g & 1][d][0][1], v[g & 1][d][1][0], v[g & 1][d][1][1]};
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(va), pb, o[d], 0, 0, 0);
           }
         }

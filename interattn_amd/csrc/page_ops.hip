@@ -19,6 +19,7 @@ namespace {
 constexpr int kCopyThreads = 256;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kListMax = 1 << 23;  // entries of a list that has a workgroup for each
 constexpr int kForkMax = 8192;   // forks of one call (the plan compares them pairwise)
 constexpr int kMaxTensors = 48;  // of one launch (kernel arguments)
 
@@ -460,7 +461,8 @@ int ia_copy_pages(const ia_page_tensor* tensors, int32_t n_tensors, const int32_
   using namespace ia;
   int rc = check_tensors(tensors, n_tensors);
   if (rc) return rc;
-  if (n < 0 || n_pages < 0 || n_pages > INT32_MAX || (n && (!src || !dst))) return fail(IA_ERR_INVALID, "page lists");
+  if (n < 0 || n >= kListMax || n_pages < 0 || n_pages > INT32_MAX || (n && (!src || !dst)))
+    return fail(IA_ERR_INVALID, "page lists");
   if (n == 0) return IA_OK;
   for (int at = 0; at < n_tensors; at += kMaxTensors) {
     const Tensors ts = some_tensors(tensors, n_tensors, at);
@@ -508,7 +510,7 @@ int ia_free_sequences(const ia_page_state* state, const int32_t* rows, int32_t n
   Table t;
   int rc = check_state(state, &t);
   if (rc) return rc;
-  if (n < 0 || (n && !rows)) return fail(IA_ERR_INVALID, "row list");
+  if (n < 0 || n >= kListMax || (n && !rows)) return fail(IA_ERR_INVALID, "row list");
   if (n == 0) return IA_OK;
   hipLaunchKernelGGL(ia_free_rows, dim3(n), dim3(kCopyThreads), 0, static_cast<hipStream_t>(stream), t, rows, n);
   return check_launch("free sequences");

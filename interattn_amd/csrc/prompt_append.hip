@@ -150,7 +150,7 @@ extern "C" int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* ro
   p.chunks = head_dim * eb / 16;
   p.tile = kAppendThreads / p.chunks;
   const int64_t tiles = (int64_t)n_tokens / p.tile + n_seq;
-  if (tiles >= (int64_t)1 << 31) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
   // few tiles: a workgroup per head, so that a short prompt is one round trip
   p.heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
   const dim3 grid((unsigned)tiles, (unsigned)((n_kv_heads + p.heads_per_wg - 1) / p.heads_per_wg));

@@ -25,13 +25,13 @@ __global__ __launch_bounds__(kArThreads) void ia_prompt_merge(PromptParams p) {
   for (int i = threadIdx.x; i < rows * (D / 4); i += kArThreads) {
     const int r = i / (D / 4), e = (i % (D / 4)) * 4;
     float m = kNegInf;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[(slot + s) * (2 * kArRows) + 2 * r]);
+    for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[((slot + s) * p.tile_rows + r) * 2]);
     const float mu = m == kNegInf ? 0.f : m;
     float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < n; ++s) {
-      const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(p.part_ml + (slot + s) * (2 * kArRows) + 2 * r);
+      const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(p.part_ml + ((slot + s) * p.tile_rows + r) * 2);
       const float a = __builtin_amdgcn_exp2f(ml[0] - mu);
-      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + ((slot + s) * kArRows + r) * (int64_t)D + e);
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + ((slot + s) * p.tile_rows + r) * D + e);
       l += a * ml[1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] += a * y[j];
@@ -59,26 +59,38 @@ int check_prompt_shape(const ia_prompt_shape* s) {
   return check_ar_q(s->q_dtype, s->q_token_stride, s->q_head_stride);
 }
 
-// Row tiles (a bound from the token and sequence counts alone) and the slices their keys
-// may be cut into: as many as keep the device's resident workgroups busy.
 int64_t resident_wgs(int kv_dtype) { return (int64_t)device_cus() * (kv_dtype == IA_F32 ? 1 : 2); }
 
+// Row tiles (a bound from the token and sequence counts alone), and the slices their keys
+// may be cut into.  Tiles of 128 rows read K/V least often and keep the matrix cores
+// busiest; a launch whose tiles of 32 rows all run at once takes those, for a quarter of
+// the products on each row's way (float32 products are as dense in both, and a tile of 128
+// rows holds one of 32's four waves as long: always 32).  Then, with fewer tiles than
+// workgroups run at once, every tile is cut along its keys to fill the device.
 void prompt_grid(const ia_prompt_shape* s, int kv_dtype, int64_t most_keys, PromptParams* p) {
   const int group = s->n_q_heads / s->n_kv_heads;
-  p->tile_tokens = kArRows / group;
-  p->n_tiles = s->n_tokens / p->tile_tokens + s->n_seq;
   const int64_t resident = resident_wgs(kv_dtype);
-  const int64_t items = std::max<int64_t>(1, (int64_t)p->n_tiles * s->n_kv_heads);
-  int64_t n = std::min<int64_t>(resident / items, kPromptMaxSlices);
+  // about how many tiles of `rows` rows: half a tile lost per sequence
+  auto about = [&](int rows) {
+    return ((int64_t)s->n_tokens / (rows / group) + (s->n_seq + 1) / 2) * s->n_kv_heads;
+  };
+  p->tile_rows = group <= kArNarrow && (kv_dtype == IA_F32 || about(kArNarrow) <= resident) ? kArNarrow : kArRows;
+  p->tile_tokens = p->tile_rows / group;
+  p->n_tiles = (int)std::min<int64_t>((int64_t)s->n_tokens / p->tile_tokens + s->n_seq, INT32_MAX);
+  const int64_t tiles = std::max<int64_t>(1, about(p->tile_rows));
+  const int64_t bound = std::max<int64_t>(1, (int64_t)p->n_tiles * s->n_kv_heads);
+  int64_t n = 5 * resident >= 6 * tiles ? (resident + tiles - 1) / tiles : 1;  // (a cut for less than a fifth costs more)
+  n = std::min<int64_t>(n, kPromptMaxSlices);
+  n = std::min<int64_t>(n, 2 * resident / bound);
   n = std::min<int64_t>(n, (most_keys + kPromptSliceTiles * kArTile - 1) / (kPromptSliceTiles * kArTile));
   p->slices = (int)std::max<int64_t>(1, n);
 }
 
-// One size for every call that cuts (a cut call has at most one slice per resident
+// One size for every call that cuts (a cut call has at most two slices per resident
 // workgroup), so a buffer kept from call to call never has to be replaced by a larger one
 // while a captured graph still uses it.
 size_t prompt_ws_size(const ia_prompt_shape* s, int kv_dtype, const PromptParams& p) {
-  return p.slices <= 1 ? 0 : (size_t)resident_wgs(kv_dtype) * kArRows * (s->head_dim + 2) * 4;
+  return p.slices <= 1 ? 0 : (size_t)(2 * resident_wgs(kv_dtype)) * kArRows * (s->head_dim + 2) * 4;
 }
 
 int run_prompt(const ia_prompt_shape* s, const void* q, int kv_dtype, PromptParams& p, const int32_t* cu, float scale,
@@ -93,14 +105,14 @@ int run_prompt(const ia_prompt_shape* s, const void* q, int kv_dtype, PromptPara
   p.n_seq = s->n_seq;
   p.n_tokens = s->n_tokens;
   prompt_grid(s, kv_dtype, most_keys, &p);
-  if ((int64_t)p.n_tiles * s->n_kv_heads * p.slices >= (int64_t)1 << 31)
+  if ((int64_t)p.n_tiles * s->n_kv_heads * p.slices >= kArMaxGrid)
     return fail(IA_ERR_UNSUPPORTED, "too many row tiles for one launch");
   const size_t need = prompt_ws_size(s, kv_dtype, p);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(IA_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned: " + std::to_string(need) +
                                       " bytes needed");
   p.part_acc = reinterpret_cast<float*>(workspace);
-  if (need) p.part_ml = p.part_acc + (size_t)p.n_tiles * s->n_kv_heads * p.slices * kArRows * s->head_dim;
+  if (need) p.part_ml = p.part_acc + (size_t)p.n_tiles * s->n_kv_heads * p.slices * p.tile_rows * s->head_dim;
   const int d = s->head_dim;
   rc = kv_dtype == IA_BF16 ? launch_prompt_bf16(p, d, st)
                            : kv_dtype == IA_F32 ? launch_prompt_f32(p, d, st) : launch_prompt_fp8(p, d, st);

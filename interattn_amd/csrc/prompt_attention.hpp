@@ -13,7 +13,8 @@ struct PromptParams {
   const int32_t* seq_lens;  // paged: [n_seq] keys of each sequence; null: its own tokens
   int64_t kv_cap;           // paged: keys a block-table row can hold
   int32_t n_seq, n_tokens;
-  int32_t tile_tokens;      // tokens of a row tile (128 / group)
+  int32_t tile_rows;        // rows of a row tile: 128 or 32
+  int32_t tile_tokens;      // its tokens, tile_rows / group
   int32_t n_tiles;          // bound over all sequences
   int32_t slices;           // most key slices of a row tile
   float* part_ml;
@@ -74,8 +75,8 @@ __global__ __launch_bounds__(kArThreads, KV == kArF32 ? 1 : 2) void ia_prompt_at
   it.n_rows = t.n_tok * p.ar.group;
   if (n > 1) {
     const int64_t slot = ((int64_t)tile * p.ar.n_kv_heads + head) * p.slices + slice;
-    it.part_ml = p.part_ml + slot * (2 * kArRows);
-    it.part_acc = p.part_acc + slot * (kArRows * (int64_t)D);
+    it.part_ml = p.part_ml + slot * p.tile_rows * 2;
+    it.part_acc = p.part_acc + slot * p.tile_rows * D;
   }
   ar_attend<KV, D>(p.ar, it, smem);
 }

@@ -92,7 +92,8 @@ size_t prefix_layout(const ia_decode_shape* s, int kv_dtype, int n_groups, Prefi
   const int group = s->n_q_heads / s->n_kv_heads;
   p->batch = s->batch;
   p->n_groups = n_groups;
-  p->tile_seqs = kArRows / group;
+  // float32 products are as dense in tiles of 32 rows, which spread over four times the waves
+  p->tile_seqs = (kv_dtype == IA_F32 && group <= kArNarrow ? kArNarrow : kArRows) / group;
   p->n_tiles = n_groups ? s->batch / p->tile_seqs + n_groups : 0;
   const int resident = device_cus() * (kv_dtype == IA_F32 ? 1 : 2);
   p->target = std::max(1, resident / s->n_kv_heads);
@@ -146,7 +147,7 @@ int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, const i
   p.seq_lens = seq_lens;
   p.group_starts = group_starts;
   p.shared_lens = shared_lens;
-  if ((int64_t)p.max_items * shape->n_kv_heads >= (int64_t)1 << 31 || p.rows >= (int64_t)1 << 31)
+  if ((int64_t)p.max_items * shape->n_kv_heads >= kArMaxGrid || p.rows >= (int64_t)1 << 31)
     return fail(IA_ERR_UNSUPPORTED, "batch too large for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int d = shape->head_dim;
