@@ -17,7 +17,7 @@ import torch
 
 from . import _native as N
 from .ops import workspace_tensor
-from .prompt import check_ints, launch, same_device
+from .prompt import check_ints, device_of, launch
 
 
 @functools.lru_cache(maxsize=512)
@@ -48,61 +48,68 @@ def _page_layout(shape, stride, itemsize):
     return size[0], size[1], size[2], n_outer, n_inner, size[3], word
 
 
-def _page_tensors(tensors, n_pages):
-    tensors = list(tensors)
-    out = (N.PageTensor * max(len(tensors), 1))()
-    for d, t in zip(out, tensors):
-        shape = t.shape
-        if len(shape) < 2 or (n_pages is not None and shape[0] != n_pages):
-            raise ValueError(f"page tensors must be [n_pages, ...] with {n_pages} pages")
-        at, lay = t.data_ptr(), _page_layout(shape, t.stride(), t.element_size())
-        if at % lay[6]:
-            if at % 4:
-                raise ValueError("pages must be 4-byte aligned")
-            lay = lay[:6] + (4,)
-        (d.data, d.page_stride, d.outer_stride, d.inner_stride, d.n_outer, d.n_inner, d.run_bytes,
-         d.word_bytes) = (at, *lay)
-    return out, len(tensors), tensors
+@functools.lru_cache(maxsize=512)
+def _struct_tail(shape, stride, dtype, word):
+    """A ``PageTensor``'s bytes behind its pointer, with words of ``word`` bytes if they fit."""
+    lay = _page_layout(shape, stride, torch.empty((), dtype=dtype).element_size())
+    return bytes(N.PageTensor(None, *lay[:6], min(lay[6], word)))[8:]
 
 
-def _state(block_table, seq_lens, refs, page_size):
-    same_device(refs, block_table=block_table, seq_lens=seq_lens)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+def _page_tensors(tensors, n_pages, ref):
+    """C array of page tensors; ``n_pages`` None takes the first tensor's."""
+    parts, dev, last, tails = [], ref.get_device(), None, {}
+    for t in tensors:
+        shape, at = t.shape, t.data_ptr()
+        layout = (shape, t.stride(), t.dtype)
+        if layout != last:  # (a model's pools are alike)
+            if n_pages is None:
+                n_pages = shape[0] if len(shape) else 0
+            if len(shape) < 2 or shape[0] != n_pages:
+                raise ValueError(f"page tensors must be [n_pages, ...] with {n_pages} pages")
+            last, tails = layout, {}
+        word = 4 if at & 15 else 16
+        tail = tails.get(word)
+        if tail is None:
+            tail = tails[word] = _struct_tail(*layout, word)
+        if at & 3:
+            raise ValueError("pages must be 4-byte aligned")
+        if t.get_device() != dev:
+            raise ValueError(f"page tensors must be on {ref.device}, got {t.device}")
+        parts.append(at.to_bytes(8, "little") + tail)
+    if not parts:
+        return None, 0, 0
+    return (N.PageTensor * len(parts)).from_buffer_copy(b"".join(parts)), len(parts), n_pages
+
+
+def _state(block_table, seq_lens, refs, page_size, *others):
+    device_of(refs, block_table, seq_lens, *others)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 [rows, max_pages] with contiguous rows")
-    rows, cols = block_table.shape
-    check_ints(refs, "refs")
+    (rows, cols), (stride, inner) = block_table.shape, block_table.stride()
+    if cols > 1 and inner != 1:
+        raise ValueError("block_table must be int32 [rows, max_pages] with contiguous rows")
+    if rows <= 1:
+        stride = cols
+    elif stride < cols:
+        raise ValueError("block_table rows must not overlap")
+    n_pages = check_ints(refs, "refs")
     if seq_lens is not None:
         check_ints(seq_lens, "seq_lens", rows)
     if page_size <= 0:
         raise ValueError("page_size must be positive")
-    stride = block_table.stride(0) if rows > 1 else cols
-    if stride < cols:
-        raise ValueError("block_table rows must not overlap")
     return N.PageState(block_table.data_ptr(), stride, rows, cols, None if seq_lens is None else seq_lens.data_ptr(),
-                       refs.data_ptr(), refs.shape[0], page_size)
-
-
-def _on_device(ref, tensors):
-    for t in tensors:
-        if t.device != ref.device:
-            raise ValueError(f"page tensors must be on {ref.device}, got {t.device}")
+                       refs.data_ptr(), n_pages, page_size)
 
 
 def copy_pages(tensors, src, dst):
     """Copy page ``src[i]`` of every tensor to page ``dst[i]`` (``[n] int32`` on the device),
     all tensors in one launch.  Pages that do not exist are skipped; no page may be twice in
     ``dst``, or in ``src`` and in ``dst``."""
-    tensors = list(tensors)
-    same_device(src, dst=dst)
-    check_ints(src, "src")
-    check_ints(dst, "dst", int(src.shape[0]))
-    if not tensors:
-        return
-    n_pages = int(tensors[0].shape[0]) if tensors[0].dim() else 0
-    desc, n, tensors = _page_tensors(tensors, n_pages)
-    _on_device(src, tensors)
-    launch(N.lib().ia_copy_pages, src, desc, n, src.data_ptr(), dst.data_ptr(), int(src.shape[0]), n_pages)
+    device_of(src, dst)
+    count = check_ints(src, "src")
+    check_ints(dst, "dst", count)
+    desc, n, n_pages = _page_tensors(tensors, None, src)
+    launch(N.lib().ia_copy_pages, src, desc, n, src.data_ptr(), dst.data_ptr(), count, n_pages)
 
 
 def fork_sequences(tensors, block_table, seq_lens, refs, src_rows, dst_rows, *, page_size, workspace=None):
@@ -113,12 +120,9 @@ def fork_sequences(tensors, block_table, seq_lens, refs, src_rows, dst_rows, *, 
     was where a row does not exist, ``dst_rows[i]`` is not empty (``free_sequences``) or
     listed before, ``src_rows[i]`` is in ``dst_rows`` or its last page is not mapped, or no
     page is free.  At most 8192 forks a call."""
-    state = _state(block_table, seq_lens, refs, page_size)
-    desc, n_t, tensors = _page_tensors(tensors, int(refs.shape[0]))
-    _on_device(refs, tensors)
-    same_device(refs, src_rows=src_rows, dst_rows=dst_rows)
-    check_ints(src_rows, "src_rows")
-    n = int(src_rows.shape[0])
+    state = _state(block_table, seq_lens, refs, page_size, src_rows, dst_rows)
+    desc, n_t, _ = _page_tensors(tensors, state.n_pages, refs)
+    n = check_ints(src_rows, "src_rows")
     check_ints(dst_rows, "dst_rows", n)
     ok = torch.empty_like(src_rows)
     lib = N.lib()
@@ -133,10 +137,8 @@ def free_sequences(block_table, seq_lens, refs, rows):
     """Rows ``rows`` (``[n] int32`` on the device) give up their pages: ``refs`` fall, table
     entries become -1, lengths 0.  A row listed twice is freed once; rows that do not exist
     are skipped."""
-    state = _state(block_table, seq_lens, refs, 1)
-    same_device(refs, rows=rows)
-    check_ints(rows, "rows")
-    launch(N.lib().ia_free_sequences, refs, state, rows.data_ptr(), int(rows.shape[0]))
+    state = _state(block_table, seq_lens, refs, 1, rows)
+    launch(N.lib().ia_free_sequences, refs, state, rows.data_ptr(), check_ints(rows, "rows"))
 
 
 def reserve_pages(block_table, seq_lens, refs, new_tokens, *, page_size, workspace=None):
@@ -144,13 +146,11 @@ def reserve_pages(block_table, seq_lens, refs, new_tokens, *, page_size, workspa
     the device; 0: none), the lowest free ones, rows in order.  Returns ``ok [rows] int32``:
     1, or 0 and the row as it was where its table row is too short or the pages left do not
     cover it."""
-    state = _state(block_table, seq_lens, refs, page_size)
-    same_device(refs, new_tokens=new_tokens)
-    rows = int(block_table.shape[0])
-    check_ints(new_tokens, "new_tokens", rows)
+    state = _state(block_table, seq_lens, refs, page_size, new_tokens)
+    rows = check_ints(new_tokens, "new_tokens", state.rows)
     lib = N.lib()
     ok = torch.empty_like(new_tokens)
-    need = max(lib.ia_reserve_workspace_size(rows, int(refs.shape[0])), 4)
+    need = max(lib.ia_reserve_workspace_size(rows, state.n_pages), 4)
     ws = workspace_tensor(workspace, ("reserve_scratch", need), (need,), device=refs.device, dtype=torch.uint8)
     launch(lib.ia_reserve_pages, refs, state, new_tokens.data_ptr(), ok.data_ptr(), ws.data_ptr(), ws.numel())
     return ok
@@ -163,11 +163,10 @@ def compact_pages(tensors, block_table, refs, *, workspace=None):
     on is free, so the pools can be cut or lent out.  Whatever else names pages (fp8
     ``sequence_scales``, copies of the table) has to be rebuilt."""
     state = _state(block_table, None, refs, 1)
-    desc, n_t, tensors = _page_tensors(tensors, int(refs.shape[0]))
-    _on_device(refs, tensors)
+    desc, n_t, _ = _page_tensors(tensors, state.n_pages, refs)
     lib = N.lib()
     n_live = torch.empty(1, device=refs.device, dtype=torch.int32)
-    need = lib.ia_compact_workspace_size(int(refs.shape[0]))
+    need = lib.ia_compact_workspace_size(state.n_pages)
     ws = workspace_tensor(workspace, ("compact_scratch", need), (need,), device=refs.device, dtype=torch.uint8)
     launch(lib.ia_compact_pages, refs, state, desc, n_t, n_live.data_ptr(), ws.data_ptr(), ws.numel())
     return n_live

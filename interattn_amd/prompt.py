@@ -8,6 +8,8 @@ current stream of their tensors' device, never synchronise, and keep scratch and
 the caller's ``workspace`` dict; calls that share one must not overlap.
 """
 
+import functools
+
 import torch
 
 from . import _native as N
@@ -16,21 +18,27 @@ from .ops import _DTYPE_CODE, _code, _stream, paged_kv, workspace_tensor
 _F32, _BF16 = torch.float32, torch.bfloat16
 
 
-def same_device(ref, **tensors):
-    """Every tensor on ``ref``'s GPU (a kernel dereferences them all there)."""
-    if not ref.is_cuda:
+def device_of(ref, *others):
+    """``ref``'s GPU, which has to hold every other tensor too (a kernel reads them there)."""
+    dev = ref.get_device()
+    if dev < 0:
         raise ValueError("interattn_amd kernels need device (cuda) tensors")
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} must be on {ref.device}, got {t.device}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"every tensor must be on {ref.device}, got one on {t.device}")
+    return dev
 
 
 def check_ints(t, name, length=None):
-    """A contiguous int32 vector."""
-    if t.dtype != torch.int32 or t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
+    """A contiguous int32 vector; returns its length."""
+    if t.dtype != torch.int32 or t.dim() != 1:
         raise ValueError(f"{name} must be a contiguous int32 vector")
-    if length is not None and t.shape[0] != length:
-        raise ValueError(f"{name} must have {length} entries, got {t.shape[0]}")
+    n = t.shape[0]
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must be a contiguous int32 vector")
+    if length is not None and n != length:
+        raise ValueError(f"{name} must have {length} entries, got {n}")
+    return n
 
 
 def launch(fn, ref, *args):
@@ -42,25 +50,80 @@ def launch(fn, ref, *args):
             N.check(fn(*args, _stream(ref)))
 
 
-def _strides(t):
-    """(token, head) strides of packed rows; a dimension of one row has any."""
-    s = t.stride()
-    return (s[0] if t.shape[0] > 1 else 0), (s[1] if t.shape[1] > 1 else 0)
+# What follows from shapes, strides and types alone is checked once per combination and kept
+# as the bytes of the C struct, pointers and row counts left out; nothing is kept of a
+# tensor.  That is a quarter of a call's host time up to the launch (an append on an 8-core
+# EPYC container: 21.3 -> 16.2 us).
 
-
-def _shape(q, cu_seqlens, hkv, d):
-    if q.dim() != 3 or (q.shape[2] > 1 and q.stride(2) != 1):
+@functools.lru_cache(maxsize=1024)
+def _q_layout(heads, stride, dtype, hkv, d):
+    """``PromptShape`` bytes of packed query rows."""
+    if len(heads) != 2 or (heads[1] > 1 and stride[2] != 1):
         raise ValueError("q must be [tokens, n_q_heads, D] with contiguous rows")
-    if q.dtype not in (_F32, _BF16):
+    if dtype not in (_F32, _BF16):
         raise ValueError("q must be float32 or bfloat16")
-    if q.shape[2] != d:
+    if heads[1] != d:
         raise ValueError("q and the keys disagree on head_dim")
-    if hkv <= 0 or q.shape[1] <= 0 or q.shape[1] % hkv:
+    if hkv <= 0 or heads[0] <= 0 or heads[0] % hkv:
         raise ValueError("n_q_heads must be a multiple of n_kv_heads (grouped query attention)")
-    check_ints(cu_seqlens, "cu_seqlens")
-    if cu_seqlens.shape[0] < 1:
-        raise ValueError("cu_seqlens must have n_seq + 1 entries")
-    return N.PromptShape(cu_seqlens.shape[0] - 1, q.shape[0], q.shape[1], hkv, d, _DTYPE_CODE[q.dtype], *_strides(q))
+    return bytes(N.PromptShape(0, 0, heads[0], hkv, d, _DTYPE_CODE[dtype], stride[0],
+                               stride[1] if heads[0] > 1 else 0))
+
+
+def _prompt_shape(q, n_seq, hkv, d):
+    tokens = q.shape[0] if q.dim() else 0
+    shape = N.PromptShape.from_buffer_copy(_q_layout(q.shape[1:], q.stride(), q.dtype, hkv, d))
+    shape.n_seq, shape.n_tokens = n_seq, tokens
+    if tokens <= 1:
+        shape.q_token_stride = 0  # (any stride means nothing then)
+    return shape
+
+
+@functools.lru_cache(maxsize=1024)
+def _row_layout(k_heads, k_stride, k_dtype, v_heads, v_stride, v_dtype):
+    """``PackedKV`` bytes of packed K and V rows."""
+    if len(k_heads) != 2 or k_heads != v_heads:
+        raise ValueError("k and v must both be [tokens, n_kv_heads, D]")
+    if k_stride[2] != 1 or v_stride[2] != 1 or k_dtype != v_dtype:
+        raise ValueError("k and v must share a dtype and have contiguous rows")
+    one = k_heads[0] <= 1
+    return bytes(N.PackedKV(None, None, _code(k_dtype, "k and v"), k_stride[0], 0 if one else k_stride[1], v_stride[0],
+                            0 if one else v_stride[1]))
+
+
+def _packed_rows(k, v, tokens):
+    rows = N.PackedKV.from_buffer_copy(_row_layout(k.shape[1:], k.stride(), k.dtype, v.shape[1:], v.stride(), v.dtype))
+    if (tokens is not None and k.shape[0] != tokens) or k.shape[0] != v.shape[0]:
+        raise ValueError("k and v must have the same tokens" + ("" if tokens is None else ", q's"))
+    rows.k, rows.v = k.data_ptr(), v.data_ptr()
+    if k.shape[0] <= 1:
+        rows.k_token_stride = rows.v_token_stride = 0
+    return rows
+
+
+_POOLS = {}  # layouts of pools -> PagedKV bytes
+
+
+def _pool(pool_k, pool_v, block_table, scales):
+    """``ops.paged_kv``'s struct."""
+    ks, vs = scales[:2] if scales is not None else (None, None)
+    key = (pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype,
+           None if block_table is None else (block_table.shape, block_table.stride(), block_table.dtype),
+           None if ks is None else (ks.shape, ks.stride(), ks.dtype, vs.shape, vs.stride(), vs.dtype))
+    held = _POOLS.get(key)
+    if held is None:
+        kv, _ = paged_kv(pool_k, pool_v, block_table, scales if ks is None else (ks, vs))
+        kv.k = kv.v = kv.block_table = kv.k_scale = kv.v_scale = None
+        if len(_POOLS) >= 1024:
+            _POOLS.clear()
+        held = _POOLS[key] = bytes(kv)
+    kv = N.PagedKV.from_buffer_copy(held)
+    kv.k, kv.v = pool_k.data_ptr(), pool_v.data_ptr()
+    if block_table is not None:
+        kv.block_table = block_table.data_ptr()
+    if kv.dtype == N.IA_FP8_E4M3:
+        kv.k_scale, kv.v_scale = ks.data_ptr(), vs.data_ptr()
+    return kv
 
 
 def output(q, out, out_dtype, workspace, key):
@@ -71,8 +134,15 @@ def output(q, out, out_dtype, workspace, key):
         raise ValueError(f"out must be a contiguous {list(q.shape)} tensor")
     if out.dtype not in (_F32, _BF16) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError("out must be float32 or bfloat16, of out_dtype where that is given")
-    same_device(q, out=out)
+    device_of(q, out)
     return out
+
+
+def _n_seq(cu_seqlens):
+    n = check_ints(cu_seqlens, "cu_seqlens") - 1
+    if n < 0:
+        raise ValueError("cu_seqlens must have n_seq + 1 entries")
+    return n
 
 
 def _workspace(shape, kv_dtype, max_keys, workspace, device):
@@ -94,20 +164,15 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None, out_dtype=Non
     no sequence are left as ``out`` had them.  The prompt side of the paged decode calls,
     and what ``_sdpa_prefill_attention_forward`` (CBT/core.py:1180-1200) computes, without
     padding.  Forward only."""
-    same_device(q, k=k, v=v, cu_seqlens=cu_seqlens)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0]:
-        raise ValueError("k and v must be [tokens, n_kv_heads, D] with q's tokens")
-    if k.stride(2) != 1 or v.stride(2) != 1 or k.dtype != v.dtype:
-        raise ValueError("k and v must share a dtype and have contiguous rows")
-    code = _code(k.dtype, "k and v")
-    shape = _shape(q, cu_seqlens, int(k.shape[1]), int(k.shape[2]))
+    device_of(q, k, v, cu_seqlens)
+    kv = _packed_rows(k, v, q.shape[0] if q.dim() else None)
+    shape = _prompt_shape(q, _n_seq(cu_seqlens), k.shape[1], k.shape[2])
     out = output(q, out, out_dtype, workspace, "prompt_output")
-    kv = N.PackedKV(k.data_ptr(), v.data_ptr(), code, *_strides(k), *_strides(v))
-    ws = _workspace(shape, code, int(q.shape[0]), workspace, q.device)
-    if q.shape[0] == 0:
+    if shape.n_tokens == 0:
         return out
+    ws = _workspace(shape, kv.dtype, shape.n_tokens, workspace, q.device)
     launch(N.lib().ia_prompt_attention, q, shape, q.data_ptr(), kv, cu_seqlens.data_ptr(),
-           q.shape[2] ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
+           shape.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
            *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())))
     return out
 
@@ -121,21 +186,21 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     prefix and a single token are the same call; bf16, float32 and fp8 pools
     (``scales=(k_scale, v_scale)``).  Returns ``[tokens, Hq, D]``; rows of no sequence are
     left as ``out`` had them, a row that sees no key is zeros.  Forward only."""
-    kv, keep = paged_kv(pool_k, pool_v, block_table, scales)
-    same_device(q, pool_k=pool_k, pool_v=pool_v, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens)
-    shape = _shape(q, cu_seqlens, int(pool_k.shape[1]), int(pool_k.shape[3]))
-    check_ints(seq_lens, "seq_lens", int(shape.n_seq))
-    if block_table is not None and block_table.shape[0] != shape.n_seq:
+    device_of(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens, *(scales or ()))
+    kv = _pool(pool_k, pool_v, block_table, scales)
+    n_seq = _n_seq(cu_seqlens)
+    shape = _prompt_shape(q, n_seq, pool_k.shape[1], pool_k.shape[3])
+    check_ints(seq_lens, "seq_lens", n_seq)
+    if block_table is not None and block_table.shape[0] != n_seq:
         raise ValueError("block_table rows must match the sequences")
     out = output(q, out, out_dtype, workspace, "prompt_output")
+    if shape.n_tokens == 0:
+        return out
     cap = (kv.bt_cols if block_table is not None else kv.n_pages) * kv.page_size
     ws = _workspace(shape, kv.dtype, min(cap, (1 << 31) - 1025), workspace, q.device)
-    if q.shape[0] == 0:
-        return out
     launch(N.lib().ia_paged_prompt_attention, q, shape, q.data_ptr(), kv, seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-           q.shape[2] ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
+           shape.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
            *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())))
-    del keep
     return out
 
 
@@ -147,31 +212,26 @@ def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seq
     ``update_block_summaries`` can have both).  A position without a page is skipped and the
     length counts up to the first of them.  The many-token form of ``append_kv``: bf16 and
     float32 pools, capturable."""
-    kv, keep = paged_kv(pool_k, pool_v, block_table)
-    same_device(pool_k, pool_v=pool_v, block_table=block_table, seq_lens=seq_lens, k_new=k_new, v_new=v_new,
-                cu_seqlens=cu_seqlens, new_seq_lens=new_seq_lens)
-    check_ints(cu_seqlens, "cu_seqlens")
-    n_seq = int(cu_seqlens.shape[0]) - 1
-    if n_seq < 0:
-        raise ValueError("cu_seqlens must have n_seq + 1 entries")
+    device_of(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, new_seq_lens)
+    n_seq = _n_seq(cu_seqlens)
     check_ints(seq_lens, "seq_lens", n_seq)
-    hkv, d = int(pool_k.shape[1]), int(pool_k.shape[3])
-    for t in (k_new, v_new):
-        if t.dim() != 3 or tuple(t.shape[1:]) != (hkv, d) or t.stride(2) != 1 or t.dtype != pool_k.dtype:
-            raise ValueError("k_new/v_new must be [tokens, Hkv, D] of the pool dtype with contiguous rows")
-    if k_new.shape[0] != v_new.shape[0]:
-        raise ValueError("k_new and v_new must have the same tokens")
+    if pool_k.dtype not in (_F32, _BF16):
+        raise ValueError("append takes bf16 or float32 pools")
+    kv = _pool(pool_k, pool_v, block_table, None)
+    hkv, d = pool_k.shape[1], pool_k.shape[3]
+    rows = _packed_rows(k_new, v_new, None)
+    if k_new.shape[1] != hkv or k_new.shape[2] != d or k_new.dtype != pool_k.dtype:
+        raise ValueError("k_new/v_new must be [tokens, Hkv, D] of the pool dtype with contiguous rows")
     if block_table is not None and block_table.shape[0] != n_seq:
         raise ValueError("block_table rows must match the sequences")
     if new_seq_lens is None:
         new_seq_lens = torch.empty_like(seq_lens)
-    check_ints(new_seq_lens, "new_seq_lens", n_seq)
-    if n_seq and abs(new_seq_lens.data_ptr() - seq_lens.data_ptr()) < 4 * n_seq:
-        raise ValueError("new_seq_lens must not overlap seq_lens")
-    rows = N.PackedKV(k_new.data_ptr(), v_new.data_ptr(), kv.dtype, *_strides(k_new), *_strides(v_new))
+    else:
+        check_ints(new_seq_lens, "new_seq_lens", n_seq)
+        if n_seq and abs(new_seq_lens.data_ptr() - seq_lens.data_ptr()) < 4 * n_seq:
+            raise ValueError("new_seq_lens must not overlap seq_lens")
     launch(N.lib().ia_append_prompt_kv, pool_k, kv, rows, cu_seqlens.data_ptr(), seq_lens.data_ptr(),
-           new_seq_lens.data_ptr(), n_seq, int(k_new.shape[0]), hkv, d)
-    del keep
+           new_seq_lens.data_ptr(), n_seq, k_new.shape[0], hkv, d)
     return new_seq_lens
 
 
@@ -188,30 +248,23 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
     sequence's own row, so forked tables (``fork_sequences``) and tables that repeat the
     prefix in pages of their own give the same.  Any group of query heads up to 64; bf16,
     float32 and fp8 pools."""
-    kv, keep = paged_kv(pool_k, pool_v, block_table, scales)
-    same_device(q, pool_k=pool_k, pool_v=pool_v, block_table=block_table, seq_lens=seq_lens,
-                group_starts=group_starts, shared_lens=shared_lens)
-    hkv, d = int(pool_k.shape[1]), int(pool_k.shape[3])
-    if q.dim() != 3 or q.stride(2) != 1 or q.dtype not in (_F32, _BF16) or q.shape[2] != d:
-        raise ValueError("q must be [batch, n_q_heads, D] float32 or bfloat16 with contiguous rows of the pool's D")
-    b, hq, _ = q.shape
-    if hkv <= 0 or hq <= 0 or hq % hkv:
-        raise ValueError("n_q_heads must be a multiple of n_kv_heads (grouped query attention)")
+    device_of(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *(scales or ()))
+    kv = _pool(pool_k, pool_v, block_table, scales)
+    rows = _prompt_shape(q, 0, pool_k.shape[1], pool_k.shape[3])  # (checks q; a row per sequence)
+    b, hq, hkv, d = rows.n_tokens, rows.n_q_heads, rows.n_kv_heads, rows.head_dim
     check_ints(seq_lens, "seq_lens", b)
-    check_ints(shared_lens, "shared_lens")
-    n_groups = int(shared_lens.shape[0])
+    n_groups = check_ints(shared_lens, "shared_lens")
     check_ints(group_starts, "group_starts", n_groups + 1)
     if block_table is not None and block_table.shape[0] != b:
         raise ValueError("block_table rows must match the batch")
     out = output(q, out, out_dtype, workspace, "attention_output")
-    shape = N.DecodeShape(b, hq, hkv, d, *_strides(q), _DTYPE_CODE[q.dtype])
+    shape = N.DecodeShape(b, hq, hkv, d, rows.q_token_stride, rows.q_head_stride, rows.q_dtype)
     key = ("shared_prefix_scratch", b, n_groups, hkv, hq, d, kv.dtype)
     ws = None if workspace is None else workspace.get(key)
-    if ws is None or ws.device != q.device:
+    if ws is None or ws.get_device() != q.get_device():
         need = N.lib().ia_shared_prefix_workspace_size(shape, kv.dtype, n_groups)
         ws = workspace_tensor(workspace, key, (max(need, 1),), device=q.device, dtype=torch.uint8)
     launch(N.lib().ia_shared_prefix_decode, q, shape, q.data_ptr(), kv, seq_lens.data_ptr(), group_starts.data_ptr(),
            shared_lens.data_ptr(), n_groups, d ** -0.5 if scale is None else float(scale), out.data_ptr(),
            _DTYPE_CODE[out.dtype], ws.data_ptr(), ws.numel())
-    del keep
     return out
