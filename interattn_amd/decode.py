@@ -261,13 +261,16 @@ class PagedTopkDecodeRunner:
     summaries the new token touched (``update_block_summaries``) and runs the fused
     top-k layer call (``sparse_topk_decode``); layers below ``full_attention_layers``
     run the HIP paged dense decode.  Prompts of one batch share a length (no
-    padding).  Install with ``condition_block_decode_context(runner)``."""
+    padding).  With ``native_prompt=True`` the prefill runs ``prompt_attention`` and
+    ``append_prompt_kv`` instead of SDPA and the copy.  Install with
+    ``condition_block_decode_context(runner)``."""
 
     def __init__(self, *, model, batch_size, max_seq_len, block_size, k, forced_first=0, forced_last=0,
-                 page_size=16, full_attention_layers=0, k_bar_dtype=None, seed=0):
-        from . import ops
+                 page_size=16, full_attention_layers=0, k_bar_dtype=None, seed=0, native_prompt=False):
+        from . import ops, prompt
 
-        self._ops = ops
+        self._ops, self._prompt = ops, prompt
+        self.native_prompt = bool(native_prompt)
         cfg = model.config
         param = next(model.parameters())
         self.device, self.dtype = param.device, param.dtype
@@ -304,13 +307,40 @@ class PagedTopkDecodeRunner:
         idx = getattr(module, "layer_idx", None)
         return int(self.module_to_layer_idx[id(module)] if idx is None else idx)
 
-    def _fill(self, layer, key, value):
-        """Copy the prompt's K/V [B, Hkv, T, D] into the layer's pool, build summaries."""
+    def _check_prompt(self, key):
         b, hkv, t, d = key.shape
         if b != self.batch_size or hkv != self.n_kv_heads or d != self.head_dim:
             raise ValueError("prompt K/V do not match the runner's batch / heads / head_dim")
         if t > self.max_seq_len:
             raise ValueError("prompt longer than max_seq_len")
+
+    def _summarize(self, layer):
+        """Block summaries of a layer whose pool holds its prompt."""
+        if layer >= self.full_attention_layers:
+            pk, pv = self.pools[layer]
+            self.summaries[layer] = self._ops.build_block_summaries(
+                pk, pv, self.block_table, self.seq_lens[layer], self.block_size, nb_max=self.nb_max,
+                k_bar_dtype=self.k_bar_dtype)
+
+    def _prefill_native(self, layer, query, key, value, scaling):
+        """The prompt on the HIP path: its rows packed, K/V into the pool, attention over them."""
+        self._check_prompt(key)
+        b, hq, t, d = query.shape
+        q, k, v = (x.transpose(1, 2).reshape(b * t, x.shape[1], d) for x in (query, key, value))
+        cu = torch.arange(0, (b + 1) * t, max(t, 1), device=query.device, dtype=torch.int32)[:b + 1]
+        pk, pv = self.pools[layer]
+        self._prompt.append_prompt_kv(pk, pv, self.block_table, self.old_seq_lens[layer].zero_(), k.to(pk.dtype),
+                                      v.to(pv.dtype), cu, new_seq_lens=self.seq_lens[layer])
+        self._summarize(layer)
+        out = torch.empty((b, t, hq, d), device=query.device, dtype=query.dtype)
+        self._prompt.prompt_attention(q, k, v, cu, scale=scaling, out=out.view(b * t, hq, d),
+                                      workspace=self.workspace_by_layer[layer])
+        return out, None
+
+    def _fill(self, layer, key, value):
+        """Copy the prompt's K/V [B, Hkv, T, D] into the layer's pool, build summaries."""
+        self._check_prompt(key)
+        b, hkv, t, d = key.shape
         pk, pv = self.pools[layer]
         n_pg = -(-t // self.page_size)
         pages = self.block_table[:, :n_pg].reshape(-1).long()
@@ -319,14 +349,13 @@ class PagedTopkDecodeRunner:
             x = x.view(b, hkv, n_pg, self.page_size, d).permute(0, 2, 1, 3, 4)
             pool[pages] = x.reshape(b * n_pg, hkv, self.page_size, d).to(pool.dtype)
         self.seq_lens[layer].fill_(t)
-        if layer >= self.full_attention_layers:
-            self.summaries[layer] = self._ops.build_block_summaries(
-                pk, pv, self.block_table, self.seq_lens[layer], self.block_size, nb_max=self.nb_max,
-                k_bar_dtype=self.k_bar_dtype)
+        self._summarize(layer)
 
     def hybrid_attention_forward(self, module, query, key, value, attention_mask, scaling, dropout=0.0, **kwargs):
         layer = self._layer(module)
         if query.shape[2] != 1:
+            if self.native_prompt and not (dropout and module.training):
+                return self._prefill_native(layer, query, key, value, scaling)
             self._fill(layer, key, value)
             return _sdpa_prefill_attention_forward(module, query, key, value, attention_mask, scaling=scaling,
                                                    dropout=dropout, **kwargs)
