@@ -63,18 +63,23 @@ int64_t resident_wgs(int kv_dtype) { return (int64_t)device_cus() * (kv_dtype ==
 
 // Row tiles (a bound from the token and sequence counts alone), and the slices their keys
 // may be cut into.  Tiles of 128 rows read K/V least often and keep the matrix cores
-// busiest; a launch whose tiles of 32 rows all run at once takes those, for a quarter of
-// the products on each row's way (float32 products are as dense in both, and a tile of 128
-// rows holds one of 32's four waves as long: always 32).  Then, with fewer tiles than
-// workgroups run at once, every tile is cut along its keys to fill the device.
+// busiest.  A launch whose tiles of 128 do not fill the device, cut along their keys or
+// not, and whose tiles of 32 rows all run at once takes those: four times the workgroups,
+// each with a quarter of the products.  float32 products are as dense in both shapes, and in
+// tiles of 32 rows a row's keys spread over four waves: always 32.  Then, with fewer tiles
+// than workgroups run at once, every tile is cut along its keys.
 void prompt_grid(const ia_prompt_shape* s, int kv_dtype, int64_t most_keys, PromptParams* p) {
   const int group = s->n_q_heads / s->n_kv_heads;
   const int64_t resident = resident_wgs(kv_dtype);
+  const int64_t most_slices = (most_keys + kPromptSliceTiles * kArTile - 1) / (kPromptSliceTiles * kArTile);
   // about how many tiles of `rows` rows: half a tile lost per sequence
   auto about = [&](int rows) {
     return ((int64_t)s->n_tokens / (rows / group) + (s->n_seq + 1) / 2) * s->n_kv_heads;
   };
-  p->tile_rows = group <= kArNarrow && (kv_dtype == IA_F32 || about(kArNarrow) <= resident) ? kArNarrow : kArRows;
+  const bool small = group <= kArNarrow &&
+                     (kv_dtype == IA_F32 ||
+                      (about(kArNarrow) <= resident && about(kArRows) * std::min(most_slices, resident) <= resident));
+  p->tile_rows = small ? kArNarrow : kArRows;
   p->tile_tokens = p->tile_rows / group;
   p->n_tiles = (int)std::min<int64_t>((int64_t)s->n_tokens / p->tile_tokens + s->n_seq, INT32_MAX);
   const int64_t tiles = std::max<int64_t>(1, about(p->tile_rows));
@@ -82,7 +87,7 @@ void prompt_grid(const ia_prompt_shape* s, int kv_dtype, int64_t most_keys, Prom
   int64_t n = 5 * resident >= 6 * tiles ? (resident + tiles - 1) / tiles : 1;  // (a cut for less than a fifth costs more)
   n = std::min<int64_t>(n, kPromptMaxSlices);
   n = std::min<int64_t>(n, 2 * resident / bound);
-  n = std::min<int64_t>(n, (most_keys + kPromptSliceTiles * kArTile - 1) / (kPromptSliceTiles * kArTile));
+  n = std::min(n, most_slices);
   p->slices = (int)std::max<int64_t>(1, n);
 }
 
