@@ -1,5 +1,10 @@
 // Causal attention of packed prompts: parameters shared by the host side and the per-type
 // kernel instances.
+//
+// 4 D flops per visible (row, key) pair, on the matrix cores; at D = 64 the softmax's vector
+// work (an exponential costs four issue slots) outweighs the products.  Two prompts of 8,192
+// tokens (8 kv heads of 128, groups of 4, bf16) took 1,249 us, 880 TFLOP/s, with the products
+// waiting on every operand's LDS read; they are read ahead since, which is not timed yet.
 #pragma once
 
 #include "attend_rows.hpp"
