@@ -3,7 +3,7 @@
 //
 // A workgroup takes up to 128 rows of one kv head (tokens x the group's query heads, so a
 // K/V tile is read once for the whole group) and streams the range in tiles of 64 keys
-// through LDS, two tiles in flight.  Row r's softmax runs online in base 2 with its scale
+// through LDS, the next one on its way while one is used.  Row r's softmax runs online in base 2 with its scale
 // folded in: s' = q.k * scale * log2(e); (m, l, acc) are float32, the products bf16 in,
 // float32 out (float32 caches: float32 products).  P is rounded to bf16 for the second
 // product, as the cache's values are; l sums the unrounded P.
@@ -36,7 +36,6 @@ constexpr int64_t kArMaxGrid = 1 << 23;  // workgroups of a launch (work items a
 constexpr float kArSlack = 8.f;   // log2 units a row's maximum may rise before it is rescaled
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
-typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
 #define IA_LDS __attribute__((address_space(3)))
 
 // K/V of a call: pages of page_rows tokens (a multiple of 16).  Packed rows are pages of
@@ -120,13 +119,11 @@ __device__ __forceinline__ u32 lds_addr(const void* p) {
   return (u32)(uintptr_t)(const IA_LDS char*)p;
 }
 
-__device__ __forceinline__ bool ar_finite(float x) { return fabsf(x) < __builtin_huge_valf(); }
-
 // ------------------------------------------------------------------ tiles
 
 // Loads tiles of one item.  A tile starts at a multiple of 16 keys, so each of its four
-// groups of 16 keys lies in one page.  Lane l keeps the page and the row in it of group
-// l & 3, fetched one tile ahead of the K/V loads that need it.
+// groups of 16 keys lies in one page.  Lane l keeps where group l & 3 lies, fetched one tile
+// ahead of the K/V loads that need it: a load's address is two lane reads and one addition.
 template <int KV, int D>
 struct ArLoader {
   using S = ArShape<KV, D>;

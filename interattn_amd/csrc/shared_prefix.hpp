@@ -163,12 +163,13 @@ __device__ __forceinline__ bool prefix_plan(const PrefixParams& p, int want, cha
     const long long c = (even * (16 + j) + 15) / 16;
     return (int)(c < kPrefixMinTiles ? kPrefixMinTiles : c);
   };
-  // wave w tries cuts w, w + 4, ...
-  for (int j = wave; j < kPrefixCuts; j += kArThreads / 64) {
+  // wave w tries cuts w, w + 4, ... (batches too wide for LDS take the last: a trial is a
+  // pass over them)
+  for (int j = wave; j < kPrefixCuts && held; j += kArThreads / 64) {
     const u32 cut = cut_at(j);
     long long items = 0;
     for (int e = lane; e < n; e += 64) {
-      const u32 t = held ? tiles[e] : prefix_tiles(prefix_range(p, gr, e));
+      const u32 t = tiles[e];
       items += (t + cut - 1) / cut;
     }
     for (int s = 32; s > 0; s >>= 1) items += __shfl_xor(items, s, 64);
@@ -177,7 +178,7 @@ __device__ __forceinline__ bool prefix_plan(const PrefixParams& p, int want, cha
   if (tid < 8) found[tid] = -1;
   __syncthreads();
   int j = 0;
-  while (j < kPrefixCuts - 1 && sums[j] > p.target) ++j;
+  while (j < kPrefixCuts - 1 && (!held || sums[j] > p.target)) ++j;
   const u32 cut = cut_at(j);
   int base = 0, rows0 = 0;
   for (int e0 = 0; e0 < n; e0 += kArThreads) {
