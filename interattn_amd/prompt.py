@@ -52,8 +52,8 @@ def launch(fn, ref, *args):
 
 # What follows from shapes, strides and types alone is checked once per combination and kept
 # as the bytes of the C struct, pointers and row counts left out; nothing is kept of a
-# tensor.  That is a quarter of a call's host time up to the launch (an append on an 8-core
-# EPYC container: 21.3 -> 16.2 us).
+# tensor.  That is a third of a call's host time up to the launch (an append on an 8-core
+# EPYC host: 21.3 -> 14.0 us).
 
 @functools.lru_cache(maxsize=1024)
 def _q_layout(heads, stride, dtype, hkv, d):
@@ -71,8 +71,9 @@ def _q_layout(heads, stride, dtype, hkv, d):
 
 
 def _prompt_shape(q, n_seq, hkv, d):
-    tokens = q.shape[0] if q.dim() else 0
-    shape = N.PromptShape.from_buffer_copy(_q_layout(q.shape[1:], q.stride(), q.dtype, hkv, d))
+    rows = q.shape
+    shape = N.PromptShape.from_buffer_copy(_q_layout(rows[1:], q.stride(), q.dtype, hkv, d))
+    tokens = rows[0]
     shape.n_seq, shape.n_tokens = n_seq, tokens
     if tokens <= 1:
         shape.q_token_stride = 0  # (any stride means nothing then)
@@ -81,49 +82,61 @@ def _prompt_shape(q, n_seq, hkv, d):
 
 @functools.lru_cache(maxsize=1024)
 def _row_layout(k_heads, k_stride, k_dtype, v_heads, v_stride, v_dtype):
-    """``PackedKV`` bytes of packed K and V rows."""
+    """``(PackedKV bytes, n_kv_heads, D)`` of packed K and V rows."""
     if len(k_heads) != 2 or k_heads != v_heads:
         raise ValueError("k and v must both be [tokens, n_kv_heads, D]")
     if k_stride[2] != 1 or v_stride[2] != 1 or k_dtype != v_dtype:
         raise ValueError("k and v must share a dtype and have contiguous rows")
     one = k_heads[0] <= 1
     return bytes(N.PackedKV(None, None, _code(k_dtype, "k and v"), k_stride[0], 0 if one else k_stride[1], v_stride[0],
-                            0 if one else v_stride[1]))
+                            0 if one else v_stride[1])), k_heads[0], k_heads[1]
 
 
-def _packed_rows(k, v, tokens):
-    rows = N.PackedKV.from_buffer_copy(_row_layout(k.shape[1:], k.stride(), k.dtype, v.shape[1:], v.stride(), v.dtype))
-    if (tokens is not None and k.shape[0] != tokens) or k.shape[0] != v.shape[0]:
-        raise ValueError("k and v must have the same tokens" + ("" if tokens is None else ", q's"))
+def _packed_rows(k, v):
+    """``(PackedKV, tokens, n_kv_heads, D)``."""
+    ks, vs = k.shape, v.shape
+    held, hkv, d = _row_layout(ks[1:], k.stride(), k.dtype, vs[1:], v.stride(), v.dtype)
+    tokens = ks[0]
+    if vs[0] != tokens:
+        raise ValueError("k and v must have the same tokens")
+    rows = N.PackedKV.from_buffer_copy(held)
     rows.k, rows.v = k.data_ptr(), v.data_ptr()
-    if k.shape[0] <= 1:
+    if tokens <= 1:
         rows.k_token_stride = rows.v_token_stride = 0
-    return rows
+    return rows, tokens, hkv, d
 
 
-_POOLS = {}  # layouts of pools -> PagedKV bytes
+_POOLS = {}  # layouts of pools -> (PagedKV bytes, n_kv_heads, D)
 
 
-def _pool(pool_k, pool_v, block_table, scales):
-    """``ops.paged_kv``'s struct."""
-    ks, vs = scales[:2] if scales is not None else (None, None)
-    key = (pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype,
-           None if block_table is None else (block_table.shape, block_table.stride(), block_table.dtype),
-           None if ks is None else (ks.shape, ks.stride(), ks.dtype, vs.shape, vs.stride(), vs.dtype))
+def _pool(pool_k, pool_v, block_table, scales, n_seq):
+    """``(PagedKV, n_kv_heads, D)``: ``ops.paged_kv``'s struct, its table of ``n_seq`` rows."""
+    key = [pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype]
+    if block_table is not None:
+        rows = block_table.shape
+        if rows[0] != n_seq:
+            raise ValueError("block_table must have a row for each sequence")
+        key += (rows, block_table.stride(), block_table.dtype)
+    ks = vs = None
+    if scales is not None:
+        ks, vs = scales[:2]
+        key += (ks.shape, ks.stride(), ks.dtype, vs.shape, vs.stride(), vs.dtype)
+    key = tuple(key)
     held = _POOLS.get(key)
     if held is None:
         kv, _ = paged_kv(pool_k, pool_v, block_table, scales if ks is None else (ks, vs))
         kv.k = kv.v = kv.block_table = kv.k_scale = kv.v_scale = None
         if len(_POOLS) >= 1024:
             _POOLS.clear()
-        held = _POOLS[key] = bytes(kv)
+        held = _POOLS[key] = bytes(kv), pool_k.shape[1], pool_k.shape[3]
+    held, hkv, d = held
     kv = N.PagedKV.from_buffer_copy(held)
     kv.k, kv.v = pool_k.data_ptr(), pool_v.data_ptr()
     if block_table is not None:
         kv.block_table = block_table.data_ptr()
     if kv.dtype == N.IA_FP8_E4M3:
         kv.k_scale, kv.v_scale = ks.data_ptr(), vs.data_ptr()
-    return kv
+    return kv, hkv, d
 
 
 def output(q, out, out_dtype, workspace, key):
@@ -165,14 +178,16 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None, out_dtype=Non
     and what ``_sdpa_prefill_attention_forward`` (CBT/core.py:1180-1200) computes, without
     padding.  Forward only."""
     device_of(q, k, v, cu_seqlens)
-    kv = _packed_rows(k, v, q.shape[0] if q.dim() else None)
-    shape = _prompt_shape(q, _n_seq(cu_seqlens), k.shape[1], k.shape[2])
+    kv, tokens, hkv, d = _packed_rows(k, v)
+    shape = _prompt_shape(q, _n_seq(cu_seqlens), hkv, d)
+    if shape.n_tokens != tokens:
+        raise ValueError("k and v must have q's tokens")
     out = output(q, out, out_dtype, workspace, "prompt_output")
-    if shape.n_tokens == 0:
+    if tokens == 0:
         return out
-    ws = _workspace(shape, kv.dtype, shape.n_tokens, workspace, q.device)
+    ws = _workspace(shape, kv.dtype, tokens, workspace, q.device)
     launch(N.lib().ia_prompt_attention, q, shape, q.data_ptr(), kv, cu_seqlens.data_ptr(),
-           shape.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
+           d ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
            *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())))
     return out
 
@@ -187,19 +202,17 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     (``scales=(k_scale, v_scale)``).  Returns ``[tokens, Hq, D]``; rows of no sequence are
     left as ``out`` had them, a row that sees no key is zeros.  Forward only."""
     device_of(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens, *(scales or ()))
-    kv = _pool(pool_k, pool_v, block_table, scales)
     n_seq = _n_seq(cu_seqlens)
-    shape = _prompt_shape(q, n_seq, pool_k.shape[1], pool_k.shape[3])
+    kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, n_seq)
+    shape = _prompt_shape(q, n_seq, hkv, d)
     check_ints(seq_lens, "seq_lens", n_seq)
-    if block_table is not None and block_table.shape[0] != n_seq:
-        raise ValueError("block_table rows must match the sequences")
     out = output(q, out, out_dtype, workspace, "prompt_output")
     if shape.n_tokens == 0:
         return out
     cap = (kv.bt_cols if block_table is not None else kv.n_pages) * kv.page_size
     ws = _workspace(shape, kv.dtype, min(cap, (1 << 31) - 1025), workspace, q.device)
     launch(N.lib().ia_paged_prompt_attention, q, shape, q.data_ptr(), kv, seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-           shape.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
+           d ** -0.5 if scale is None else float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype],
            *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())))
     return out
 
@@ -217,13 +230,10 @@ def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seq
     check_ints(seq_lens, "seq_lens", n_seq)
     if pool_k.dtype not in (_F32, _BF16):
         raise ValueError("append takes bf16 or float32 pools")
-    kv = _pool(pool_k, pool_v, block_table, None)
-    hkv, d = pool_k.shape[1], pool_k.shape[3]
-    rows = _packed_rows(k_new, v_new, None)
-    if k_new.shape[1] != hkv or k_new.shape[2] != d or k_new.dtype != pool_k.dtype:
+    kv, hkv, d = _pool(pool_k, pool_v, block_table, None, n_seq)
+    rows, tokens, *heads = _packed_rows(k_new, v_new)
+    if heads != [hkv, d] or rows.dtype != kv.dtype:
         raise ValueError("k_new/v_new must be [tokens, Hkv, D] of the pool dtype with contiguous rows")
-    if block_table is not None and block_table.shape[0] != n_seq:
-        raise ValueError("block_table rows must match the sequences")
     if new_seq_lens is None:
         new_seq_lens = torch.empty_like(seq_lens)
     else:
@@ -231,7 +241,7 @@ def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seq
         if n_seq and abs(new_seq_lens.data_ptr() - seq_lens.data_ptr()) < 4 * n_seq:
             raise ValueError("new_seq_lens must not overlap seq_lens")
     launch(N.lib().ia_append_prompt_kv, pool_k, kv, rows, cu_seqlens.data_ptr(), seq_lens.data_ptr(),
-           new_seq_lens.data_ptr(), n_seq, k_new.shape[0], hkv, d)
+           new_seq_lens.data_ptr(), n_seq, tokens, hkv, d)
     return new_seq_lens
 
 
@@ -249,14 +259,14 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
     prefix in pages of their own give the same.  Any group of query heads up to 64; bf16,
     float32 and fp8 pools."""
     device_of(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *(scales or ()))
-    kv = _pool(pool_k, pool_v, block_table, scales)
-    rows = _prompt_shape(q, 0, pool_k.shape[1], pool_k.shape[3])  # (checks q; a row per sequence)
-    b, hq, hkv, d = rows.n_tokens, rows.n_q_heads, rows.n_kv_heads, rows.head_dim
-    check_ints(seq_lens, "seq_lens", b)
+    b = check_ints(seq_lens, "seq_lens")
+    kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, b)
+    rows = _prompt_shape(q, 0, hkv, d)  # (checks q; a row per sequence)
+    hq = rows.n_q_heads
+    if rows.n_tokens != b:
+        raise ValueError("q must have a row for each sequence")
     n_groups = check_ints(shared_lens, "shared_lens")
     check_ints(group_starts, "group_starts", n_groups + 1)
-    if block_table is not None and block_table.shape[0] != b:
-        raise ValueError("block_table rows must match the batch")
     out = output(q, out, out_dtype, workspace, "attention_output")
     shape = N.DecodeShape(b, hq, hkv, d, rows.q_token_stride, rows.q_head_stride, rows.q_dtype)
     key = ("shared_prefix_scratch", b, n_groups, hkv, hq, d, kv.dtype)

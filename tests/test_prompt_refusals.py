@@ -266,7 +266,7 @@ def test_row_layouts():
         with pytest.raises(ValueError):
             prompt._q_layout(torch.Size(heads), stride, dtype, hkv, d)
     ok = (torch.Size((2, 64)), (128, 64, 1), torch.float32)
-    assert ctypes.sizeof(N.PackedKV) == len(prompt._row_layout(*ok, *ok))
+    assert ctypes.sizeof(N.PackedKV) == len(prompt._row_layout(*ok, *ok)[0])
     for other in ((torch.Size((3, 64)), (128, 64, 1), torch.float32), (torch.Size((2, 64)), (128, 64, 2), torch.float32),
                   (torch.Size((2, 64)), (128, 64, 1), torch.bfloat16)):
         with pytest.raises(ValueError):
