@@ -301,6 +301,7 @@ class PagedTopkDecodeRunner:
         self.old_seq_lens = [torch.zeros_like(t) for t in self.seq_lens]
         self.summaries = [None] * self.n_layers
         self.workspace_by_layer = [{} for _ in range(self.n_layers)]
+        self.prompt_workspace = {}  # (partials of one prompt call: its layers follow each other)
         self.module_to_layer_idx = {id(layer.self_attn): int(i) for i, layer in enumerate(model.model.layers)}
 
     def _layer(self, module):
@@ -334,7 +335,7 @@ class PagedTopkDecodeRunner:
         self._summarize(layer)
         out = torch.empty((b, t, hq, d), device=query.device, dtype=query.dtype)
         self._prompt.prompt_attention(q, k, v, cu, scale=scaling, out=out.view(b * t, hq, d),
-                                      workspace=self.workspace_by_layer[layer])
+                                      workspace=self.prompt_workspace)
         return out, None
 
     def _fill(self, layer, key, value):
