@@ -285,7 +285,8 @@ __device__ __forceinline__ const char* ar_q_row(const ArParams& p, const ArItem&
          ((int64_t)tok * p.q_tok + (int64_t)(it.head * p.group + g) * p.q_head) * (p.q_f32 ? 4 : 2);
 }
 
-// eight q elements at element e of a row as a bf16 operand (zero rows past the last)
+// eight q elements at element e of a row as a bf16 operand (zero rows past the last); a
+// float32 q is rounded to bf16, the products' type over these caches, as in the decode calls
 __device__ __forceinline__ bf16x8_t ar_q8(const ArParams& p, const char* row, int e, bool live) {
   u32 w[4] = {0, 0, 0, 0};
   if (live) {

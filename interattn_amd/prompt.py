@@ -173,7 +173,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None, out_dtype=Non
     (any token and head strides of 16-byte multiples with contiguous rows: views of one
     fused projection need no copy), the query heads of a kv head neighbours.  Token i of a
     sequence attends tokens 0..i of it, softmax in float32.  ``k, v`` bf16 or float32 (then
-    ``q`` too).  Returns ``[tokens, Hq, D]`` of ``out_dtype`` (``q``'s by default); rows of
+    ``q`` too; over bf16 a float32 ``q`` is rounded to bf16).  Returns ``[tokens, Hq, D]`` of ``out_dtype`` (``q``'s by default); rows of
     no sequence are left as ``out`` had them.  The prompt side of the paged decode calls,
     and what ``_sdpa_prefill_attention_forward`` (CBT/core.py:1180-1200) computes, without
     padding.  Forward only."""
