@@ -16,7 +16,8 @@
 // Two shapes:
 //   wide   (33..128 rows): 32x32 matrix tiles, a wave per 32 rows, all keys of the tile
 //   narrow (1..32 rows):   16x16 matrix tiles, a wave per 16 keys, all rows; the four
-//                          waves' (m, l, acc) meet in LDS at the end
+//                          waves' (m, l, acc) meet in LDS at the end.  Its EXACT form also
+//                          does items over, 32 rows at a time
 //
 // LDS rows are whole cache rows in 16-byte chunks, chunk c of row r at c ^ f(r): f is
 // linear over the bits of r and chosen so that neither the row-per-lane key reads nor the
@@ -113,6 +114,12 @@ __device__ __forceinline__ int ar_swizzle(int r) {
 __device__ __forceinline__ void ar_dma16(const char* src, u32 lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
+// x, but nothing computed from it before is kept in registers (for the second pass, for the
+// last stores)
+__device__ __forceinline__ int ar_anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ void ar_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ u32 lds_addr(const void* p) {
@@ -139,8 +146,8 @@ struct ArLoader {
   float ks, vs;            // fp8: its scales, of the tile last issued
   u32x4_t kr[KV == kArFp8 ? S::kLoads : 1], vr[KV == kArFp8 ? S::kLoads : 1];
 
-  __device__ __forceinline__ ArLoader(const ArSource& kv_, const ArItem& it_) : kv(kv_), it(it_) {
-    tid = threadIdx.x;
+  __device__ __forceinline__ ArLoader(const ArSource& kv_, const ArItem& it_, bool anew) : kv(kv_), it(it_) {
+    tid = anew ? ar_anew(threadIdx.x) : threadIdx.x;
     lane = tid & 63;
     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     ks = vs = 0.f;
@@ -332,91 +339,50 @@ __device__ __forceinline__ int64_t ar_out_row(const ArParams& p, const ArItem& i
   return ((int64_t)tok * p.n_kv_heads * p.group + it.head * p.group + g) * d;
 }
 
-// One row again, key by key, by one wave.  The matrix cores multiply a hidden key's V by
-// P = 0, which is NaN where V is not finite; a row that came out so in a range where some
-// keys are hidden from it is done over here, with the hidden keys left out.
-template <int KV, int D>
-__device__ void ar_row_by_key(const ArParams& p, const ArItem& it, int r, int lane) {
-  constexpr int kE = D / 64;
-  const ArSource& kv = p.kv;
-  const char* qr = ar_q_row(p, it, r);
-  float q[kE], acc[kE], m = kNegInf, l = 0.f;
+// The second pass.  A key hidden from a row meets it with P = 0, and 0 * V is NaN where V is
+// not finite.  The shapes do not look: an item whose rows come out not finite while keys are
+// hidden from some of them is done over in the narrow shape with EXACT true.  There V
+// enters the product with zeros in place of what is not finite, and a second product of
+// marks with the rows' visibility (1 or 0) counts what each row sees: +inf is 1, -inf is 128,
+// NaN both; sums over a tile's 64 keys stay exact in float32, and 128 keys of one kind would
+// be needed for a carry.  A weight too small for float32 counts as positive.
+constexpr u32 kMarkUp = 1, kMarkDown = 128;
+
+__device__ __forceinline__ void ar_marks_bf16(u32 w, u32* fin, u32* mark) {
+  *fin = *mark = 0;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    const int d = lane * kE + e;
-    q[e] = p.q_f32 ? reinterpret_cast<const float*>(qr)[d]
-                   : bf16_lo(reinterpret_cast<const unsigned short*>(qr)[d]);
-    if (p.q_f32 && KV != kArF32) q[e] = bf16_lo(f32_to_bf16_bits(q[e]));
-    if (p.q_flip) q[e] = -q[e];
-    acc[e] = 0.f;
+  for (int s = 0; s < 32; s += 16) {
+    const u32 x = (w >> s) & 0xffffu;
+    const bool bad = (x & 0x7f80u) == 0x7f80u;
+    // 1.0, 128.0 and 129.0 as bf16
+    const u32 m = x == 0x7f80u ? 0x3f80u : x == 0xff80u ? 0x4300u : 0x4301u;
+    *fin |= (bad ? 0u : x) << s;
+    *mark |= (bad ? m : 0u) << s;
   }
-  const int lim = ar_limit(it, it.tok0 + r / p.group);
-  for (int key = it.k_lo; key < lim; ++key) {
-    const int lp = key / kv.page_rows;
-    int pg = lp;
-    if (kv.table) pg = lp < kv.bt_cols ? it.table[lp] : -1;
-    if (pg < 0 || pg >= kv.n_pages) continue;
-    const int in = key - lp * kv.page_rows;
-    const char* kr = kv.k + it.head * kv.k_head + it.row0 * kv.k_tok + (int64_t)pg * kv.k_page + (int64_t)in * kv.k_tok;
-    const char* vr = kv.v + it.head * kv.v_head + it.row0 * kv.v_tok + (int64_t)pg * kv.v_page + (int64_t)in * kv.v_tok;
-    float s = 0.f, v[kE], ks = 1.f, vs = 1.f;
-    if constexpr (KV == kArFp8) {
-      ks = kv.k_scale[(int64_t)pg * kv.scale_page + it.head];
-      vs = kv.v_scale[(int64_t)pg * kv.scale_page + it.head];
-    }
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const int d = lane * kE + e;
-      float kx;
-      if constexpr (KV == kArF32) {
-        kx = reinterpret_cast<const float*>(kr)[d];
-        v[e] = reinterpret_cast<const float*>(vr)[d];
-      } else if constexpr (KV == kArBf16) {
-        kx = bf16_lo(reinterpret_cast<const unsigned short*>(kr)[d]);
-        v[e] = bf16_lo(reinterpret_cast<const unsigned short*>(vr)[d]);
-      } else {
-        kx = __builtin_amdgcn_cvt_f32_fp8((int)(unsigned char)kr[d], 0);
-        v[e] = __builtin_amdgcn_cvt_f32_fp8((int)(unsigned char)vr[d], 0);
-      }
-      s += q[e] * kx;
-    }
-    s = wave_sum(s) * ks * p.scale_log2;
-    const float mn = fmaxf(m, s), mu = mn == kNegInf ? 0.f : mn;
-    const float a = exp2f(m - mu), w = exp2f(s - mu);
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) acc[e] = acc[e] * a + w * vs * v[e];
-    m = mn;
-  }
-  if (it.part_ml) {
-    if (lane == 0) {
-      it.part_ml[2 * r] = m;
-      it.part_ml[2 * r + 1] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < kE; ++e) it.part_acc[(int64_t)r * D + lane * kE + e] = acc[e];
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    const int64_t at = ar_out_row(p, it, r, D) + lane * kE + e;
-    const float x = acc[e] * inv;
-    if (p.out_f32)
-      reinterpret_cast<float*>(p.out)[at] = x;
-    else
-      reinterpret_cast<unsigned short*>(p.out)[at] = f32_to_bf16_bits(x);
-  }
+}
+__device__ __forceinline__ void ar_marks_f32(float x, float* fin, float* mark) {
+  const bool bad = !(__builtin_fabsf(x) < __builtin_huge_valf());
+  const float m = x == __builtin_huge_valf() ? kMarkUp : x == kNegInf ? kMarkDown : kMarkUp + kMarkDown;
+  *fin = bad ? 0.f : x;
+  *mark = bad ? m : 0.f;
+}
+// an accumulator and the marks its row saw
+__device__ __forceinline__ float ar_marked(float o, float marks) {
+  const u32 n = (u32)marks;
+  if (n % kMarkDown) o += __builtin_huge_valf();
+  if (n / kMarkDown) o += kNegInf;
+  return o;
 }
 
 // ------------------------------------------------------------------ wide
 
+// returns whether the item has to be done over (the same in every thread)
 template <int KV, int D>
-__device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, char* smem) {
+__device__ __forceinline__ bool ar_wide(const ArParams& p, const ArItem& it, char* smem) {
   using S = ArShape<KV, D>;
   constexpr int kDb = D / 32;                                // 32-dim blocks of O^T
   constexpr int kQ = KV == kArF32 ? D / 8 : D / 16;          // q operands per lane
-  ArLoader<KV, D> ld(p.kv, it);
+  ArLoader<KV, D> ld(p.kv, it, false);
   const int lane = ld.lane, wave = ld.wave, h = lane >> 5, c = lane & 31;
   const int r = wave * 32 + c;
   const bool row_live = r < it.n_rows, wave_live = wave * 32 < it.n_rows;
@@ -441,7 +407,6 @@ __device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, cha
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m = kNegInf, l = 0.f;
-  bool mixed = false, bad_before = false;
 
   // LDS offsets: key row c of a 32-key block; V rows and columns of the transposing read
   const int fk = ar_swizzle<KV, D>(c) ^ h;
@@ -532,15 +497,6 @@ __device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, cha
       }
       const bool holes = tb < it.k_lo || tb + kArTile > it.k_hi || __ballot(pg < 0) != 0;
       if (holes || tb + kArTile > lim_min) {
-        if (!mixed && tb + kArTile > lim_min) {
-          mixed = true;
-          float x = 0.f;
-#pragma unroll
-          for (int d = 0; d < kDb; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x += 0.f * o[d][i];
-          bad_before = half_sum(x) != 0.f;
-        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const bool gone = __builtin_amdgcn_readlane(pg, g) < 0;
@@ -618,58 +574,54 @@ __device__ __forceinline__ void ar_wide(const ArParams& p, const ArItem& it, cha
     }
     if (t + 1 < n_tiles) ld.commit(nxt);
   }
-  if (!wave_live) return;
-  l = half_sum(l);
-  unsigned long long redo = 0;
-  if (mixed) {
-    float x = 0.f;
+  float x = 0.f;  // (0, or NaN: a value of the row is not finite)
+  if (it.k_hi > lim_min) {
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) x += 0.f * o[d][i];
-    x = half_sum(x);
-    redo = __ballot(row_live && !(x == 0.f) && !bad_before) & 0xffffffffull;
   }
-  const bool again = (redo >> c) & 1;
-  if (row_live && !again) {
-    if (it.part_ml) {
-      if (h == 0) *reinterpret_cast<f32x2_t*>(it.part_ml + 2 * r) = f32x2_t{m, l};
+  if (__syncthreads_or(row_live && !(x == 0.f))) return true;
+  if (!wave_live) return false;
+  l = half_sum(l);
+  if (!row_live) return false;
+  const int lane_out = ar_anew(lane), h_out = lane_out >> 5, r_out = wave * 32 + (lane_out & 31);
+  if (it.part_ml) {
+    if (h_out == 0) *reinterpret_cast<f32x2_t*>(it.part_ml + 2 * r_out) = f32x2_t{m, l};
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
+    for (int d = 0; d < kDb; ++d)
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-          *reinterpret_cast<f32x4_t*>(it.part_acc + (int64_t)r * D + 32 * d + 8 * a + 4 * h) =
-              f32x4_t{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]};
-    } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = ar_out_row(p, it, r, D);
+      for (int a = 0; a < 4; ++a)
+        *reinterpret_cast<f32x4_t*>(it.part_acc + (int64_t)r_out * D + 32 * d + 8 * a + 4 * h_out) =
+            f32x4_t{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]};
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t at = ar_out_row(p, it, r_out, D);
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
+    for (int d = 0; d < kDb; ++d)
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          float x[4];
+      for (int a = 0; a < 4; ++a) {
+        float x[4];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) x[b] = o[d][4 * a + b] * inv;
-          ar_store4(p, at + 32 * d + 8 * a + 4 * h, x);
-        }
-    }
+        for (int b = 0; b < 4; ++b) x[b] = o[d][4 * a + b] * inv;
+        ar_store4(p, at + 32 * d + 8 * a + 4 * h_out, x);
+      }
   }
-  while (redo) {
-    const int rr = __builtin_ctzll(redo);
-    redo &= redo - 1;
-    ar_row_by_key<KV, D>(p, it, wave * 32 + rr, lane);
-  }
+  return false;
 }
 
 // ------------------------------------------------------------------ narrow
 
-template <int KV, int D, int NRB>
-__device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, char* smem) {
+// the rows row0 .. row0 + 16 NRB - 1 of the item; returns whether they have to be done over
+// (EXACT false; the same in every thread)
+template <int KV, int D, int NRB, bool EXACT>
+__device__ __forceinline__ bool ar_narrow(const ArParams& p, const ArItem& it, char* smem, float (*ml)[kArNarrow][2],
+                                          int row0) {
   using S = ArShape<KV, D>;
   constexpr int kDb = D / 16;
   constexpr int kQ = KV == kArF32 ? D / 16 : D / 32;
   static_assert(S::kSmem >= 4 * NRB * 16 * D * 4, "the waves' accumulators meet in the tiles' LDS");
-  ArLoader<KV, D> ld(p.kv, it);
+  ArLoader<KV, D> ld(p.kv, it, EXACT);
   const int lane = ld.lane, wave = ld.wave, g4 = lane >> 4, c = lane & 15;
   bf16x8_t qb[NRB][KV == kArF32 ? 1 : kQ];
   f32x4_t qf[NRB][KV == kArF32 ? kQ : 1];
@@ -677,7 +629,7 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
   int lo_lim = it.k_hi;
 #pragma unroll
   for (int b = 0; b < NRB; ++b) {
-    const int r = b * 16 + c;
+    const int r = row0 + b * 16 + c;
     const bool live = r < it.n_rows;
     limit[b] = live ? ar_limit(it, it.tok0 + r / p.group) : it.k_hi;
     lo_lim = limit[b] < lo_lim ? limit[b] : lo_lim;
@@ -781,6 +733,7 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
           s[b][i] = __builtin_amdgcn_exp2f(s[b][i] - mu);
           l[b] += s[b][i];
           if constexpr (KV == kArFp8) s[b][i] *= vs;
+          if constexpr (EXACT) s[b][i] = kw + 4 * g4 + i < limit[b] ? s[b][i] : 0.f;
         }
         if constexpr (KV != kArF32) {
           w[b][0] = pack_bf16x2(s[b][0], s[b][1]);
@@ -789,7 +742,44 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
       }
 #pragma unroll
       for (int d = 0; d < kDb; ++d) {
-        if constexpr (KV == kArF32) {
+        if constexpr (EXACT) {
+          auto sees = [&](int b, int i) { return kw + 4 * g4 + i < limit[b]; };
+          f32x4_t marks[NRB];
+#pragma unroll
+          for (int b = 0; b < NRB; ++b) marks[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          if constexpr (KV == kArF32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = wave * 16 + 4 * g4 + i;
+              const int ch = (4 * d + (c >> 2)) ^ ar_swizzle<KV, D>(row);
+              float x = *reinterpret_cast<const float*>(vt + row * S::kRowBytes + ch * 16 + 4 * (c & 3)), mark;
+              ar_marks_f32(x, &x, &mark);
+#pragma unroll
+              for (int b = 0; b < NRB; ++b) {
+                o[b][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[b][i], o[b][d], 0, 0, 0);
+                marks[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(mark, sees(b, i) ? 1.f : 0.f, marks[b], 0, 0, 0);
+              }
+            }
+          } else {
+            const u32x2_t x = ar_read_tr(vt + v_off + (((2 * d) ^ vc0) << 4));
+            u32 fin[2], mark[2];
+            ar_marks_bf16(x[0], &fin[0], &mark[0]);
+            ar_marks_bf16(x[1], &fin[1], &mark[1]);
+#pragma unroll
+            for (int b = 0; b < NRB; ++b) {
+              const u32 s0 = (sees(b, 0) ? 0x3f80u : 0u) | (sees(b, 1) ? 0x3f800000u : 0u);
+              const u32 s1 = (sees(b, 2) ? 0x3f80u : 0u) | (sees(b, 3) ? 0x3f800000u : 0u);
+              o[b][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_i16x4(fin[0], fin[1]), as_i16x4(w[b][0], w[b][1]),
+                                                                  o[b][d], 0, 0, 0);
+              marks[b] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_i16x4(mark[0], mark[1]), as_i16x4(s0, s1),
+                                                                   marks[b], 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < NRB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[b][d][i] = ar_marked(o[b][d][i], marks[b][i]);
+        } else if constexpr (KV == kArF32) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = wave * 16 + 4 * g4 + i;
@@ -811,8 +801,19 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
   }
   // the four waves' partials meet in LDS: acc [4][16 NRB][D], then every thread sums its
   // elements in wave order
-  __shared__ float ml[4][NRB * 16][2];
-  __syncthreads();
+  bool again = false;
+  if (!EXACT && it.k_hi > lim_min) {
+#pragma unroll
+    for (int b = 0; b < NRB; ++b) {
+      float x = 0.f;  // (0, or NaN: a value of the row is not finite)
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x += 0.f * o[b][d][i];
+      again |= row0 + b * 16 + c < it.n_rows && !(x == 0.f);
+    }
+  }
+  if (__syncthreads_or(again)) return true;
   float* acc = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int b = 0; b < NRB; ++b) {
@@ -827,30 +828,25 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
       *reinterpret_cast<f32x4_t*>(acc + ((wave * NRB * 16 + r) * D + 16 * d + 4 * g4)) = o[b][d];
   }
   __syncthreads();
-  const bool mixed = it.k_hi > lim_min;
-  for (int r = wave; r < it.n_rows; r += 4) {
+  for (int i = wave; i < NRB * 16 && row0 + i < it.n_rows; i += 4) {
+    const int r = row0 + i;
     float mt = kNegInf;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[w][r][0]);
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[w][i][0]);
     const float mu = mt == kNegInf ? 0.f : mt;
     float a[4], lt = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      a[w] = __builtin_amdgcn_exp2f(ml[w][r][0] - mu);
-      lt += a[w] * ml[w][r][1];
+      a[w] = __builtin_amdgcn_exp2f(ml[w][i][0] - mu);
+      lt += a[w] * ml[w][i][1];
     }
     constexpr int kE = D / 64;
-    float x[kE], bad = 0.f;
+    float x[kE];
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       x[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) x[e] += a[w] * acc[(w * NRB * 16 + r) * D + lane * kE + e];
-      bad += 0.f * x[e];
-    }
-    if (mixed && __ballot(!(bad == 0.f)) != 0) {
-      ar_row_by_key<KV, D>(p, it, r, lane);
-      continue;
+      for (int w = 0; w < 4; ++w) x[e] += a[w] * acc[(w * NRB * 16 + i) * D + lane * kE + e];
     }
     if (it.part_ml) {
       if (lane == 0) *reinterpret_cast<f32x2_t*>(it.part_ml + 2 * r) = f32x2_t{mt, lt};
@@ -868,16 +864,24 @@ __device__ __forceinline__ void ar_narrow(const ArParams& p, const ArItem& it, c
       }
     }
   }
+  return false;
 }
 
 template <int KV, int D>
 __device__ __forceinline__ void ar_attend(const ArParams& p, const ArItem& it, char* smem) {
+  __shared__ float ml[4][kArNarrow][2];
+  bool again;
   if (it.n_rows > kArNarrow)
-    ar_wide<KV, D>(p, it, smem);
+    again = ar_wide<KV, D>(p, it, smem);
   else if (it.n_rows > 16)
-    ar_narrow<KV, D, 2>(p, it, smem);
+    again = ar_narrow<KV, D, 2, false>(p, it, smem, ml, 0);
   else
-    ar_narrow<KV, D, 1>(p, it, smem);
+    again = ar_narrow<KV, D, 1, false>(p, it, smem, ml, 0);
+  if (again)
+    for (int r = 0; r < it.n_rows; r += kArNarrow) {
+      ar_narrow<KV, D, 2, true>(p, it, smem, ml, r);
+      __syncthreads();  // (the rows' sums have been read)
+    }
 }
 
 }  // namespace ia
