@@ -341,7 +341,9 @@ __device__ __forceinline__ int64_t ar_out_row(const ArParams& p, const ArItem& i
 
 // The second pass.  A key hidden from a row meets it with P = 0, and 0 * V is NaN where V is
 // not finite.  The shapes do not look: an item whose rows come out not finite while keys are
-// hidden from some of them is done over in the narrow shape with EXACT true.  There V
+// hidden from some of them is done over in the narrow shape with EXACT true; so is one of
+// the wide shape whose sum l is not finite, where a scale of 0 met a hidden score (-inf,
+// which the narrow shape puts in after the scale).  There V
 // enters the product with zeros in place of what is not finite, and a second product of
 // marks with the rows' visibility (1 or 0) counts what each row sees: +inf is 1, -inf is 128,
 // NaN both; sums over a tile's 64 keys stay exact in float32, and 128 keys of one kind would
@@ -574,7 +576,8 @@ __device__ __forceinline__ bool ar_wide(const ArParams& p, const ArItem& it, cha
     }
     if (t + 1 < n_tiles) ld.commit(nxt);
   }
-  float x = 0.f;  // (0, or NaN: a value of the row is not finite)
+  // 0, or NaN: a sum or a value of the row is not finite
+  float x = 0.f * l;
   if (it.k_hi > lim_min) {
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
