@@ -35,6 +35,7 @@ constexpr int kArNarrow = 32;     // most rows of a narrow one
 constexpr int kArMaxGroup = 64;   // query heads per kv head: a row tile holds at least two tokens
 constexpr int64_t kArMaxGrid = 1 << 23;  // workgroups of a launch (work items are 32 bits)
 constexpr float kArSlack = 8.f;   // log2 units a row's maximum may rise before it is rescaled
+constexpr float kArFar = 65536.f; // log2 units at which a rounded maximum is off by up to 2^-8
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 #define IA_LDS __attribute__((address_space(3)))
@@ -343,7 +344,8 @@ __device__ __forceinline__ int64_t ar_out_row(const ArParams& p, const ArItem& i
 // not finite.  The shapes do not look: an item whose rows come out not finite while keys are
 // hidden from some of them is done over in the narrow shape with EXACT true; so is one of
 // the wide shape whose sum l is not finite, where a scale of 0 met a hidden score (-inf,
-// which the narrow shape puts in after the scale).  There V
+// which the narrow shape puts in after the scale), or whose maximum lies so far out that its
+// own rounding matters (the narrow shape rounds every scaled score alike).  There V
 // enters the product with zeros in place of what is not finite, and a second product of
 // marks with the rows' visibility (1 or 0) counts what each row sees: +inf is 1, -inf is 128,
 // NaN both; sums over a tile's 64 keys stay exact in float32, and 128 keys of one kind would
@@ -576,8 +578,9 @@ __device__ __forceinline__ bool ar_wide(const ArParams& p, const ArItem& it, cha
     }
     if (t + 1 < n_tiles) ld.commit(nxt);
   }
-  // 0, or NaN: a sum or a value of the row is not finite
-  float x = 0.f * l;
+  // 0, or NaN: a sum or a value of the row is not finite, or its scores are too far out for
+  // the products above, which subtract the rounded maximum from the unrounded score
+  float x = m > kArFar || (m < -kArFar && m != kNegInf) ? __builtin_nanf("") : 0.f * l;
   if (it.k_hi > lim_min) {
 #pragma unroll
     for (int d = 0; d < kDb; ++d)

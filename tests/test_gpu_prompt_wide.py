@@ -43,3 +43,51 @@ def test_scale_of_zero_with_a_missing_page(kv, device):
     torch.cuda.synchronize()
     want, mag = reference_heads(q, k[keep], v[keep], total - 16 - new, 0.0)
     check(out, want, mag, kv, total, kv)
+
+
+def far_scores(device, n, hq, d, kv, top, negative):
+    """q and k whose scores of token j are ``+-64 * 2^top * b[j]`` exactly, b distinct bf16
+    values in [1, 2): neighbours differ by 2^(top - 1) or more, so that a row's softmax is
+    one at its largest score and zero elsewhere to any precision."""
+    q = torch.zeros((n, hq, d), device=device, dtype=DT[kv])
+    q[..., :64] = 2.0 ** (top // 2)
+    order = torch.randperm(128, generator=torch.Generator().manual_seed(top))[:n]
+    b = (1 + order.float() / 128).to(device)
+    k = torch.zeros((n, 1, d), device=device, dtype=DT[kv])
+    k[..., :64] = (b * 2.0 ** (top - top // 2) * (-1 if negative else 1))[:, None, None].to(DT[kv])
+    best = [max(range(i + 1), key=lambda j: -int(order[j]) if negative else int(order[j])) for i in range(n)]
+    return q, k, best
+
+
+@pytest.mark.parametrize("negative", [False, True])
+@pytest.mark.parametrize("top", [11, 28, 60])
+@pytest.mark.parametrize("kv,d,hq", [("bf16", 128, 64), ("bf16", 64, 40), ("f32", 64, 64), ("bf16", 128, 4)])
+def test_scores_far_out(kv, d, hq, top, negative, device):
+    """Finite scores from 2^17 to 2^67 in size: every row is the value at its largest score.
+    ``scale`` 1: log2 units are 1.44 times the scores, gaps at least 2^10."""
+    announce(f"far scores {kv} {d} {hq} 2^{top} {negative}")
+    n = 100
+    q, k, best = far_scores(device, n, hq, d, kv, top, negative)
+    v = torch.randn((n, 1, d), device=device).to(DT[kv])
+    cu = i32(device, [0, n])
+    out = ia.prompt_attention(q, k, v, cu, scale=1.0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, v[best].expand(n, hq, d))
+
+
+def test_far_scores_in_pages_and_prefixes(device):
+    """The same through the pool: a single token of 64 heads, and a group of nine sequences."""
+    announce("far scores, pages")
+    n, d, page = 100, 128, 16
+    q, k, best = far_scores(device, n, 64, d, "bf16", 40, False)
+    v = torch.randn((n, 1, d), device=device).to(torch.bfloat16)
+    pk, pv = (torch.nn.functional.pad(x, (0, 0, 0, 0, 0, 12)).view(7, page, 1, d).transpose(1, 2) for x in (k, v))
+    table = torch.arange(7, device=device, dtype=torch.int32)[None]
+    out = ia.paged_prompt_attention(q[:1], pk, pv, table, i32(device, [n]), i32(device, [0, 1]), scale=1.0, workspace={})
+    lens = [100, 97, 100, 98, 100, 99, 100, 100, 97]
+    many = ia.shared_prefix_decode(q[:9, :8], pk, pv, table.expand(9, 7).contiguous(), i32(device, lens),
+                                   i32(device, [0, 9]), i32(device, [97]), scale=1.0, workspace={})
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], v[best[n - 1]].expand(64, d))
+    for b, m in enumerate(lens):
+        assert torch.equal(many[b], v[best[m - 1]].expand(8, d)), b
