@@ -574,6 +574,7 @@ IA_API int ia_paged_prompt_attention(const ia_prompt_shape* shape, const void* q
  * group's prefix attends its own tokens only; where the first sequence is shorter, the
  * prefix ends there.  Query heads as in ia_prompt_shape: any number up to 64 per kv head.
  * out: [batch, n_q_heads, D] contiguous, out_dtype; a sequence of no tokens gives zeros.
+ * At most 32768 sequences and as many groups (the plan grows with the square of the batch).
  * Two launches: the items, planned from the device's lengths, and their merge.  The
  * workspace (ia_shared_prefix_workspace_size bytes) needs no initialisation.  No counterpart in
  * the reference, whose K/V is per sequence.

@@ -257,7 +257,7 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
     through the block-table row of the group's first sequence, the rest through each
     sequence's own row, so forked tables (``fork_sequences``) and tables that repeat the
     prefix in pages of their own give the same.  Any group of query heads up to 64; bf16,
-    float32 and fp8 pools."""
+    float32 and fp8 pools; at most 32768 sequences and as many groups."""
     device_of(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *(scales or ()))
     b = check_ints(seq_lens, "seq_lens")
     kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, b)
