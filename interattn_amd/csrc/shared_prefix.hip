@@ -104,8 +104,10 @@ size_t prefix_layout(const ia_decode_shape* s, int kv_dtype, int n_groups, Prefi
   const int resident = device_cus() * (kv_dtype == IA_F32 ? 1 : 2);
   p->target = std::max(1, resident / s->n_kv_heads);
   p->max_items = p->target + p->n_tiles + s->batch;
-  // a range is cut into at most its share of target, and one more
-  p->rows = (int64_t)(p->n_tiles ? p->target + p->n_tiles : 0) * kArRows + (int64_t)(p->target + s->batch) * group;
+  // Every range has an item (a sequence is in one row tile and has its own tokens), and cuts
+  // add at most target more, of a whole tile's rows where there are tiles.
+  const int64_t most = n_groups ? std::min(p->tile_seqs, s->batch) : 1;
+  p->rows = ((n_groups ? 2 : 1) * (int64_t)s->batch + p->target * most) * group;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     char* x = ws ? ws + at : nullptr;

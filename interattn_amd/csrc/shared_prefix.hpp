@@ -207,8 +207,10 @@ __device__ __forceinline__ bool prefix_plan(const PrefixParams& p, int want, cha
       base += wave_n[w];
       rows0 += wave_rows[w];
     }
-    if (blockIdx.x == 0 && e < n) p.entries[e] = PrefixEntry{row, items, rows, 0};
-    if (want >= at && want < at + items) {
+    // (starts that decrease put a sequence in several tiles: past the partials' room, none)
+    const bool room = row + items * rows <= p.rows;
+    if (blockIdx.x == 0 && e < n) p.entries[e] = PrefixEntry{row, room ? items : 0, rows, 0};
+    if (want >= at && want < at + items && room) {
       const int i = want - at, per = (t + items - 1) / items, tb = r.k_lo & ~15;
       const int lo = tb + i * per * kArTile, hi = lo + per * kArTile;
       found[0] = r.tok0;

@@ -268,11 +268,15 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
     n_groups = check_ints(shared_lens, "shared_lens")
     check_ints(group_starts, "group_starts", n_groups + 1)
     out = output(q, out, out_dtype, workspace, "attention_output")
-    shape = N.DecodeShape(b, hq, hkv, d, rows.q_token_stride, rows.q_head_stride, rows.q_dtype)
-    key = ("shared_prefix_scratch", b, n_groups, hkv, hq, d, kv.dtype)
+    shape_tail = hq, hkv, d, rows.q_token_stride, rows.q_head_stride, rows.q_dtype
+    shape = N.DecodeShape(b, *shape_tail)
+    # one buffer for every batch and group count up to a power of two: a later, larger call
+    # never replaces one that a captured graph uses, and a server whose batch changes keeps few
+    cap = 1 << (max(b, n_groups, 64) - 1).bit_length()
+    key = ("shared_prefix_scratch", q.get_device(), cap, hkv, hq, d, kv.dtype)
     ws = None if workspace is None else workspace.get(key)
-    if ws is None or ws.get_device() != q.get_device():
-        need = N.lib().ia_shared_prefix_workspace_size(shape, kv.dtype, n_groups)
+    if ws is None:
+        need = N.lib().ia_shared_prefix_workspace_size(N.DecodeShape(cap, *shape_tail), kv.dtype, cap)
         ws = workspace_tensor(workspace, key, (max(need, 1),), device=q.device, dtype=torch.uint8)
     launch(N.lib().ia_shared_prefix_decode, q, shape, q.data_ptr(), kv, seq_lens.data_ptr(), group_starts.data_ptr(),
            shared_lens.data_ptr(), n_groups, d ** -0.5 if scale is None else float(scale), out.data_ptr(),

@@ -14,3 +14,17 @@ def test_prefix_batches_whose_plan_would_hold_the_device_are_refused(kw):
     size = N.lib().ia_shared_prefix_workspace_size
     assert size(struct(N.DecodeShape, DECODE, **kw.get("shape", {})), N.IA_BF16, kw.get("groups", 1)) == 0
     assert size(struct(N.DecodeShape, DECODE, batch=32768), N.IA_BF16, 32768) > 0
+
+
+def test_prefix_scratch_is_what_its_partials_need():
+    """Two partial rows for each query row, and what the cuts add: at most 64 items of 128
+    rows per kv head (512 workgroups of 8 heads)."""
+    size = lambda batch, groups: N.lib().ia_shared_prefix_workspace_size(  # noqa: E731
+        struct(N.DecodeShape, DECODE, batch=batch, n_q_heads=32, n_kv_heads=8), N.IA_BF16, groups)
+    row = 8 * 130 * 4  # eight heads' (acc, m, l)
+    for batch, groups in ((1, 0), (32, 1), (64, 8), (512, 256), (4096, 4096)):
+        rows = 2 * 4 * batch + 64 * 128
+        plan = 16 * (batch + batch // 32 + groups)
+        assert size(batch, groups) <= rows * row + plan + 4 * 256, (batch, groups)
+    # more of either never needs less
+    assert size(40, 3) <= size(64, 64) <= size(65, 64) and size(64, 64) <= size(64, 65)
