@@ -4,8 +4,10 @@ paged pool that holds them.
 Packed rows put the sequences of a batch one behind the other with no padding:
 ``cu_seqlens [n_seq + 1] int32`` on the device holds the first row of each, and the end of
 the last.  Pools, block tables and scales are those of ``ops``.  Calls launch on the
-current stream of their tensors' device, never synchronise, and keep scratch and output in
-the caller's ``workspace`` dict; calls that share one must not overlap.
+current stream of their tensors' device, never synchronise, and keep scratch in the caller's
+``workspace`` dict; calls that share one must not overlap.  An output is a new tensor unless
+``out`` is given: batches differ from call to call, and a kept buffer of another size would
+be replaced under a captured graph that writes it.
 """
 
 import functools
@@ -139,10 +141,10 @@ def _pool(pool_k, pool_v, block_table, scales, n_seq):
     return kv, hkv, d
 
 
-def output(q, out, out_dtype, workspace, key):
-    """The caller's ``out`` or the workspace's, ``q``'s shape, contiguous."""
+def output(q, out, out_dtype):
+    """The caller's ``out`` or a new tensor, ``q``'s shape, contiguous."""
     if out is None:
-        return workspace_tensor(workspace, key, q.shape, device=q.device, dtype=out_dtype or q.dtype)
+        return torch.empty(q.shape, device=q.device, dtype=out_dtype or q.dtype)
     if out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {list(q.shape)} tensor")
     if out.dtype not in (_F32, _BF16) or (out_dtype is not None and out.dtype != out_dtype):
@@ -182,7 +184,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None, out_dtype=Non
     shape = _prompt_shape(q, _n_seq(cu_seqlens), hkv, d)
     if shape.n_tokens != tokens:
         raise ValueError("k and v must have q's tokens")
-    out = output(q, out, out_dtype, workspace, "prompt_output")
+    out = output(q, out, out_dtype)
     if tokens == 0:
         return out
     ws = _workspace(shape, kv.dtype, tokens, workspace, q.device)
@@ -206,7 +208,7 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, n_seq)
     shape = _prompt_shape(q, n_seq, hkv, d)
     check_ints(seq_lens, "seq_lens", n_seq)
-    out = output(q, out, out_dtype, workspace, "prompt_output")
+    out = output(q, out, out_dtype)
     if shape.n_tokens == 0:
         return out
     cap = (kv.bt_cols if block_table is not None else kv.n_pages) * kv.page_size
@@ -267,7 +269,7 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
         raise ValueError("q must have a row for each sequence")
     n_groups = check_ints(shared_lens, "shared_lens")
     check_ints(group_starts, "group_starts", n_groups + 1)
-    out = output(q, out, out_dtype, workspace, "attention_output")
+    out = output(q, out, out_dtype)
     shape_tail = hq, hkv, d, rows.q_token_stride, rows.q_head_stride, rows.q_dtype
     shape = N.DecodeShape(b, *shape_tail)
     # one buffer for every batch and group count up to a power of two: a later, larger call
