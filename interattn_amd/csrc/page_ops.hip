@@ -438,7 +438,10 @@ int check_tensors(const ia_page_tensor* t, int n) {
 }
 
 int check_state(const ia_page_state* s, Table* t, bool lens = true) {
-  if (!s || !s->block_table || (lens && !s->seq_lens) || !s->refs) return fail(IA_ERR_INVALID, "null pointer argument");
+  // (arrays without entries have no address)
+  if (!s || (!s->block_table && s->rows > 0 && s->cols > 0) || (lens && !s->seq_lens && s->rows > 0) ||
+      (!s->refs && s->n_pages > 0))
+    return fail(IA_ERR_INVALID, "null pointer argument");
   if (s->rows < 0 || s->cols < 0 || s->bt_stride < s->cols || s->n_pages < 0 || s->page_size <= 0)
     return fail(IA_ERR_INVALID, "page state: rows, cols, n_pages >= 0, bt_stride >= cols, page_size > 0");
   if (s->n_pages > INT32_MAX - 4) return fail(IA_ERR_UNSUPPORTED, "too many pages");

@@ -105,7 +105,9 @@ extern "C" int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* ro
                                    const int32_t* seq_lens, int32_t* new_seq_lens, int32_t n_seq, int32_t n_tokens,
                                    int32_t n_kv_heads, int32_t head_dim, void* stream) {
   using namespace ia;
-  if (!rows || !cu_seqlens || !seq_lens || !new_seq_lens) return fail(IA_ERR_INVALID, "null pointer argument");
+  // (arrays without entries have no address)
+  if (!rows || (n_seq > 0 && (!cu_seqlens || !seq_lens || !new_seq_lens)))
+    return fail(IA_ERR_INVALID, "null pointer argument");
   if (head_dim != 64 && head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   if (kv && kv->dtype != IA_F32 && kv->dtype != IA_BF16)
     return fail(IA_ERR_UNSUPPORTED, "append takes bf16 or f32 pools");
@@ -114,7 +116,7 @@ extern "C" int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* ro
   if (rows->dtype != kv->dtype) return fail(IA_ERR_INVALID, "the new rows must have the pool's dtype");
   if (n_seq < 0 || n_tokens < 0 || n_kv_heads <= 0) return fail(IA_ERR_INVALID, "sequence, token or head counts");
   if (n_tokens > 0 && (!rows->k || !rows->v)) return fail(IA_ERR_INVALID, "null pointer argument");
-  if (new_seq_lens == seq_lens) return fail(IA_ERR_INVALID, "new_seq_lens must not be seq_lens");
+  if (n_seq > 0 && new_seq_lens == seq_lens) return fail(IA_ERR_INVALID, "new_seq_lens must not be seq_lens");
   const int eb = kv->dtype == IA_F32 ? 4 : 2;
   const int64_t strides[4] = {rows->k_token_stride, rows->k_head_stride, rows->v_token_stride, rows->v_head_stride};
   for (int64_t s : strides)

@@ -139,12 +139,12 @@ int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, const i
   if (rc) return rc;
   rc = check_kv(kv, shape->head_dim);
   if (rc) return rc;
+  if (shape->batch == 0) return IA_OK;  // (arrays without entries have no address)
   if (!seq_lens || (n_groups && (!group_starts || !shared_lens))) return fail(IA_ERR_INVALID, "null pointer argument");
   PrefixParams p{};
   rc = set_ar_params(&p.ar, q, shape->q_dtype, shape->q_batch_stride, shape->q_row_stride,
                      shape->n_q_heads / shape->n_kv_heads, shape->n_kv_heads, kv->dtype, scale, out, out_dtype);
   if (rc) return rc;
-  if (shape->batch == 0) return IA_OK;
   const size_t need = prefix_layout(shape, kv->dtype, n_groups, &p, nullptr);
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(IA_ERR_WORKSPACE, "workspace missing, too small or not 256-byte aligned: " + std::to_string(need) +

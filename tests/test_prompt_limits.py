@@ -4,7 +4,7 @@ followed)."""
 import pytest
 
 from interattn_amd import _native as N
-from tests.test_prompt_refusals import DECODE, prefix_call, refused, struct
+from tests.test_prompt_refusals import BIG, DECODE, KV, P, STATE, append_call, prefix_call, refused, struct
 
 
 @pytest.mark.parametrize("kw", [dict(shape=dict(batch=32769)), dict(shape=dict(batch=1 << 19)), dict(groups=32769),
@@ -28,3 +28,17 @@ def test_prefix_scratch_is_what_its_partials_need():
         assert size(batch, groups) <= rows * row + plan + 4 * 256, (batch, groups)
     # more of either never needs less
     assert size(40, 3) <= size(64, 64) <= size(65, 64) and size(64, 64) <= size(64, 65)
+
+
+def test_arrays_without_entries_may_be_null():
+    lib = N.lib()
+    none = struct(N.DecodeShape, DECODE, batch=0)
+    assert lib.ia_shared_prefix_decode(none, None, struct(N.PagedKV, KV), None, None, None, 0, 0.1, None, N.IA_BF16,
+                                       None, 0, None) == N.IA_OK
+    assert append_call(cu=None, seq=None, new=None, n_seq=0) == N.IA_OK
+    for kw in (dict(rows=0, block_table=None, seq_lens=None), dict(rows=0, block_table=None, seq_lens=None, n_pages=0,
+                                                                   refs=None)):
+        assert lib.ia_reserve_pages(struct(N.PageState, STATE, **kw), None, None, None, 0, None) == N.IA_OK
+        assert lib.ia_free_sequences(struct(N.PageState, STATE, **kw), None, 0, None) == N.IA_OK
+    for kw in (dict(block_table=None), dict(seq_lens=None), dict(refs=None)):
+        refused(lib.ia_reserve_pages(struct(N.PageState, STATE, **kw), P, P, P, BIG, None), N.IA_ERR_INVALID, "null")
