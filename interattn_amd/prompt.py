@@ -135,7 +135,8 @@ def _pool(pool_k, pool_v, block_table, scales, n_seq):
     kv = N.PagedKV.from_buffer_copy(held)
     kv.k, kv.v = pool_k.data_ptr(), pool_v.data_ptr()
     if block_table is not None:
-        kv.block_table = block_table.data_ptr()
+        # (one of no columns has no address; null would be the identity table)
+        kv.block_table = block_table.data_ptr() or kv.k
     if kv.dtype == N.IA_FP8_E4M3:
         kv.k_scale, kv.v_scale = ks.data_ptr(), vs.data_ptr()
     return kv, hkv, d

@@ -54,6 +54,21 @@ def test_append_of_nothing(device):
     assert lens.tolist() == [7, 0] and torch.equal(pk, k0) and torch.equal(pv, v0)
 
 
+def test_tables_without_columns_hold_no_token(device):
+    """A table of no columns is not the identity table that None stands for."""
+    announce("tables without columns")
+    pk, pv = pools(device)
+    k0 = pk.clone()
+    t, lens = table(device, 2, 0), i32(device, [20, 0])
+    out = ia.paged_prompt_attention(rows(device, 2, HQ), pk, pv, t, lens, i32(device, [0, 1, 2]))
+    one = ia.shared_prefix_decode(rows(device, 2, HQ), pk, pv, t, lens, i32(device, [0, 2]), i32(device, [16]))
+    new = rows(device, 3, HKV)
+    after = ia.append_prompt_kv(pk, pv, t, i32(device, [0, 0]), new, new, i32(device, [0, 2, 3]))
+    torch.cuda.synchronize()
+    assert bool((out == 0).all()) and bool((one == 0).all())
+    assert after.tolist() == [0, 0] and torch.equal(pk, k0)
+
+
 def test_pages_of_tables_without_rows(device):
     announce("empty page states")
     pk, pv = pools(device)
