@@ -262,7 +262,8 @@ class PagedTopkDecodeRunner:
     top-k layer call (``sparse_topk_decode``); layers below ``full_attention_layers``
     run the HIP paged dense decode.  Prompts of one batch share a length (no
     padding).  With ``native_prompt=True`` the prefill runs ``prompt_attention`` and
-    ``append_prompt_kv`` instead of SDPA and the copy.  Install with
+    ``append_prompt_kv`` instead of SDPA and the copy, except where dropout or gradients
+    are asked for; either way it is causal and reads no ``attention_mask``.  Install with
     ``condition_block_decode_context(runner)``."""
 
     def __init__(self, *, model, batch_size, max_seq_len, block_size, k, forced_first=0, forced_last=0,
@@ -355,7 +356,9 @@ class PagedTopkDecodeRunner:
     def hybrid_attention_forward(self, module, query, key, value, attention_mask, scaling, dropout=0.0, **kwargs):
         layer = self._layer(module)
         if query.shape[2] != 1:
-            if self.native_prompt and not (dropout and module.training):
+            # (prompt_attention is forward only: what dropout or gradients ask for is SDPA's)
+            grad = torch.is_grad_enabled() and any(x.requires_grad for x in (query, key, value))
+            if self.native_prompt and not grad and not (dropout and module.training):
                 return self._prefill_native(layer, query, key, value, scaling)
             self._fill(layer, key, value)
             return _sdpa_prefill_attention_forward(module, query, key, value, attention_mask, scaling=scaling,
