@@ -328,6 +328,8 @@ class PagedTopkDecodeRunner:
         """The prompt on the HIP path: its rows packed, K/V into the pool, attention over them."""
         self._check_prompt(key)
         b, hq, t, d = query.shape
+        if key.shape[2] != t:
+            raise ValueError("the native prefill takes whole prompts: as many keys as queries")
         q, k, v = (x.transpose(1, 2).reshape(b * t, x.shape[1], d) for x in (query, key, value))
         cu = torch.arange(0, (b + 1) * t, max(t, 1), device=query.device, dtype=torch.int32)[:b + 1]
         pk, pv = self.pools[layer]

@@ -72,3 +72,15 @@ def test_without_gradients_both_prefills_agree(device):
     for a, b in zip(*pools):
         a, b = (x.permute(0, 1, 3, 2, 4).reshape(B, -1, HKV, D)[:, :t] for x in (a, b))
         assert torch.equal(a, b)
+
+
+def test_native_prefill_refuses_a_chunk(device):
+    """Keys of cached tokens besides the new ones: refused before anything is written."""
+    announce("runner, chunk")
+    r, module = runner(device, True)
+    q, k, v = inputs(device, 20, False)
+    before = [p.clone() for p in r.pools[0]]
+    with pytest.raises(ValueError, match="whole prompts"):
+        r.hybrid_attention_forward(module, q[:, :, 12:], k, v, None, D ** -0.5)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, r.pools[0])) and r.seq_lens[0].tolist() == [0] * B
