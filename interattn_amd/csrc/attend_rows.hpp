@@ -284,7 +284,7 @@ __device__ __forceinline__ int wave_min_i32(int v) {
 
 __device__ __forceinline__ int ar_limit(const ArItem& it, int tok) {
   const int lim = it.lens ? it.lens[tok] : it.limit0 + (tok - it.tok0);
-  return lim < it.k_hi ? lim : it.k_hi;
+  return lim < 0 ? 0 : lim < it.k_hi ? lim : it.k_hi;  // (0: its negative exists, unlike INT32_MIN's)
 }
 
 __device__ __forceinline__ const char* ar_q_row(const ArParams& p, const ArItem& it, int r) {

@@ -6,7 +6,7 @@ import torch
 
 import interattn_amd as ia
 from tests._util import announce
-from tests.test_gpu_prompt_attention import DT, check, gather, packed, paged
+from tests.test_gpu_prompt_attention import DT, check, gather, packed, paged, reference
 from tests.test_gpu_prompt_edges import i32, reference_heads
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +91,22 @@ def test_far_scores_in_pages_and_prefixes(device):
     assert torch.equal(out[0], v[best[n - 1]].expand(64, d))
     for b, m in enumerate(lens):
         assert torch.equal(many[b], v[best[m - 1]].expand(8, d)), b
+
+
+@pytest.mark.parametrize("low", [-1, -2 ** 31])
+def test_negative_lengths_leave_the_other_members_alone(low, device):
+    announce(f"negative length {low}")
+    hkv, hq, d, page, shared = 1, 8, 64, 16, 96
+    lens = [120, low, 110, 101, 97, low, 100, 120, 99]
+    pk, pv, _, table = paged(device, [120] * 9, hkv, d, page, "bf16", "split", 13)
+    table[:, :6] = table[0, :6].clone()
+    q = torch.randn((9, hq, d), device=device).to(torch.bfloat16)
+    out = ia.shared_prefix_decode(q, pk, pv, table, i32(device, lens), i32(device, [0, 9]), i32(device, [shared]),
+                                  workspace={})
+    torch.cuda.synchronize()
+    for b, n in enumerate(lens):
+        if n < 0:
+            assert bool((out[b] == 0).all())
+            continue
+        want, mag = reference(q[b:b + 1], gather(pk, None, table[b], n), gather(pv, None, table[b], n), n - 1, d ** -0.5)
+        check(out[b:b + 1], want, mag, "bf16", n, b)
