@@ -551,8 +551,9 @@ typedef struct ia_packed_kv {
  *
  * Few rows over many keys are cut along the keys and merged in a second launch, for which
  * the workspace holds partials: ia_prompt_attention_workspace_size bytes (0 where nothing
- * is cut, else one size per device, kv_dtype and head_dim) with max_keys the keys a sequence can have (n_tokens for packed K/V, else what
- * the pool's table can hold).  Its contents need no initialisation.
+ * is cut, else one size per device, kv_dtype and head_dim) with max_keys the keys a
+ * sequence can have (n_tokens for packed K/V, else what the pool's table can hold).  Its
+ * contents need no initialisation.
  */
 IA_API size_t ia_prompt_attention_workspace_size(const ia_prompt_shape* shape, int32_t kv_dtype, int64_t max_keys);
 IA_API int ia_prompt_attention(const ia_prompt_shape* shape, const void* q, const ia_packed_kv* kv,

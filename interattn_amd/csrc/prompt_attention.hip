@@ -15,7 +15,7 @@ __global__ __launch_bounds__(kArThreads) void ia_prompt_merge(PromptParams p) {
   if (t.n_tok == 0) return;
   int limit0, k_end;
   prompt_keys(p, t, &limit0, &k_end);
-  const int n = prompt_slices((k_end + kArTile - 1) / kArTile, p.slices);
+  const int n = prompt_slices(p, (k_end + kArTile - 1) / kArTile);
   if (n <= 1) return;
   const int64_t slot = ((int64_t)tile * p.ar.n_kv_heads + head) * p.slices;
   ArItem it{};
@@ -47,6 +47,12 @@ namespace {
 
 constexpr int kPromptMaxSlices = 64;
 
+// Fewest key tiles a slice is worth.  Merging 128 rows takes as long as ten key tiles of
+// bf16 or fp8 products (1,000 tokens in halves of 8 tiles 50 us, uncut 33), but as two of
+// float32's (eight of 1-500 tokens at 0-1,500 keys: 8 tiles 79, 16 tiles 104); with tiles of
+// 32 rows, 16 instead of 8 took 33 us for 27 (16 tokens at 4,000 keys).
+int least_key_tiles(int kv_dtype, int rows) { return rows == kArNarrow || kv_dtype == IA_F32 ? 8 : 16; }
+
 int check_prompt_shape(const ia_prompt_shape* s) {
   if (!s) return fail(IA_ERR_INVALID, "shape is null");
   if (s->n_seq < 0 || s->n_tokens < 0 || s->n_q_heads <= 0 || s->n_kv_heads <= 0)
@@ -62,32 +68,47 @@ int check_prompt_shape(const ia_prompt_shape* s) {
 int64_t resident_wgs(int kv_dtype) { return (int64_t)device_cus() * (kv_dtype == IA_F32 ? 1 : 2); }
 
 // Row tiles (a bound from the token and sequence counts alone), and the slices their keys
-// may be cut into.  Tiles of 128 rows read K/V least often and keep the matrix cores
-// busiest.  A launch whose tiles of 128 do not fill the device, cut along their keys or
-// not, and whose tiles of 32 rows all run at once takes those: four times the workgroups,
-// each with a quarter of the products.  float32 products are as dense in both shapes, and in
-// tiles of 32 rows a row's keys spread over four waves: always 32.  Then, with fewer tiles
-// than workgroups run at once, every tile is cut along its keys.
+// may be cut into.  Times are of the launches alone, in us, groups of 4, D = 128 unless said.
+//
+// Tiles of 128 rows read K/V least often and keep the matrix cores busiest; tiles of 32
+// rows spread a key tile over four waves, a quarter of the time for each.  They pay where
+// all of them run at once and, over bf16 and fp8 caches, the keys are long enough to be cut
+// but 128-row tiles, cut or not, leave a quarter of the device idle.  bf16, 8 kv heads, 32
+// rows / 128: 16 tokens at 4,000 keys 28 / 35, 64 at 8,000 55 / 95, four of 32 at 2,000
+// 38 / 58; but prompts of 333 tokens 19 / 17, of 1,000 49 / 33, and four of 64 tokens at
+// 8,000 keys 113 / 112.  float32, whose products are as dense in both (4 kv heads of 64):
+// one prompt of 500 25 / 47, four of 500 (1,016 tiles of 32 for 256 places) 66 / 50.
+//
+// Keys are cut into as many slices as all run at once.  One more round of workgroups undoes
+// the gain (five of 320 tokens at 8,000 keys, 400 tiles: uncut 277, halves 308).  In
+// place: 256 tokens at 32,000 keys, 64 tiles, 8 slices 216 against 841; four of 256 at
+// 20,000, 256 tiles in halves 423 against 634; eight single tokens at 8,000 keys 55 against
+// 153.
 void prompt_grid(const ia_prompt_shape* s, int kv_dtype, int64_t most_keys, PromptParams* p) {
   const int group = s->n_q_heads / s->n_kv_heads;
   const int64_t resident = resident_wgs(kv_dtype);
-  const int64_t most_slices = (most_keys + kPromptSliceTiles * kArTile - 1) / (kPromptSliceTiles * kArTile);
-  // about how many tiles of `rows` rows: half a tile lost per sequence
-  auto about = [&](int rows) {
-    return ((int64_t)s->n_tokens / (rows / group) + (s->n_seq + 1) / 2) * s->n_kv_heads;
+  const int64_t key_tiles = (most_keys + kArTile - 1) / kArTile;
+  auto slices = [&](int rows) {
+    const int least = least_key_tiles(kv_dtype, rows);
+    return (key_tiles + least - 1) / least;
   };
-  const bool small = group <= kArNarrow &&
-                     (kv_dtype == IA_F32 ||
-                      (about(kArNarrow) <= resident && about(kArRows) * std::min(most_slices, resident) <= resident));
+  // tiles of `rows` rows, at least: one for each sequence, as many as whole ones hold
+  auto tiles_of = [&](int rows) {
+    return std::max<int64_t>(s->n_tokens / (rows / group), std::min(s->n_seq, s->n_tokens)) * s->n_kv_heads;
+  };
+  const bool small =
+      group <= kArNarrow && tiles_of(kArNarrow) <= resident &&
+      (kv_dtype == IA_F32 || (key_tiles > least_key_tiles(kv_dtype, kArNarrow) &&
+                              4 * tiles_of(kArRows) * std::min(slices(kArRows), resident) <= 3 * resident));
   p->tile_rows = small ? kArNarrow : kArRows;
   p->tile_tokens = p->tile_rows / group;
   p->n_tiles = (int)std::min<int64_t>((int64_t)s->n_tokens / p->tile_tokens + s->n_seq, INT32_MAX);
-  const int64_t tiles = std::max<int64_t>(1, about(p->tile_rows));
+  p->slice_tiles = least_key_tiles(kv_dtype, p->tile_rows);
   const int64_t bound = std::max<int64_t>(1, (int64_t)p->n_tiles * s->n_kv_heads);
-  int64_t n = 5 * resident >= 6 * tiles ? (resident + tiles - 1) / tiles : 1;  // (a cut for less than a fifth costs more)
+  int64_t n = resident / std::max<int64_t>(1, tiles_of(p->tile_rows));
   n = std::min<int64_t>(n, kPromptMaxSlices);
   n = std::min<int64_t>(n, 2 * resident / bound);
-  n = std::min(n, most_slices);
+  n = std::min(n, slices(p->tile_rows));
   p->slices = (int)std::max<int64_t>(1, n);
 }
 
@@ -225,8 +246,10 @@ int ia_prompt_attention(const ia_prompt_shape* shape, const void* q, const ia_pa
   s.v_page = 16 * s.v_tok;
   s.n_pages = INT64_MAX;
   s.page_rows = 16;
-  return run_prompt(shape, q, kv->dtype, p, cu_seqlens, scale, out, out_dtype, workspace, workspace_bytes,
-                    shape->n_tokens, static_cast<hipStream_t>(stream));
+  // (what is cut for: a sequence of the mean length)
+  const int64_t keys = shape->n_seq ? ((int64_t)shape->n_tokens + shape->n_seq - 1) / shape->n_seq : 0;
+  return run_prompt(shape, q, kv->dtype, p, cu_seqlens, scale, out, out_dtype, workspace, workspace_bytes, keys,
+                    static_cast<hipStream_t>(stream));
 }
 
 int ia_paged_prompt_attention(const ia_prompt_shape* shape, const void* q, const ia_paged_kv* kv,

@@ -22,16 +22,15 @@ struct PromptParams {
   int32_t tile_tokens;      // its tokens, tile_rows / group
   int32_t n_tiles;          // bound over all sequences
   int32_t slices;           // most key slices of a row tile
+  int32_t slice_tiles;      // fewest key tiles a slice is worth
   float* part_ml;
   float* part_acc;
 };
 
-constexpr int kPromptSliceTiles = 8;  // fewest key tiles a slice is worth (512 keys)
-
-// slices the keys of a row tile are cut into, and the key tiles of each
-__host__ __device__ inline int prompt_slices(int key_tiles, int most) {
-  int n = (key_tiles + kPromptSliceTiles - 1) / kPromptSliceTiles;
-  return n < 1 ? 1 : n > most ? most : n;
+// slices the keys of a row tile are cut into
+__host__ __device__ inline int prompt_slices(const PromptParams& p, int key_tiles) {
+  int n = (key_tiles + p.slice_tiles - 1) / p.slice_tiles;
+  return n < 1 ? 1 : n > p.slices ? p.slices : n;
 }
 
 int launch_prompt_bf16(const PromptParams& p, int d, hipStream_t st);
@@ -68,7 +67,7 @@ __global__ __launch_bounds__(kArThreads, KV == kArF32 ? 1 : 2) void ia_prompt_at
   int k_end = 0;
   prompt_keys(p, t, &it.limit0, &k_end);
   const int key_tiles = (k_end + kArTile - 1) / kArTile;
-  const int n = prompt_slices(key_tiles, p.slices);
+  const int n = prompt_slices(p, key_tiles);
   if (slice >= n) return;
   const int per = (key_tiles + n - 1) / n;
   it.k_lo = slice * per * kArTile;

@@ -24,7 +24,7 @@ def check_values(got, want, mag, kv, keys, what):
     check(torch.where(odd, torch.zeros_like(g), g), want.masked_fill(odd, 0), mag.masked_fill(odd, 0), kv, keys, what)
 
 
-# query heads, kv heads: groups of 64 and 40 run in tiles of 128 rows, of 4 in tiles of 32
+# query heads, kv heads (tiles of 128 rows, but of 32 for the float32 group of 4)
 SHAPES = [("bf16", 128, 64, 1), ("bf16", 64, 40, 1), ("f32", 64, 64, 1), ("f32", 128, 40, 1), ("bf16", 128, 4, 1),
           ("bf16", 64, 8, 2), ("f32", 128, 4, 1)]
 

@@ -1,10 +1,12 @@
 """Limits and workspace sizes of the prompt and prefix calls (CPU only: the pointers are never
 followed)."""
 
+import random
+
 import pytest
 
 from interattn_amd import _native as N
-from tests.test_prompt_refusals import BIG, DECODE, KV, P, STATE, append_call, prefix_call, refused, struct
+from tests.test_prompt_refusals import BIG, DECODE, KV, P, SHAPE, STATE, append_call, prefix_call, refused, struct
 
 
 @pytest.mark.parametrize("kw", [dict(shape=dict(batch=32769)), dict(shape=dict(batch=1 << 19)), dict(groups=32769),
@@ -42,3 +44,19 @@ def test_arrays_without_entries_may_be_null():
         assert lib.ia_free_sequences(struct(N.PageState, STATE, **kw), None, 0, None) == N.IA_OK
     for kw in (dict(block_table=None), dict(seq_lens=None), dict(refs=None)):
         refused(lib.ia_reserve_pages(struct(N.PageState, STATE, **kw), P, P, P, BIG, None), N.IA_ERR_INVALID, "null")
+
+
+def test_a_packed_call_is_never_cut_without_workspace():
+    """Callers size the workspace for n_tokens keys; the call cuts for the mean length."""
+    rng = random.Random(0)
+    size = N.lib().ia_prompt_attention_workspace_size
+    cut = 0
+    for _ in range(20000):
+        hkv, g = rng.choice([1, 2, 3, 4, 8, 32]), rng.choice([1, 2, 3, 4, 6, 8, 16, 32, 40, 64])
+        n_seq, tokens = int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 17))
+        shape = struct(N.PromptShape, SHAPE, n_seq=n_seq, n_tokens=tokens, n_q_heads=hkv * g, n_kv_heads=hkv)
+        kv = rng.choice([N.IA_BF16, N.IA_F32])
+        mean = size(shape, kv, -(-tokens // n_seq))
+        cut += mean > 0
+        assert mean == 0 or size(shape, kv, tokens) == mean, (hkv, g, n_seq, tokens, kv)
+    assert cut > 100
