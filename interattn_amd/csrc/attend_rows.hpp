@@ -3,10 +3,10 @@
 //
 // A workgroup takes up to 128 rows of one kv head (tokens x the group's query heads, so a
 // K/V tile is read once for the whole group) and streams the range in tiles of 64 keys
-// through LDS, the next one on its way while one is used.  Row r's softmax runs online in base 2 with its scale
-// folded in: s' = q.k * scale * log2(e); (m, l, acc) are float32, the products bf16 in,
-// float32 out (float32 caches: float32 products).  P is rounded to bf16 for the second
-// product, as the cache's values are; l sums the unrounded P.
+// through LDS, the next one on its way while one is used.  Row r's softmax runs online in
+// base 2 with its scale folded in: s' = q.k * scale * log2(e); (m, l, acc) are float32, the
+// products bf16 in, float32 out (float32 caches: float32 products).  P is rounded to bf16
+// for the second product, as the cache's values are; l sums the unrounded P.
 //
 // Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds
 // scores of ONE row: the row's maximum and sum cost one exchange between half-waves, and

@@ -7,12 +7,12 @@
 // captured serving step can replay every call.
 //
 // A call is one launch that decides (one workgroup: a few thousand entries and one pass
-// over refs, 4 bytes a page; bound by its round trips: 10.7 us for 16 forks among 1,100
-// pages, 6.8 us for a reservation, 12.9 us for the plan of 16,384 pages' compaction) and,
+// over refs, 4 bytes a page; bound by its round trips: 10.4 us for 16 forks among 1,100
+// pages, 6.7 us for a reservation, 12.9 us for the plan of 16,384 pages' compaction) and,
 // where pages move, one that copies.  Copying is bound by HBM: a workgroup per (page,
 // tensor), 16 bytes a lane and eight of them in flight: 700 pages of 8 fp8 pools and their
-// scales, 184 MB read and written, in 34.8 us (5.3 TB/s); 4,096 pages of 4 bf16 pools moved
-// by a compaction, 1.07 GB, in 253 us (4.2 TB/s).
+// scales, 184 MB read and written, in 35.0 us (5.3 TB/s); 4,096 pages of 4 bf16 pools moved
+// by a compaction, 1.07 GB, in 255 us (4.2 TB/s).
 #include <algorithm>
 
 #include "ia_common.hpp"

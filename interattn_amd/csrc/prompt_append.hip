@@ -4,8 +4,8 @@
 //   cover the 16-byte chunks of a head's row for 8, 16 or 32 tokens), looping over its
 //   heads with every K and V load of a pass in flight.  A thread's token and page are
 //   fixed, so the block table is read once per thread.  Bound by HBM: each row is read and
-//   written once (16 prompts of 500-4,000 tokens, 8 heads of 128 bf16: 322 MB in 54.7 us,
-//   5.9 TB/s); 37 tokens take 3.0 us, a workgroup per head and 16 of them.
+//   written once (16 prompts of 500-4,000 tokens, 8 heads of 128 bf16: 322 MB in 53.0 us,
+//   6.1 TB/s); 37 tokens take 3.3 us, a workgroup per head and 16 of them.
 #include <algorithm>
 
 #include "packed_rows.hpp"

@@ -1,10 +1,11 @@
 // Causal attention of packed prompts: parameters shared by the host side and the per-type
 // kernel instances.
 //
-// 4 D flops per visible (row, key) pair, on the matrix cores; at D = 64 the softmax's vector
-// work (an exponential costs four issue slots) outweighs the products.  Two prompts of 8,192
-// tokens (8 kv heads of 128, groups of 4, bf16) took 1,249 us, 880 TFLOP/s, with the products
-// waiting on every operand's LDS read; they are read ahead since, which is not timed yet.
+// 4 D flops per visible (row, key) pair, on the matrix cores.  Two prompts of 8,192 tokens (8
+// kv heads of 128, groups of 4, bf16) take 1,192 us, 920 TFLOP/s: of the cycles that a SIMD
+// has work, the matrix unit is busy 44% and a vector instruction issues in 54%, so the
+// products and the softmax take turns.  At D = 64 (24 prompts of 1-2,000 tokens, groups of 8:
+// 218 us, 570 TFLOP/s) the vector side is 72% and the matrix side 29%.
 #pragma once
 
 #include "attend_rows.hpp"

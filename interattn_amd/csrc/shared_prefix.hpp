@@ -7,11 +7,12 @@
 // of at most a cut of key tiles, one workgroup each, and a row's partials (its
 // prefix's items, then its own) are merged in that order: sums do not depend on timing.
 //
-// Bound by HBM where prefixes are long: 32 sequences behind 32,768 shared tokens (8 kv heads
-// of 128, groups of 4, bf16; 212 MB of K/V) took 54.5 us, 4.5 TB/s with the 34 MB of
-// partials that items of 128 rows leave, and 7.7 us to merge them.  Items on two workgroups
-// per CU: with one of eight waves and a deeper ring the same took 87-91 us, since its waves
-// load, multiply and exponentiate in step.
+// Bound by the K/V stream where prefixes are long: 32 sequences behind 32,768 shared tokens (8
+// kv heads of 128, groups of 4, bf16; 212 MB of K/V) take 50.4 us, 4.2 TB/s, while 17 MB of
+// partials are written, and 8.2 us to merge them; 70 us with inputs that no cache holds.  Items
+// on two workgroups per CU: with one of eight waves and a deeper ring the same took 87-91 us,
+// since its waves load, multiply and exponentiate in step.  fp8 (5, 1, 9 and 4 members on
+// 1,000-8,200 tokens): 34.9 us and 6.5 us of merge, a tile's latency with half the bytes in flight.
 #pragma once
 
 #include "attend_rows.hpp"
@@ -29,7 +30,7 @@ struct PrefixParams {
   const int32_t* group_starts;  // [n_groups + 1]
   const int32_t* shared_lens;   // [n_groups]
   int32_t batch, n_groups;
-  int32_t tile_seqs;            // sequences of a row tile (128 / group)
+  int32_t tile_seqs;            // sequences of a row tile (128 / group; float32 32 / group)
   int32_t n_tiles;              // bound of the prefixes' row tiles
   int32_t max_items;            // per kv head: workgroups launched
   int32_t target;               // items per kv head the device runs at once
