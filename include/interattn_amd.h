@@ -600,6 +600,91 @@ IA_API int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* rows, 
                                int32_t n_kv_heads, int32_t head_dim, void* stream);
 
 /*
+ * Rotary positions: the pair p of a head at position t is turned by t * turns[p], turns a
+ * device array [dim / 2] of unsigned 64-bit fixed point, 2^-64 of a full turn per position
+ * (so t * turns[p] modulo 2^64 is the angle, exact for every position), and multiplied by
+ * factor.  Pairs are (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved; channels from dim
+ * on are left as they are.
+ */
+typedef struct ia_rotary {
+  const uint64_t* turns;
+  int32_t dim; /* even, at most head_dim */
+  int32_t interleaved;
+  float factor;
+} ia_rotary;
+
+/* Rows to rotate: in[t, h, :] and out[t, h, :] (strides in elements, 16-byte multiples; out
+ * may be in). */
+typedef struct ia_rotary_rows {
+  const void* in;
+  void* out;
+  int64_t in_token_stride, in_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int32_t n_heads;
+} ia_rotary_rows;
+
+/*
+ * Rows of one or two tensors (queries and keys) of n_tokens packed tokens turned to
+ * positions[t] (a device array [n_tokens], any sign).  inverse: the transposed rotation
+ * (angles negated, the same factor), which is the gradient.  dtype IA_F32 or IA_BF16,
+ * head_dim a multiple of 16 up to 256; sums in float32, rounded once.
+ */
+IA_API int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* rows, int32_t n_tensors, int32_t dtype,
+                           int32_t head_dim, const int32_t* positions, int32_t n_tokens, int32_t inverse,
+                           void* stream);
+
+/*
+ * Packed tokens into the paged pool, as ia_append_prompt_kv, with keys (and the queries q,
+ * where given) rotated to their positions in the sequence, or to positions[t] (device array
+ * [n_tokens]) where that is given.  rotary null: nothing is turned.  q's dtype is rows->dtype;
+ * its rows are written where the pool has no page too.  cu_seqlens null: one token per
+ * sequence (n_tokens = n_seq); then, and only then, new_seq_lens may be seq_lens.
+ *
+ * IA_FP8_E4M3 pools take f32 or bf16 rows and set k_scale / v_scale of the pages they write.
+ * With a the largest finite magnitude of the call's rows in a (page, kv head), the scale is
+ * the least power of two s >= 2^-126 with a <= 448 s; a page that holds earlier tokens of the
+ * sequence (its first one) keeps its scale s0 (finite, at least 2^-126) where a <= 448 s0, else
+ * the earlier rows' codes c become e4m3(c * s0 / s).  Codes are x / s rounded to nearest even;
+ * values that are not finite become NaN codes.  Rows of a page past the sequence's tokens keep
+ * their codes.  A page must not be written by two sequences of a call.  kv->seq_scale must be
+ * null: such copies of the scales have to be gathered again.
+ */
+IA_API int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows* q, const ia_packed_kv* rows,
+                               const ia_paged_kv* kv, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                               int32_t* new_seq_lens, const int32_t* positions, int32_t n_seq, int32_t n_tokens,
+                               int32_t n_kv_heads, int32_t head_dim, void* stream);
+
+/*
+ * Cached rows as packed tensors: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of k_out and
+ * v_out ([n_tokens, n_kv_heads, head_dim], contiguous, out_dtype IA_F32 or IA_BF16) are the
+ * positions starts[b], starts[b] + 1, ... (device array [n_seq]) of sequence b in the pool,
+ * fp8 codes times their page's scale.  Positions without a page give zeros; rows of no
+ * sequence are left as they were.
+ */
+IA_API int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32_t out_dtype, const int32_t* starts,
+                      const int32_t* cu_seqlens, int32_t n_seq, int32_t n_tokens, int32_t n_kv_heads,
+                      int32_t head_dim, void* stream);
+
+/*
+ * Beam search's selection: of every batch entry's beams x vocab continuations the n with the
+ * largest scores[b, j] + logits[b * beams + j, v] - logsumexp(logits[b * beams + j]), best
+ * first, equal ones by j * vocab + v.  logits [batch * beams, vocab] with row_stride
+ * elements between rows (bf16 or f32, any alignment of whole elements), scores [batch, beams]
+ * float32.  done [batch, beams] (may be null): a beam that has ended offers pad_token with its
+ * score as it is, and nothing else; its logits are not read.  NaN logits, and beams whose
+ * score or logsumexp is no number or whose logits reach +infinity, offer nothing.  out_scores,
+ * out_tokens and out_rows [batch, n]: score, token and row b * beams + j; where fewer than n
+ * are offered, -infinity and the lowest continuations that were not.  beams and n at most 64.
+ * The workspace needs no initialisation.
+ */
+IA_API size_t ia_beam_select_workspace_size(int32_t batch, int32_t beams, int32_t vocab, int32_t n,
+                                            int32_t logits_dtype);
+IA_API int ia_beam_select(const void* logits, int32_t logits_dtype, int64_t row_stride, const float* scores,
+                          const uint8_t* done, int32_t pad_token, int32_t batch, int32_t beams, int32_t vocab,
+                          int32_t n, float* out_scores, int32_t* out_tokens, int32_t* out_rows, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
  * Pages of one tensor: page p starts at data + p * page_stride and holds n_outer x n_inner
  * runs of run_bytes at the given strides (all in bytes, multiples of word_bytes: 16, or 4
  * for small rows such as fp8 scales).  A K or V pool, or a scale array, of one layer.
@@ -666,6 +751,21 @@ IA_API int ia_free_sequences(const ia_page_state* state, const int32_t* rows, in
 IA_API size_t ia_reserve_workspace_size(int32_t rows, int64_t n_pages);
 IA_API int ia_reserve_pages(const ia_page_state* state, const int32_t* new_tokens, int32_t* ok, void* workspace,
                             size_t workspace_bytes, void* stream);
+
+/*
+ * Every row becomes what row parents[row] (device array [rows], rows <= 8192) was, all at
+ * once.  Of the rows with one parent, the parent itself, else the lowest, takes its pages over
+ * as they are; the others share its whole pages (refs rise), get a copy of the page its last
+ * tokens partly fill in the lowest free page, rows in order, and no page past its length.
+ * Pages that no row holds afterwards are free (before the copies take theirs).  A parent
+ * outside [0, rows) leaves the row empty.  ok[row] is 1, or 0 and the row empty: where the
+ * partly filled page is not mapped, the length does not fit the table, or no page is free.
+ * workspace: ia_reorder_workspace_size bytes.
+ */
+IA_API size_t ia_reorder_workspace_size(int32_t rows, int32_t cols);
+IA_API int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,
+                                const int32_t* parents, int32_t* ok, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /*
  * Live pages moved to the front of the pools: with n_live pages held, those at or past

@@ -5,6 +5,7 @@ The compute path is the HIP library ``libinterattn_amd.so`` (C ABI in
 """
 
 from ._native import NativeLibraryMissing, NativeError  # noqa: F401
+from .beam import beam_select  # noqa: F401
 from .ops import (  # noqa: F401
     append_kv,
     build_block_summaries,
@@ -19,12 +20,21 @@ from .ops import (  # noqa: F401
     wait_fallbacks,
     workspace_tensor,
 )
-from .pages import copy_pages, compact_pages, fork_sequences, free_sequences, reserve_pages  # noqa: F401
+from .pages import (  # noqa: F401
+    compact_pages,
+    copy_pages,
+    fork_sequences,
+    free_sequences,
+    reorder_sequences,
+    reserve_pages,
+)
 from .prompt import (  # noqa: F401
     append_prompt_kv,
     paged_prompt_attention,
     prompt_attention,
+    read_kv,
     shared_prefix_decode,
 )
+from .rotary import RotaryPlan, apply_rotary, rotary_append_kv, rotary_frequencies, rotary_plan  # noqa: F401
 
 __version__ = "0.1.0"

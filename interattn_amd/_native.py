@@ -144,6 +144,27 @@ class PackedKV(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("factor", ctypes.c_float),
+    ]
+
+
+class RotaryRows(ctypes.Structure):
+    _fields_ = [
+        ("in_", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("in_token_stride", ctypes.c_int64),
+        ("in_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("n_heads", ctypes.c_int32),
+    ]
+
+
 class PageTensor(ctypes.Structure):
     _fields_ = [
         ("data", ctypes.c_void_p),
@@ -266,6 +287,18 @@ SIGNATURES = {
     "ia_append_prompt_kv": (
         ctypes.c_int,
         [ctypes.POINTER(PagedKV), ctypes.POINTER(PackedKV), _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "ia_apply_rotary": (
+        ctypes.c_int,
+        [ctypes.POINTER(Rotary), ctypes.POINTER(RotaryRows), _I32, _I32, _I32, _P, _I32, _I32, _P]),
+    "ia_rotary_append_kv": (
+        ctypes.c_int,
+        [ctypes.POINTER(Rotary), ctypes.POINTER(RotaryRows), ctypes.POINTER(PackedKV), ctypes.POINTER(PagedKV), _P, _P,
+         _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "ia_read_kv": (ctypes.c_int, [ctypes.POINTER(PagedKV), _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "ia_beam_select_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "ia_beam_select": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _SZ, _P]),
     "ia_copy_pages": (ctypes.c_int, [ctypes.POINTER(PageTensor), _I32, _P, _P, _I32, _I64, _P]),
     "ia_fork_workspace_size": (_SZ, [_I32]),
     "ia_fork_sequences": (
@@ -274,6 +307,10 @@ SIGNATURES = {
     "ia_free_sequences": (ctypes.c_int, [ctypes.POINTER(PageState), _P, _I32, _P]),
     "ia_reserve_workspace_size": (_SZ, [_I32, _I64]),
     "ia_reserve_pages": (ctypes.c_int, [ctypes.POINTER(PageState), _P, _P, _P, _SZ, _P]),
+    "ia_reorder_workspace_size": (_SZ, [_I32, _I32]),
+    "ia_reorder_sequences": (
+        ctypes.c_int,
+        [ctypes.POINTER(PageState), ctypes.POINTER(PageTensor), _I32, _P, _P, _P, _SZ, _P]),
     "ia_compact_workspace_size": (_SZ, [_I64]),
     "ia_compact_pages": (
         ctypes.c_int, [ctypes.POINTER(PageState), ctypes.POINTER(PageTensor), _I32, _P, _P, _SZ, _P]),

@@ -329,6 +329,120 @@ __global__ __launch_bounds__(kPlanThreads) void ia_reserve_rows(Table t, const i
   }
 }
 
+// ------------------------------------------------------------------ reorder
+
+// Row i becomes what row parents[i] was.  One row takes over what its parent held (the
+// parent itself, else the lowest of them); the others share the whole pages and get a copy
+// of the partly filled one.
+struct ReorderPlan {
+  const int32_t* parents;
+  int32_t* ok;     // caller's
+  int32_t* kind;   // workspace [rows]: what becomes of the row
+  int32_t* len;    // [rows] its length
+  int32_t* from;   // [rows] the page it needs a copy of, -1: none
+  int32_t* to;     // [rows]
+  int32_t* list;   // [rows]
+  int32_t* table;  // [rows, cols] its pages
+};
+enum { kRowStays = 0, kRowChanges = 1, kRowEmpty = 2 };
+
+// A workgroup per row and stretch of columns: the row's new pages and their counts.  The table
+// itself is read only; the counts change by sums, whose order does not matter.
+__global__ __launch_bounds__(kCopyThreads) void ia_reorder_take(Table t, ReorderPlan r, int span) {
+  const int i = blockIdx.x, tid = threadIdx.x, src = r.parents[i];
+  const bool exists = src >= 0 && src < t.rows;
+  bool heir = src == i;
+  if (exists && !heir) {
+    int before = r.parents[src] == src;
+    for (int j = tid; j < i && !before; j += kCopyThreads) before = r.parents[j] == src;
+    heir = !__syncthreads_or(before);
+  }
+  int kind = src == i ? kRowStays : exists ? kRowChanges : kRowEmpty, ok = 1, len = 0, whole = 0, from = -1;
+  if (exists) {
+    len = t.seq_lens[src];
+    if (!heir) {
+      ok = len >= 0 && len <= (int64_t)t.cols * t.page_rows;
+      if (ok) whole = len / t.page_rows;
+      if (ok && len % t.page_rows) {
+        from = t.table[src * t.stride + whole];
+        ok = from >= 0 && from < t.n_pages;
+      }
+      if (!ok) {
+        kind = kRowEmpty;
+        len = 0;
+        from = -1;
+      }
+    }
+  }
+  if (blockIdx.y == 0 && tid == 0) {
+    r.ok[i] = ok;
+    r.kind[i] = kind;
+    r.len[i] = len;
+    r.from[i] = from;
+  }
+  if (kind == kRowStays) return;
+  const int c0 = blockIdx.y * span, c1 = min(c0 + span, t.cols);
+  for (int c = c0 + tid; c < c1; c += kCopyThreads) {
+    const int old = t.table[i * t.stride + c];
+    int pg = -1;
+    if (kind == kRowChanges && (heir || c < whole)) pg = t.table[src * t.stride + c];
+    r.table[(int64_t)i * t.cols + c] = pg;
+    if (pg == old) continue;
+    if (old >= 0 && old < t.n_pages) atomicSub(&t.refs[old], 1);
+    if (pg >= 0 && pg < t.n_pages) atomicAdd(&t.refs[pg], 1);
+  }
+}
+
+// Pages for the copies, in the rows' order.
+__global__ __launch_bounds__(kPlanThreads) void ia_reorder_plan(Table t, ReorderPlan r) {
+  __shared__ int scratch[kPlanWaves];
+  const int tid = threadIdx.x;
+  int base = 0;
+  for (int i0 = 0; i0 < t.rows; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const int need = i < t.rows && r.from[i] >= 0;
+    const int upto = wave_inclusive_scan(need);
+    int before, total;
+    wave_prefix(__builtin_amdgcn_readlane(upto, 63), scratch, &before, &total);
+    if (i < t.rows) r.to[i] = need ? base + before + upto - 1 : -1;  // (its rank, for now)
+    base += total;
+  }
+  const int have = lowest_free(t.refs, t.n_pages, base, r.list, scratch);
+  for (int i = tid; i < t.rows; i += kPlanThreads) {
+    const int rank = r.to[i];
+    if (rank < 0) continue;
+    if (rank >= have) {
+      r.ok[i] = 0;
+      r.to[i] = -1;
+      continue;
+    }
+    r.to[i] = r.list[rank];
+    t.refs[r.list[rank]] = 1;
+  }
+}
+
+// y = 0: the table rows and lengths; y > 0: tensor y - 1's partly filled page
+__global__ __launch_bounds__(kCopyThreads) void ia_reorder_apply(Table t, Tensors ts, ReorderPlan r, int with_table) {
+  const int i = blockIdx.x, tid = threadIdx.x, kind = r.kind[i];
+  if (kind == kRowStays) return;
+  const int y = (int)blockIdx.y - with_table;
+  if (y >= 0) {
+    if (r.to[i] >= 0) copy_page(ts.t[y], r.from[i], r.to[i], tid);
+    return;
+  }
+  const int len = r.len[i], whole = r.to[i] >= 0 ? len / t.page_rows : -1;
+  const bool given_up = kind == kRowChanges && !r.ok[i];  // no page was left: what it shares goes back
+  for (int c = tid; c < t.cols; c += kCopyThreads) {
+    int pg = r.table[(int64_t)i * t.cols + c];
+    if (given_up) {
+      if (pg >= 0 && pg < t.n_pages) atomicSub(&t.refs[pg], 1);
+      pg = -1;
+    }
+    t.table[i * t.stride + c] = c == whole ? r.to[i] : pg;
+  }
+  if (tid == 0) t.seq_lens[i] = given_up ? 0 : len;
+}
+
 // ------------------------------------------------------------------ compact
 
 // Live pages at or past the number of live pages move, in ascending order, into the free
@@ -542,6 +656,45 @@ int ia_reserve_pages(const ia_page_state* state, const int32_t* new_tokens, int3
   hipLaunchKernelGGL(ia_reserve_rows, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), t, new_tokens,
                      ok, w, w + t.rows);
   return check_launch("reserve pages");
+}
+
+size_t ia_reorder_workspace_size(int32_t rows, int32_t cols) {
+  return rows > 0 && cols >= 0 ? 4 * (size_t)rows * (5 + (size_t)cols) : 0;
+}
+
+int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,
+                         const int32_t* parents, int32_t* ok, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace ia;
+  Table t;
+  int rc = check_state(state, &t);
+  if (rc) return rc;
+  rc = check_tensors(tensors, n_tensors);
+  if (rc) return rc;
+  if (t.rows == 0) return IA_OK;
+  if (t.rows > kForkMax) return fail(IA_ERR_UNSUPPORTED, "at most " + std::to_string(kForkMax) + " rows are reordered");
+  if (!parents || !ok) return fail(IA_ERR_INVALID, "null pointer argument");
+  if (!workspace || workspace_bytes < ia_reorder_workspace_size(t.rows, t.cols) ||
+      reinterpret_cast<uintptr_t>(workspace) % 4)
+    return fail(IA_ERR_WORKSPACE, "workspace missing or too small");
+  int32_t* w = static_cast<int32_t*>(workspace);
+  const size_t n = t.rows;
+  const ReorderPlan r{parents, ok, w, w + n, w + 2 * n, w + 3 * n, w + 4 * n, w + 5 * n};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // (a row's length and counts are written even where the table has no column)
+  const int span = 4 * kCopyThreads, spans = std::max(1, (t.cols + span - 1) / span);
+  hipLaunchKernelGGL(ia_reorder_take, dim3(t.rows, spans), dim3(kCopyThreads), 0, st, t, r, span);
+  rc = check_launch("reorder");
+  if (rc) return rc;
+  hipLaunchKernelGGL(ia_reorder_plan, dim3(1), dim3(kPlanThreads), 0, st, t, r);
+  rc = check_launch("reorder plan");
+  for (int at = 0; !rc && (at == 0 || at < n_tensors); at += kMaxTensors) {
+    const Tensors ts = some_tensors(tensors, n_tensors, at);
+    const int with_table = at == 0;
+    hipLaunchKernelGGL(ia_reorder_apply, dim3(t.rows, ts.n + with_table), dim3(kCopyThreads), 0, st, t, ts, r,
+                       with_table);
+    rc = check_launch("reorder apply");
+  }
+  return rc;
 }
 
 size_t ia_compact_workspace_size(int64_t n_pages) { return n_pages >= 0 ? 4 * (2 * (size_t)n_pages + 16) : 0; }

@@ -1,0 +1,206 @@
+// Rotary positions: angles from whole positions, and rows of a head as pairs.
+//
+// Pair p of a head at position t turns by t * w[p].  w is held as turns of a circle in 64-bit
+// fixed point, so that t * w modulo one turn is an integer product that drops what overflows:
+// every position of 31 bits and sign has its angle to 2^-32 turns (1.5e-9), with no table and
+// no range reduction in floating point (in float32, t * w at t = 10^6 is off by 0.03).
+#pragma once
+
+#include "ia_common.hpp"
+
+namespace ia {
+
+// The angle's turn in 2^-32, of position t and frequency w (2^-64 turns a position): the
+// upper half of the low 64 bits of t * w.
+__device__ __forceinline__ u32 rotary_turn(int t, unsigned long long w) {
+  const u32 lo = (u32)w, hi = (u32)(w >> 32);
+  return __umulhi((u32)t, lo) + (u32)t * hi - (t < 0 ? lo : 0u);
+}
+
+// Sine and cosine of a turn: the nearest quarter is taken off, and what is left, x in
+// [-pi/4, pi/4], goes through the Taylor sums to x^9 and x^8 (remainders 2e-9 and 2.5e-8).
+__device__ __forceinline__ void rotary_sincos(u32 turn, float* sn, float* cs) {
+  const u32 near = turn + 0x20000000u, quarter = near >> 30;
+  const float x = (float)(int)(turn - (near & 0xc0000000u)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+  const float z = x * x;
+  float s = fmaf(z, 2.7557319223985891e-6f, -1.9841269841269841e-4f);
+  s = fmaf(z, s, 8.3333333333333333e-3f);
+  s = fmaf(z, s, -1.6666666666666667e-1f);
+  s = fmaf(x * z, s, x);
+  float c = fmaf(z, 2.4801587301587302e-5f, -1.3888888888888889e-3f);
+  c = fmaf(z, c, 4.1666666666666667e-2f);
+  c = fmaf(z, c, -0.5f);
+  c = fmaf(z, c, 1.f);
+  const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+  *sn = quarter & 2 ? -a : a;
+  *cs = (quarter + 1) & 2 ? -b : b;
+}
+
+// How a head's D elements are taken as D / 2 pairs.  A lane holds VEC neighbouring pairs, unit
+// u the pairs u * VEC ...; pairs past rot / 2 are not turned.  VEC fills 16 bytes but in the
+// last layout.
+//   kRowsPlain        no pairs: 2 * VEC elements in a row, never turned
+//   kRowsHalf         (i, i + rot / 2): two 16-byte chunks; rot a multiple of 2 * VEC
+//   kRowsInterleaved  (2 i, 2 i + 1): 2 * VEC elements in a row
+//   kRowsHalfOdd      as kRowsHalf for any even rot: one pair a lane, so that a wave's accesses
+//                     are neighbours though the halves begin anywhere
+enum RowLayout { kRowsPlain = 0, kRowsHalf = 1, kRowsInterleaved = 2, kRowsHalfOdd = 3 };
+
+template <typename T, int LAYOUT>
+struct RowVec {
+  static constexpr int kVec = LAYOUT == kRowsHalfOdd ? 1 : 16 / (int)sizeof(T);
+};
+
+struct bf16_t {
+  unsigned short bits;
+};
+
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((u32)v.bits << 16); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+
+// 16 bytes of T as floats and back
+__device__ __forceinline__ void widen(const u32x4_t& w, float* x, bf16_t) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = bf16_lo(w[j]);
+    x[2 * j + 1] = bf16_hi(w[j]);
+  }
+}
+__device__ __forceinline__ void widen(const u32x4_t& w, float* x, float) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]);
+}
+__device__ __forceinline__ u32x4_t narrow(const float* x, bf16_t) {
+  return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+__device__ __forceinline__ u32x4_t narrow(const float* x, float) {
+  return u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+}
+
+// Elements at which a unit's two chunks begin.
+template <int LAYOUT, int VEC>
+__device__ __forceinline__ void unit_chunks(int u, int rot, int* a, int* b) {
+  if constexpr (LAYOUT == kRowsHalf || LAYOUT == kRowsHalfOdd) {
+    const int turned = rot / (2 * VEC);  // units that turn; the rest are pairs of neighbours
+    *a = u < turned ? u * VEC : u * 2 * VEC;
+    *b = u < turned ? rot / 2 + u * VEC : *a + VEC;
+  } else {
+    *a = u * 2 * VEC;
+    *b = *a + VEC;
+  }
+}
+
+// One unit of a row as it lies in memory.
+template <typename T, int LAYOUT>
+struct RowUnit {
+  static constexpr int kVec = RowVec<T, LAYOUT>::kVec;
+  static constexpr int kA = LAYOUT == kRowsInterleaved ? 2 : 1;      // pair j is x[kA j]
+  static constexpr int kB = LAYOUT == kRowsInterleaved ? 1 : kVec;  // and x[kA j + kB]
+  u32x4_t w0, w1;
+
+  __device__ __forceinline__ void load(const T* row, int u, int rot) {
+    int a, b;
+    unit_chunks<LAYOUT, kVec>(u, rot, &a, &b);
+    w0 = ld_stream16(row + a);
+    w1 = ld_stream16(row + b);
+  }
+
+  __device__ __forceinline__ void zero() { w0 = w1 = u32x4_t{0u, 0u, 0u, 0u}; }
+
+  // x[0 .. VEC) and x[VEC .. 2 VEC): the elements of the two chunks, the unit's first n pairs
+  // turned (the others as they are, whatever their neighbour holds)
+  __device__ __forceinline__ void turned(const float* cs, const float* sn, int n, float* x) const {
+    widen(w0, x, T{});
+    widen(w1, x + kVec, T{});
+    if constexpr (LAYOUT != kRowsPlain) {
+      if (n == kVec) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
+      } else if constexpr (LAYOUT == kRowsInterleaved) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (j < n) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+    const float x = a;
+    a = fmaf(x, c, -b * s);
+    b = fmaf(b, c, x * s);
+  }
+};
+
+template <typename T>
+struct RowUnit<T, kRowsHalfOdd> {
+  static constexpr int kVec = 1;
+  T e0, e1;
+
+  __device__ __forceinline__ void load(const T* row, int u, int rot) {
+    int a, b;
+    unit_chunks<kRowsHalfOdd, 1>(u, rot, &a, &b);
+    e0 = row[a];
+    e1 = row[b];
+  }
+  __device__ __forceinline__ void zero() { e0 = e1 = T{}; }
+  __device__ __forceinline__ void turned(const float* cs, const float* sn, int n, float* x) const {
+    x[0] = to_f32(e0);
+    x[1] = to_f32(e1);
+    if (n) RowUnit<T, kRowsHalf>::turn(x[0], x[1], cs[0], sn[0]);
+  }
+};
+
+__device__ __forceinline__ void put_one(bf16_t* to, float x) { to->bits = f32_to_bf16_bits(x); }
+__device__ __forceinline__ void put_one(float* to, float x) { *to = x; }
+
+// The unit's elements to a row of T.
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void store_unit(T* row, int u, int rot, const float* x) {
+  constexpr int kVec = RowVec<T, LAYOUT>::kVec;
+  int a, b;
+  unit_chunks<LAYOUT, kVec>(u, rot, &a, &b);
+  if constexpr (LAYOUT == kRowsHalfOdd) {
+    put_one(row + a, x[0]);
+    put_one(row + b, x[1]);
+  } else {
+    *reinterpret_cast<u32x4_t*>(row + a) = narrow(x, T{});
+    *reinterpret_cast<u32x4_t*>(row + b) = narrow(x + kVec, T{});
+  }
+}
+
+// The rotation as the kernels take it.
+struct RotaryArgs {
+  const unsigned long long* w;  // [rot / 2]
+  int rot;
+  float factor;
+  float sign;  // -1: the transposed rotation
+};
+
+// How many of unit u's VEC pairs turn.
+template <int VEC>
+__device__ __forceinline__ int unit_turns(int rot, int u) {
+  return min(max(rot / 2 - u * VEC, 0), VEC);
+}
+
+// Cosines and sines, times the factor, of a unit's first n pairs at position t.
+template <int VEC>
+__device__ __forceinline__ void unit_angles(const RotaryArgs& r, int t, int u, int n, float* cs, float* sn) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    float s = 0.f, c = 1.f;
+    if (j < n) rotary_sincos(rotary_turn(t, r.w[u * VEC + j]), &s, &c);
+    cs[j] = c * r.factor;
+    sn[j] = s * (r.factor * r.sign);
+  }
+}
+
+int check_rotary(const ia_rotary* r, int head_dim);  // rotary.hip
+
+// The layout whose loads fit: kRowsHalfOdd where the halves are no whole chunks.
+inline int rotary_layout(const ia_rotary* r, int elem_bytes) {
+  if (!r || r->dim == 0) return kRowsPlain;
+  if (r->interleaved) return kRowsInterleaved;
+  return r->dim % (2 * (16 / elem_bytes)) ? kRowsHalfOdd : kRowsHalf;
+}
+
+}  // namespace ia

@@ -1,0 +1,460 @@
+// Keys rotated into the paged pool, values into the pool, queries rotated out, for gfx950:
+// the write side of a serving step, into bf16, f32 and fp8 pages.
+//
+// A workgroup per (sequence, page its new tokens touch, slice of heads).  A wave takes one
+// head's rows of the page, 16 at a time, as units of VEC pairs: lane = (row, unit), so that the
+// angles of its rows are computed once and serve every head, and a pair turns inside a lane.
+//
+// fp8 pages have one float32 scale per (page, kv head).  The wave that holds the page's new
+// rows takes the largest magnitude a of its finite values (a reduction inside the wave) and
+//   s = 2^ceil(log2(a / 448)), at least 2^-126;
+// a page that holds earlier tokens keeps its scale s0 where a <= 448 s0, else its earlier codes
+// c become e4m3(c * s0 / s).  A power of two costs e4m3 no relative precision (only up to one
+// binade of range at the small end) and makes both the division and the re-encoding exact, but
+// for values that turn subnormal: a cache written token by token holds what one written at once
+// does.  Codes are rounded from float32, without a rounding to bf16 between.
+//
+// Bound by HBM for prompts, by its round trips (length, page, rows, scale) for single tokens.
+#include <algorithm>
+
+#include "packed_rows.hpp"
+#include "rotary.hpp"
+
+namespace ia {
+
+int check_kv(const ia_paged_kv* kv, int d);
+
+namespace {
+
+constexpr int kWriteThreads = 256, kWriteMaxThreads = 512;
+constexpr int kSub = 16;  // rows of a page taken at a time
+constexpr float kLargestCode = 448.f;
+constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
+
+struct WriteParams {
+  // new rows and rotated queries (strides in bytes)
+  const char* q;
+  char* q_out;
+  const char* k_new;
+  const char* v_new;
+  int64_t q_tok, q_head, qo_tok, qo_head, kn_tok, kn_head, vn_tok, vn_head;
+  // pool (strides in bytes)
+  char* k;
+  char* v;
+  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;
+  float* k_scale;
+  float* v_scale;
+  int64_t scale_page;
+  const int32_t* table;
+  int64_t bt_stride, bt_cols, n_pages;
+  int32_t page_rows;
+  // batch
+  const int32_t* cu;  // null: one token per sequence
+  const int32_t* seq_lens;
+  int32_t* new_lens;
+  const int32_t* positions;  // null: the place in the sequence
+  int32_t n_seq, n_tokens, n_kv_heads, group, kv_heads_per_wg;
+  RotaryArgs rot;
+};
+
+__device__ __forceinline__ int64_t write_page(const WriteParams& p, int b, int64_t lp) {
+  int64_t pg = lp;
+  if (p.table) pg = lp < p.bt_cols ? p.table[(int64_t)b * p.bt_stride + lp] : -1;
+  return pg < 0 || pg >= p.n_pages ? -1 : pg;
+}
+
+// The least power of two, 2^-126 at least, that brings a down to 448 or less: with
+// a = m 2^e, m in [1, 2), 448 = 1.75 2^8 asks for 2^(e - 8), or twice that for m > 1.75.
+__device__ __forceinline__ float page_scale(float a) {
+  const u32 bits = __float_as_uint(a);
+  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return __uint_as_float((u32)(max(e, -126) + 127) << 23);
+}
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// Four floats, already divided by their scale, as e4m3 codes; not finite: NaN.
+__device__ __forceinline__ u32 fp8_codes(const float* x) {
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = finite(x[j]) ? x[j] : __uint_as_float(0x7fc00000u);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  return (u32)w;
+}
+
+// The earlier rows [0, n) of one head's page from scale s0 to s.
+template <int D>
+__device__ void recode(char* rows, int64_t tok_stride, int n, float s0, float s, int lane) {
+  const float ratio = s0 / s;
+  constexpr int kLanes = D / 16;
+  for (int r = lane / kLanes; r < n; r += 64 / kLanes) {
+    u32x4_t* at = reinterpret_cast<u32x4_t*>(rows + r * tok_stride + lane % kLanes * 16);
+    u32x4_t w = *at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
+      fp8x4_to_f32(w[i], x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= ratio;
+      w[i] = fp8_codes(x);
+    }
+    *at = w;
+  }
+}
+
+// One page of one sequence, as all of its tasks see it.
+struct WritePage {
+  int64_t page;    // -1: none
+  int64_t tok;     // packed row of page row 0 (may lie before the first row)
+  int lo, hi;      // the new rows' places in the page
+  int sub0, sub1;  // 16-row parts that hold them
+};
+
+// Rows of T, 16 of a page at a time, by one wave.
+template <typename T, int D, int LAYOUT>
+struct PageRows {
+  using Unit = RowUnit<T, LAYOUT>;
+  static constexpr int kVec = Unit::kVec;
+  static constexpr int kUnits = D / (2 * kVec);  // of a row
+  static constexpr int kRows = 64 / kUnits;      // a wave's rows at once
+  static constexpr int kGroups = kSub / kRows;   // of 16 rows
+  static_assert(kRows >= 1 && kRows <= kSub, "a wave holds 1 to 16 rows, a unit a lane");
+
+  const WriteParams& p;
+  const WritePage& w;
+  int unit, row, turns;
+  float cs[kGroups][kVec], sn[kGroups][kVec];
+
+  __device__ __forceinline__ PageRows(const WriteParams& p_, const WritePage& w_, int lane)
+      : p(p_), w(w_), unit(lane % kUnits), row(lane / kUnits), turns(unit_turns<kVec>(p_.rot.rot, lane % kUnits)) {}
+
+  __device__ __forceinline__ int place(int sub, int g) const { return sub * kSub + g * kRows + row; }
+  __device__ __forceinline__ bool mine(int at) const { return at >= w.lo && at < w.hi; }
+
+  __device__ __forceinline__ void angles(int sub, int64_t pos0) {
+    if constexpr (LAYOUT != kRowsPlain) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int at = place(sub, g);
+        const int t = !mine(at) ? 0 : p.positions ? p.positions[w.tok + at] : (int)(pos0 + at);
+        unit_angles<kVec>(p.rot, t, unit, turns, cs[g], sn[g]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load(Unit* x, const char* rows, int64_t tok_stride, int sub) const {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int at = place(sub, g);
+      if (mine(at)) x[g].load(reinterpret_cast<const T*>(rows + (w.tok + at) * tok_stride), unit, p.rot.rot);
+      else x[g].zero();
+    }
+  }
+
+  // as rows of T, row0 the row of the page's first place
+  __device__ __forceinline__ void put(const Unit* x, char* rows, int64_t tok_stride, int64_t row0, int sub) const {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int at = place(sub, g);
+      if (!mine(at)) continue;
+      float y[2 * kVec];
+      x[g].turned(cs[g], sn[g], turns, y);
+      store_unit<T, LAYOUT>(reinterpret_cast<T*>(rows + (row0 + at) * tok_stride), unit, p.rot.rot, y);
+    }
+  }
+
+  // largest finite magnitude of the 16 places' new rows, in every lane
+  __device__ __forceinline__ float largest(const Unit* x) const {
+    float a = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      float y[2 * kVec];
+      x[g].turned(cs[g], sn[g], turns, y);
+#pragma unroll
+      for (int j = 0; j < 2 * kVec; ++j) a = fmaxf(a, finite(y[j]) ? fabsf(y[j]) : 0.f);
+    }
+    return wave_max(a);
+  }
+
+  // as e4m3 codes over the scale s; inv is its reciprocal where that is exact, else 0
+  __device__ __forceinline__ void put_codes(const Unit* x, char* rows, int64_t tok_stride, int sub, float s,
+                                            float inv) const {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int at = place(sub, g);
+      if (!mine(at)) continue;
+      float y[2 * kVec];
+      x[g].turned(cs[g], sn[g], turns, y);
+#pragma unroll
+      for (int j = 0; j < 2 * kVec; ++j) y[j] = inv != 0.f ? y[j] * inv : y[j] / s;
+      char* to = rows + at * tok_stride;
+      int a, b;
+      unit_chunks<LAYOUT, kVec>(unit, p.rot.rot, &a, &b);
+      if constexpr (kVec == 8) {
+        *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(y), fp8_codes(y + 4)};
+        *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(y + 8), fp8_codes(y + 12)};
+      } else if constexpr (kVec == 4) {
+        *reinterpret_cast<u32*>(to + a) = fp8_codes(y);
+        *reinterpret_cast<u32*>(to + b) = fp8_codes(y + 4);
+      } else {
+        const float z[4] = {y[0], y[1], 0.f, 0.f};
+        const u32 c = fp8_codes(z);
+        to[a] = (char)(c & 0xff);
+        to[b] = (char)(c >> 8 & 0xff);
+      }
+    }
+  }
+
+  // One head's new rows into its fp8 page.
+  __device__ __forceinline__ void quantise(const char* from, int64_t from_tok, char* rows, int64_t tok, float* scale,
+                                           int64_t pos0, int lane) {
+    const bool one = w.sub1 - w.sub0 == 1;  // the rows stay in registers between scale and codes
+    Unit x[kGroups];
+    float a = 0.f;
+    for (int sub = w.sub0; sub < w.sub1; ++sub) {
+      load(x, from, from_tok, sub);
+      if (!one) angles(sub, pos0);
+      a = fmaxf(a, largest(x));
+    }
+    float s = page_scale(a);
+    if (w.lo > 0) {  // earlier tokens: their scale, or their codes follow
+      const float s0 = *scale;
+      if (finite(s0) && s0 >= kLeastScale && a <= kLargestCode * s0)
+        s = s0;
+      else
+        recode<D>(rows, tok, w.lo, s0, s, lane);
+    }
+    if (lane == 0) *scale = s;
+    const float inv = (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
+    for (int sub = w.sub0; sub < w.sub1; ++sub) {
+      if (!one) {
+        load(x, from, from_tok, sub);
+        angles(sub, pos0);
+      }
+      put_codes(x, rows, tok, sub, s, inv);
+    }
+  }
+};
+
+template <typename T, bool FP8, int D, int LAYOUT>
+__global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p) {
+  using Turned = PageRows<T, D, LAYOUT>;
+  using Plain = PageRows<T, D, kRowsPlain>;
+  __shared__ int first_gap;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int waves = blockDim.x >> 6;
+  int b, first, count;
+  int64_t local;
+  if (p.cu) {
+    const PackedTile t = packed_tile(p.cu, p.n_seq, p.n_tokens, p.page_rows, blockIdx.x, lane, 2);
+    b = t.b;
+    first = t.first;
+    count = t.count;
+    local = t.local;
+  } else {
+    b = blockIdx.x;
+    first = b;
+    count = 1;
+    local = 0;
+  }
+  if (local < 0) return;
+  const int64_t past = p.seq_lens[b];
+  if (local == 0 && blockIdx.y == 0) {
+    // the length: up to the first position without a page
+    if (tid == 0) first_gap = INT32_MAX;
+    __syncthreads();  // (and every thread has read the length, which may be written in place)
+    const int64_t end = past + count;
+    if (past >= 0 && count > 0)
+      for (int64_t lp = past / p.page_rows + tid; lp * p.page_rows < end; lp += blockDim.x)
+        if (write_page(p, b, lp) < 0) {
+          atomicMin(&first_gap, (int)lp);
+          break;
+        }
+    __syncthreads();
+    if (tid == 0) {
+      int64_t len = past;
+      if (past >= 0) {
+        const int64_t gap = (int64_t)first_gap * p.page_rows;
+        len = end < gap ? end : past > gap ? past : gap;
+      }
+      p.new_lens[b] = (int)len;
+    }
+  }
+  const int64_t start = past < 0 ? 0 : past;  // (a negative length: the queries only)
+  const int64_t lp = start / p.page_rows + local, base = lp * p.page_rows;
+  if (base >= start + count) return;
+  WritePage w;
+  w.page = past < 0 ? -1 : write_page(p, b, lp);
+  w.tok = first + (base - start);
+  w.lo = (int)(start > base ? start - base : 0);
+  w.hi = (int)(start + count - base < p.page_rows ? start + count - base : p.page_rows);
+  w.sub0 = w.lo / kSub;
+  w.sub1 = (w.hi + kSub - 1) / kSub;
+  const int64_t pos0 = base + (past < 0 ? past : 0);
+  const int kv0 = blockIdx.y * p.kv_heads_per_wg, kv1 = min(kv0 + p.kv_heads_per_wg, p.n_kv_heads);
+  Turned turned(p, w, lane);
+  Plain plain(p, w, lane);
+  const int n_kv = kv1 - kv0, n_q = p.q ? n_kv * p.group : 0;
+  for (int sub = w.sub0; sub < w.sub1; ++sub) {
+    turned.angles(sub, pos0);
+    for (int i = wave; i < n_q; i += waves) {
+      const int64_t h = (int64_t)kv0 * p.group + i;
+      typename Turned::Unit x[Turned::kGroups];
+      turned.load(x, p.q + h * p.q_head, p.q_tok, sub);
+      turned.put(x, p.q_out + h * p.qo_head, p.qo_tok, w.tok, sub);
+    }
+    if (FP8 || w.page < 0) continue;
+    for (int i = wave; i < 2 * n_kv; i += waves) {
+      const int64_t h = kv0 + (i < n_kv ? i : i - n_kv);
+      if (i < n_kv) {
+        typename Turned::Unit x[Turned::kGroups];
+        turned.load(x, p.k_new + h * p.kn_head, p.kn_tok, sub);
+        turned.put(x, p.k + w.page * p.k_page + h * p.k_head, p.k_tok, 0, sub);
+      } else {
+        typename Plain::Unit x[Plain::kGroups];
+        plain.load(x, p.v_new + h * p.vn_head, p.vn_tok, sub);
+        plain.put(x, p.v + w.page * p.v_page + h * p.v_head, p.v_tok, 0, sub);
+      }
+    }
+  }
+  if constexpr (FP8) {
+    if (w.page < 0) return;
+    for (int i = wave; i < 2 * n_kv; i += waves) {
+      const int64_t h = kv0 + (i < n_kv ? i : i - n_kv);
+      if (i < n_kv)
+        turned.quantise(p.k_new + h * p.kn_head, p.kn_tok, p.k + w.page * p.k_page + h * p.k_head, p.k_tok,
+                        p.k_scale + w.page * p.scale_page + h, pos0, lane);
+      else
+        plain.quantise(p.v_new + h * p.vn_head, p.vn_tok, p.v + w.page * p.v_page + h * p.v_head, p.v_tok,
+                       p.v_scale + w.page * p.scale_page + h, pos0, lane);
+    }
+  }
+}
+
+template <typename T, bool FP8, int D>
+void launch_write(int layout, dim3 grid, dim3 block, hipStream_t st, const WriteParams& p) {
+  if (layout == kRowsHalf)
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalf>), grid, block, 0, st, p);
+  else if (layout == kRowsInterleaved)
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsInterleaved>), grid, block, 0, st, p);
+  else if (layout == kRowsHalfOdd)
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalfOdd>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsPlain>), grid, block, 0, st, p);
+}
+
+template <typename T, bool FP8>
+void launch_write_d(int d, int layout, dim3 grid, dim3 block, hipStream_t st, const WriteParams& p) {
+  if (d == 64)
+    launch_write<T, FP8, 64>(layout, grid, block, st, p);
+  else
+    launch_write<T, FP8, 128>(layout, grid, block, st, p);
+}
+
+}  // namespace
+}  // namespace ia
+
+extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows* q, const ia_packed_kv* rows,
+                                   const ia_paged_kv* kv, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                                   int32_t* new_seq_lens, const int32_t* positions, int32_t n_seq, int32_t n_tokens,
+                                   int32_t n_kv_heads, int32_t head_dim, void* stream) {
+  using namespace ia;
+  if (!rows || (n_seq > 0 && (!seq_lens || !new_seq_lens))) return fail(IA_ERR_INVALID, "null pointer argument");
+  if (head_dim != 64 && head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  int rc = check_kv(kv, head_dim);
+  if (rc) return rc;
+  if (rotary && (rc = check_rotary(rotary, head_dim))) return rc;
+  const bool fp8 = kv->dtype == IA_FP8_E4M3;
+  if (rows->dtype != IA_F32 && rows->dtype != IA_BF16) return fail(IA_ERR_INVALID, "the new rows must be f32 or bf16");
+  if (!fp8 && rows->dtype != kv->dtype) return fail(IA_ERR_INVALID, "the new rows must have the pool's dtype");
+  if (fp8 && kv->n_pages > 1 && kv->scale_page_stride < n_kv_heads)
+    return fail(IA_ERR_INVALID, "every page needs scales of its own");
+  if (kv->seq_scale) return fail(IA_ERR_INVALID, "scales gathered per sequence are not written: pass none");
+  if (n_seq < 0 || n_tokens < 0 || n_kv_heads <= 0) return fail(IA_ERR_INVALID, "sequence, token or head counts");
+  if (n_tokens > 0 && (!rows->k || !rows->v)) return fail(IA_ERR_INVALID, "null pointer argument");
+  if (!cu_seqlens && n_tokens != n_seq)
+    return fail(IA_ERR_INVALID, "without cu_seqlens every sequence has one token");
+  const int eb = rows->dtype == IA_F32 ? 4 : 2, pb = fp8 ? 1 : eb;
+  const int64_t strides[4] = {rows->k_token_stride, rows->k_head_stride, rows->v_token_stride, rows->v_head_stride};
+  for (int64_t s : strides)
+    if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
+  if ((reinterpret_cast<uintptr_t>(rows->k) | reinterpret_cast<uintptr_t>(rows->v)) % 16)
+    return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
+  const bool in_place = n_seq > 0 && new_seq_lens == seq_lens;
+  if (in_place && cu_seqlens)
+    return fail(IA_ERR_INVALID, "lengths advance in place for single tokens only (cu_seqlens null)");
+  WriteParams p{};
+  p.group = 1;
+  if (q) {
+    if (q->n_heads <= 0 || q->n_heads % n_kv_heads)
+      return fail(IA_ERR_INVALID, "n_q_heads must be a positive multiple of n_kv_heads");
+    if (n_tokens > 0 && (!q->in || !q->out)) return fail(IA_ERR_INVALID, "null pointer argument");
+    const int64_t qs[4] = {q->in_token_stride, q->in_head_stride, q->out_token_stride, q->out_head_stride};
+    for (int64_t s : qs)
+      if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
+    if ((reinterpret_cast<uintptr_t>(q->in) | reinterpret_cast<uintptr_t>(q->out)) % 16)
+      return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
+    p.q = static_cast<const char*>(q->in);
+    p.q_out = static_cast<char*>(q->out);
+    p.q_tok = q->in_token_stride * eb;
+    p.q_head = q->in_head_stride * eb;
+    p.qo_tok = q->out_token_stride * eb;
+    p.qo_head = q->out_head_stride * eb;
+    p.group = q->n_heads / n_kv_heads;
+  }
+  if (n_seq == 0) return IA_OK;
+  p.k_new = static_cast<const char*>(rows->k);
+  p.v_new = static_cast<const char*>(rows->v);
+  p.kn_tok = rows->k_token_stride * eb;
+  p.kn_head = rows->k_head_stride * eb;
+  p.vn_tok = rows->v_token_stride * eb;
+  p.vn_head = rows->v_head_stride * eb;
+  p.k = static_cast<char*>(const_cast<void*>(kv->k));
+  p.v = static_cast<char*>(const_cast<void*>(kv->v));
+  p.k_page = kv->k_page_stride * pb;
+  p.k_head = kv->k_head_stride * pb;
+  p.k_tok = kv->k_token_stride * pb;
+  p.v_page = kv->v_page_stride * pb;
+  p.v_head = kv->v_head_stride * pb;
+  p.v_tok = kv->v_token_stride * pb;
+  p.k_scale = const_cast<float*>(kv->k_scale);
+  p.v_scale = const_cast<float*>(kv->v_scale);
+  p.scale_page = kv->scale_page_stride;
+  p.table = kv->block_table;
+  p.bt_stride = kv->bt_stride;
+  p.bt_cols = kv->bt_cols;
+  p.n_pages = kv->n_pages;
+  p.page_rows = kv->page_size;
+  p.cu = cu_seqlens;
+  p.seq_lens = seq_lens;
+  p.new_lens = new_seq_lens;
+  p.positions = positions;
+  p.n_seq = n_seq;
+  p.n_tokens = n_tokens;
+  p.n_kv_heads = n_kv_heads;
+  p.rot = RotaryArgs{rotary ? reinterpret_cast<const unsigned long long*>(rotary->turns) : nullptr,
+                     rotary ? rotary->dim : 0, rotary ? rotary->factor : 1.f, 1.f};
+  const int64_t tiles = cu_seqlens ? (int64_t)n_tokens / p.page_rows + 2 * (int64_t)n_seq : n_seq;
+  if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  // few tiles: a workgroup for each kv head.  Lengths that advance in place are read by one
+  // workgroup only, of as many waves as it has tasks.
+  int threads = kWriteThreads;
+  p.kv_heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
+  if (in_place) {
+    p.kv_heads_per_wg = n_kv_heads;
+    threads = std::min(kWriteMaxThreads, 64 * (2 + (q ? p.group : 0)) * n_kv_heads);
+  }
+  const int64_t ny = (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg;
+  if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
+  const dim3 grid((unsigned)tiles, (unsigned)ny), block((unsigned)threads);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int layout = rotary_layout(rotary, eb);
+  if (rows->dtype == IA_BF16)
+    fp8 ? launch_write_d<bf16_t, true>(head_dim, layout, grid, block, st, p)
+        : launch_write_d<bf16_t, false>(head_dim, layout, grid, block, st, p);
+  else
+    fp8 ? launch_write_d<float, true>(head_dim, layout, grid, block, st, p)
+        : launch_write_d<float, false>(head_dim, layout, grid, block, st, p);
+  return check_launch("rotary append kv");
+}

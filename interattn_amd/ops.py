@@ -235,10 +235,18 @@ def update_block_summaries(summ, pool_k, pool_v, block_table, old_seq_lens, seq_
     return summ
 
 
-def append_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new):
+def append_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, *, scales=None):
     """Write one token per sequence (``k_new, v_new [batch, Hkv, D]``) at position
     ``seq_lens[b]`` of the paged pool and advance ``seq_lens`` in place, on the
-    device (capturable in a graph)."""
+    device (capturable in a graph).  fp8 pools take bf16 or float32 rows and
+    ``scales=(k_scale, v_scale)``, which the call sets for the pages it writes (see
+    ``rotary_append_kv``)."""
+    if scales is not None:
+        from .rotary import rotary_append_kv
+
+        if pool_k.dtype != torch.float8_e4m3fn:
+            raise ValueError("scales are for fp8 pools only")
+        return rotary_append_kv(None, k_new, v_new, None, pool_k, pool_v, block_table, seq_lens, scales=scales)[1]
     kv, keep = paged_kv(pool_k, pool_v, block_table)
     _require_cuda(seq_lens, k_new, v_new)
     _check_i32(seq_lens, "seq_lens")

@@ -156,6 +156,29 @@ def reserve_pages(block_table, seq_lens, refs, new_tokens, *, page_size, workspa
     return ok
 
 
+def reorder_sequences(tensors, block_table, seq_lens, refs, parents, *, page_size, workspace=None):
+    """Every row becomes what row ``parents[row]`` (``[rows] int32`` on the device) was, all at
+    once: beams that follow their parents.  Of the rows with one parent, the parent itself,
+    else the lowest, takes its pages over as they are; the others share its whole pages
+    (``refs`` rise) and get a copy, in every tensor, of the page its last tokens partly fill, in
+    the lowest free page, rows in order.  Pages that no row holds any more are free, for the
+    copies too.  A parent outside the rows (-1) leaves the row empty.  Rows that are no beams
+    are their own parents: nothing of them is touched.  Returns ``ok [rows] int32``: 1, or 0 and
+    the row empty where the partly filled page is not mapped, the length does not fit the
+    table or no page is free.  At most 8192 rows.  What else follows rows (block summaries,
+    sequence scales) is indexed with ``parents`` by the caller."""
+    state = _state(block_table, seq_lens, refs, page_size, parents)
+    desc, n_t, _ = _page_tensors(tensors, state.n_pages, refs)
+    check_ints(parents, "parents", state.rows)
+    ok = torch.empty_like(parents)
+    lib = N.lib()
+    need = max(lib.ia_reorder_workspace_size(state.rows, state.cols), 4)
+    ws = workspace_tensor(workspace, ("reorder_scratch", need), (need,), device=refs.device, dtype=torch.uint8)
+    launch(lib.ia_reorder_sequences, refs, state, desc, n_t, parents.data_ptr(), ok.data_ptr(), ws.data_ptr(),
+           ws.numel())
+    return ok
+
+
 def compact_pages(tensors, block_table, refs, *, workspace=None):
     """Move the live pages to the front of the pools: of ``n_live`` held pages, those at or
     past ``n_live`` move, in ascending order, to the free pages before it; ``block_table`` and

@@ -94,7 +94,7 @@ def _row_layout(k_heads, k_stride, k_dtype, v_heads, v_stride, v_dtype):
                             0 if one else v_stride[1])), k_heads[0], k_heads[1]
 
 
-def _packed_rows(k, v):
+def packed_rows(k, v):
     """``(PackedKV, tokens, n_kv_heads, D)``."""
     ks, vs = k.shape, v.shape
     held, hkv, d = _row_layout(ks[1:], k.stride(), k.dtype, vs[1:], v.stride(), v.dtype)
@@ -111,7 +111,7 @@ def _packed_rows(k, v):
 _POOLS = {}  # layouts of pools -> (PagedKV bytes, n_kv_heads, D)
 
 
-def _pool(pool_k, pool_v, block_table, scales, n_seq):
+def pool_of(pool_k, pool_v, block_table, scales, n_seq):
     """``(PagedKV, n_kv_heads, D)``: ``ops.paged_kv``'s struct, its table of ``n_seq`` rows."""
     key = [pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype]
     if block_table is not None:
@@ -181,7 +181,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None, out_dtype=Non
     and what ``_sdpa_prefill_attention_forward`` (CBT/core.py:1180-1200) computes, without
     padding.  Forward only."""
     device_of(q, k, v, cu_seqlens)
-    kv, tokens, hkv, d = _packed_rows(k, v)
+    kv, tokens, hkv, d = packed_rows(k, v)
     shape = _prompt_shape(q, _n_seq(cu_seqlens), hkv, d)
     if shape.n_tokens != tokens:
         raise ValueError("k and v must have q's tokens")
@@ -206,7 +206,7 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     left as ``out`` had them, a row that sees no key is zeros.  Forward only."""
     device_of(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens, *(scales or ()))
     n_seq = _n_seq(cu_seqlens)
-    kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, n_seq)
+    kv, hkv, d = pool_of(pool_k, pool_v, block_table, scales, n_seq)
     shape = _prompt_shape(q, n_seq, hkv, d)
     check_ints(seq_lens, "seq_lens", n_seq)
     out = output(q, out, out_dtype)
@@ -220,32 +220,81 @@ def paged_prompt_attention(q, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
     return out
 
 
-def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, *, new_seq_lens=None):
+def prompt_lengths(seq_lens, new_seq_lens, n_seq, in_place=False):
+    """Where an append writes the lengths after it; ``in_place`` ``seq_lens`` itself may be it
+    (and is by default)."""
+    if new_seq_lens is None:
+        return seq_lens if in_place else torch.empty_like(seq_lens)
+    check_ints(new_seq_lens, "new_seq_lens", n_seq)
+    apart = abs(new_seq_lens.data_ptr() - seq_lens.data_ptr())
+    if n_seq and apart < 4 * n_seq and not (in_place and apart == 0):
+        raise ValueError("new_seq_lens must not overlap seq_lens")
+    return new_seq_lens
+
+
+def append_prompt_kv(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, *, scales=None,
+                     new_seq_lens=None):
     """Write the K/V rows of packed prompts (``k_new, v_new [tokens, Hkv, D]`` of the pool's
     dtype, any token and head strides) into the pool: sequence b's rows go to positions
     ``seq_lens[b], seq_lens[b] + 1, ...`` through the block table.  Returns the lengths
     after it, ``[n_seq] int32`` (``new_seq_lens`` when given; never ``seq_lens`` itself, so
     ``update_block_summaries`` can have both).  A position without a page is skipped and the
-    length counts up to the first of them.  The many-token form of ``append_kv``: bf16 and
-    float32 pools, capturable."""
-    device_of(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, new_seq_lens)
+    length counts up to the first of them.  The many-token form of ``append_kv``, capturable.
+    fp8 pools take bf16 or float32 rows and ``scales=(k_scale, v_scale)``, which the call sets
+    for the pages it writes (see ``rotary_append_kv``)."""
+    device_of(pool_k, pool_v, block_table, seq_lens, k_new, v_new, cu_seqlens, new_seq_lens, *(scales or ()))
     n_seq = _n_seq(cu_seqlens)
     check_ints(seq_lens, "seq_lens", n_seq)
+    if scales is not None:
+        from .rotary import rotary_append_kv
+
+        if pool_k.dtype != torch.float8_e4m3fn:
+            raise ValueError("scales are for fp8 pools only")
+        return rotary_append_kv(None, k_new, v_new, None, pool_k, pool_v, block_table, seq_lens, cu_seqlens,
+                                scales=scales, new_seq_lens=new_seq_lens)[1]
     if pool_k.dtype not in (_F32, _BF16):
-        raise ValueError("append takes bf16 or float32 pools")
-    kv, hkv, d = _pool(pool_k, pool_v, block_table, None, n_seq)
-    rows, tokens, *heads = _packed_rows(k_new, v_new)
+        raise ValueError("append takes bf16 or float32 pools, or fp8 ones with scales=(k_scale, v_scale)")
+    kv, hkv, d = pool_of(pool_k, pool_v, block_table, None, n_seq)
+    rows, tokens, *heads = packed_rows(k_new, v_new)
     if heads != [hkv, d] or rows.dtype != kv.dtype:
         raise ValueError("k_new/v_new must be [tokens, Hkv, D] of the pool dtype with contiguous rows")
-    if new_seq_lens is None:
-        new_seq_lens = torch.empty_like(seq_lens)
-    else:
-        check_ints(new_seq_lens, "new_seq_lens", n_seq)
-        if n_seq and abs(new_seq_lens.data_ptr() - seq_lens.data_ptr()) < 4 * n_seq:
-            raise ValueError("new_seq_lens must not overlap seq_lens")
+    new_seq_lens = prompt_lengths(seq_lens, new_seq_lens, n_seq)
     launch(N.lib().ia_append_prompt_kv, pool_k, kv, rows, cu_seqlens.data_ptr(), seq_lens.data_ptr(),
            new_seq_lens.data_ptr(), n_seq, tokens, hkv, d)
     return new_seq_lens
+
+
+def read_kv(pool_k, pool_v, block_table, starts, cu_seqlens, n_tokens, *, scales=None, out_dtype=None, k_out=None,
+            v_out=None):
+    """Cached rows as packed tensors again, the way back from ``append_prompt_kv``: rows
+    ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` of ``k, v [n_tokens, Hkv, D]`` are positions
+    ``starts[b], starts[b] + 1, ...`` (``[n_seq] int32`` on the device) of sequence b, fp8 codes
+    times their page's scale.  ``n_tokens`` is the packed rows in all, known on the host;
+    ``out_dtype`` bf16 or float32 (the pool's by default, bf16 of fp8 pools).  For what a
+    quantised cache really holds, sequences that move elsewhere, attention that wants packed
+    K/V.  Positions without a page give zeros; rows of no sequence are left as ``k_out`` /
+    ``v_out`` had them.  Any pool, capturable."""
+    device_of(pool_k, pool_v, block_table, starts, cu_seqlens, k_out, v_out, *(scales or ()))
+    n_seq = _n_seq(cu_seqlens)
+    check_ints(starts, "starts", n_seq)
+    kv, hkv, d = pool_of(pool_k, pool_v, block_table, scales, n_seq)
+    if n_tokens < 0:
+        raise ValueError("n_tokens must be >= 0")
+    out_dtype = out_dtype or (pool_k.dtype if pool_k.dtype in (_F32, _BF16) else _BF16)
+    if out_dtype not in (_F32, _BF16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    shape = (int(n_tokens), hkv, d)
+    outs = []
+    for out in (k_out, v_out):
+        if out is None:
+            out = torch.empty(shape, device=pool_k.device, dtype=out_dtype)
+        elif out.shape != shape or out.dtype != out_dtype or not out.is_contiguous():
+            raise ValueError(f"k_out and v_out must be contiguous {list(shape)} tensors of out_dtype")
+        outs.append(out)
+    k, v = outs
+    launch(N.lib().ia_read_kv, pool_k, kv, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[out_dtype], starts.data_ptr(),
+           cu_seqlens.data_ptr(), n_seq, shape[0], hkv, d)
+    return k, v
 
 
 def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *, scale=None,
@@ -263,7 +312,7 @@ def shared_prefix_decode(q, pool_k, pool_v, block_table, seq_lens, group_starts,
     float32 and fp8 pools; at most 32768 sequences and as many groups."""
     device_of(q, pool_k, pool_v, block_table, seq_lens, group_starts, shared_lens, *(scales or ()))
     b = check_ints(seq_lens, "seq_lens")
-    kv, hkv, d = _pool(pool_k, pool_v, block_table, scales, b)
+    kv, hkv, d = pool_of(pool_k, pool_v, block_table, scales, b)
     rows = _prompt_shape(q, 0, hkv, d)  # (checks q; a row per sequence)
     hq = rows.n_q_heads
     if rows.n_tokens != b:
