@@ -233,14 +233,15 @@ struct MergeParams {
 
 __global__ __launch_bounds__(kMergeThreads) void ia_beam_merge(MergeParams p) {
   __shared__ unsigned long long near_keys[kNear], near_places[kNear];  // of those that stay
-  __shared__ double lse[kMaxBeams];
+  __shared__ double log_sum[kMaxBeams];
+  __shared__ float top[kMaxBeams];
   __shared__ u32 wave_least[kMergeThreads / 64];
   __shared__ int stay;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int total = p.beams * p.slices * p.n;
   unsigned long long* far_keys = p.far + 2 * (size_t)b * total;
   unsigned long long* far_places = far_keys + total;
-  // each beam's log of the sum; +infinity where the beam has nothing to offer
+  // each beam's reference and log of its sum; +infinity where the beam has nothing to offer
   for (int j = wave; j < p.beams; j += kMergeThreads / 64) {
     const int64_t row = (int64_t)b * p.beams + j;
     float m = kNegInf;
@@ -255,7 +256,10 @@ __global__ __launch_bounds__(kMergeThreads) void ia_beam_merge(MergeParams p) {
         if (r != kNegInf) l += p.sum[row * p.slices + s] * exp((double)r - (double)m);
       }
     for (int s = 32; s > 0; s >>= 1) l += __shfl_xor(l, s, 64);
-    if (lane == 0) lse[j] = l > 0. ? (double)m + log(l) : (double)__builtin_huge_valf();
+    if (lane == 0) {
+      top[j] = m;
+      log_sum[j] = l > 0. ? log(l) : (double)__builtin_huge_valf();
+    }
   }
   if (tid == 0) stay = 0;
   __syncthreads();
@@ -272,7 +276,9 @@ __global__ __launch_bounds__(kMergeThreads) void ia_beam_merge(MergeParams p) {
       }
     } else {
       const Candidate c = p.best[row * p.slices * p.n + (i - j * p.slices * p.n)];
-      if (c.at != 0xffffffffu) key = (double)p.scores[row] + ((double)order_value(c.key) - lse[j]);
+      // (x - top is exact: rows that differ by a constant have the same keys)
+      if (c.at != 0xffffffffu)
+        key = (double)p.scores[row] + (((double)order_value(c.key) - (double)top[j]) - log_sum[j]);
       at = c.at;
     }
     *place = (unsigned long long)j * (u32)p.vocab + at;
