@@ -263,11 +263,14 @@ class PagedTopkDecodeRunner:
     run the HIP paged dense decode.  Prompts of one batch share a length (no
     padding).  With ``native_prompt=True`` the prefill runs ``prompt_attention`` and
     ``append_prompt_kv`` instead of SDPA and the copy, except where dropout or gradients
-    are asked for; either way it is causal and reads no ``attention_mask``.  Install with
-    ``condition_block_decode_context(runner)``."""
+    are asked for; either way it is causal and reads no ``attention_mask``.  With
+    ``kv_dtype=torch.float8_e4m3fn`` the pools hold 8 bits a value and a scale per (page, kv
+    head), set as rows are written (bf16 models); the prompt attends its own rows, decode the
+    rounded ones.
+    Install with ``condition_block_decode_context(runner)``."""
 
     def __init__(self, *, model, batch_size, max_seq_len, block_size, k, forced_first=0, forced_last=0,
-                 page_size=16, full_attention_layers=0, k_bar_dtype=None, seed=0, native_prompt=False):
+                 page_size=16, full_attention_layers=0, k_bar_dtype=None, seed=0, native_prompt=False, kv_dtype=None):
         from . import ops, prompt
 
         self._ops, self._prompt = ops, prompt
@@ -277,6 +280,11 @@ class PagedTopkDecodeRunner:
         self.device, self.dtype = param.device, param.dtype
         if self.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("the paged runner serves bf16 or fp32 models")
+        self.kv_dtype = kv_dtype or self.dtype
+        if self.kv_dtype not in (self.dtype, torch.float8_e4m3fn):
+            raise ValueError("kv_dtype must be the model's dtype or torch.float8_e4m3fn")
+        if self.kv_dtype != self.dtype and self.dtype != torch.bfloat16:
+            raise ValueError("an fp8 cache (kv_dtype) serves bf16 models: its decode takes bf16 queries")
         self.n_layers = int(cfg.num_hidden_layers)
         self.n_kv_heads = int(cfg.num_key_value_heads)
         self.head_dim = int(getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads)
@@ -294,8 +302,11 @@ class PagedTopkDecodeRunner:
         perm = torch.randperm(self.batch_size * pages_per_seq, generator=gen).to(torch.int32)
         self.block_table = perm.view(self.batch_size, pages_per_seq).to(self.device)
         shape = (self.batch_size * pages_per_seq, self.n_kv_heads, self.page_size, self.head_dim)
-        self.pools = [(torch.zeros(shape, device=self.device, dtype=self.dtype),
-                       torch.zeros(shape, device=self.device, dtype=self.dtype)) for _ in range(self.n_layers)]
+        self.pools = [(torch.zeros(shape, device=self.device, dtype=self.kv_dtype),
+                       torch.zeros(shape, device=self.device, dtype=self.kv_dtype)) for _ in range(self.n_layers)]
+        # (k_scale, v_scale) of each layer's fp8 pools
+        self.scales = [(torch.ones(shape[:2], device=self.device), torch.ones(shape[:2], device=self.device))
+                       if self.kv_dtype == torch.float8_e4m3fn else None for _ in range(self.n_layers)]
         # each layer advances its own lengths (append_kv moves them on the device)
         self.seq_lens = [torch.zeros(self.batch_size, device=self.device, dtype=torch.int32)
                          for _ in range(self.n_layers)]
@@ -322,7 +333,17 @@ class PagedTopkDecodeRunner:
             pk, pv = self.pools[layer]
             self.summaries[layer] = self._ops.build_block_summaries(
                 pk, pv, self.block_table, self.seq_lens[layer], self.block_size, nb_max=self.nb_max,
-                k_bar_dtype=self.k_bar_dtype)
+                k_bar_dtype=self.k_bar_dtype, scales=self.scales[layer])
+
+    def _append_prompt(self, layer, k, v, b, t):
+        """The prompts' packed rows into the layer's pool, its summaries; returns ``cu_seqlens``."""
+        cu = torch.arange(0, (b + 1) * t, max(t, 1), device=k.device, dtype=torch.int32)[:b + 1]
+        pk, pv = self.pools[layer]
+        self._prompt.append_prompt_kv(pk, pv, self.block_table, self.old_seq_lens[layer].zero_(), k.to(self.dtype),
+                                      v.to(self.dtype), cu, scales=self.scales[layer],
+                                      new_seq_lens=self.seq_lens[layer])
+        self._summarize(layer)
+        return cu
 
     def _prefill_native(self, layer, query, key, value, scaling):
         """The prompt on the HIP path: its rows packed, K/V into the pool, attention over them."""
@@ -331,11 +352,7 @@ class PagedTopkDecodeRunner:
         if key.shape[2] != t:
             raise ValueError("the native prefill takes whole prompts: as many keys as queries")
         q, k, v = (x.transpose(1, 2).reshape(b * t, x.shape[1], d) for x in (query, key, value))
-        cu = torch.arange(0, (b + 1) * t, max(t, 1), device=query.device, dtype=torch.int32)[:b + 1]
-        pk, pv = self.pools[layer]
-        self._prompt.append_prompt_kv(pk, pv, self.block_table, self.old_seq_lens[layer].zero_(), k.to(pk.dtype),
-                                      v.to(pv.dtype), cu, new_seq_lens=self.seq_lens[layer])
-        self._summarize(layer)
+        cu = self._append_prompt(layer, k, v, b, t)
         out = torch.empty((b, t, hq, d), device=query.device, dtype=query.dtype)
         self._prompt.prompt_attention(q, k, v, cu, scale=scaling, out=out.view(b * t, hq, d),
                                       workspace=self.prompt_workspace)
@@ -345,6 +362,10 @@ class PagedTopkDecodeRunner:
         """Copy the prompt's K/V [B, Hkv, T, D] into the layer's pool, build summaries."""
         self._check_prompt(key)
         b, hkv, t, d = key.shape
+        if self.scales[layer] is not None:
+            k, v = (x.detach().transpose(1, 2).reshape(b * t, hkv, d) for x in (key, value))
+            self._append_prompt(layer, k, v, b, t)
+            return
         pk, pv = self.pools[layer]
         n_pg = -(-t // self.page_size)
         pages = self.block_table[:, :n_pg].reshape(-1).long()
@@ -371,19 +392,22 @@ class PagedTopkDecodeRunner:
         pk, pv = self.pools[layer]
         seq, old = self.seq_lens[layer], self.old_seq_lens[layer]
         old.copy_(seq)
-        ops.append_kv(pk, pv, self.block_table, seq, key[:, :, -1].to(pk.dtype), value[:, :, -1].to(pv.dtype))
+        scales = self.scales[layer]
+        ops.append_kv(pk, pv, self.block_table, seq, key[:, :, -1].to(self.dtype), value[:, :, -1].to(self.dtype),
+                      scales=scales)
         q = query[:, :, 0].contiguous()
         ws = self.workspace_by_layer[layer]
         if layer < self.full_attention_layers:
             out = ops.paged_decode(q, pk, pv, self.block_table, seq, max_seq_len=self.max_seq_len, scale=scaling,
-                                   out_dtype=query.dtype, workspace=ws)
+                                   scales=scales, out_dtype=query.dtype, workspace=ws)
         else:
             summ = self.summaries[layer]
-            ops.update_block_summaries(summ, pk, pv, self.block_table, old, seq, self.block_size, max_new_tokens=1)
+            ops.update_block_summaries(summ, pk, pv, self.block_table, old, seq, self.block_size, max_new_tokens=1,
+                                       scales=scales)
             out = ops.sparse_topk_decode(q, pk, pv, self.block_table, seq, summ["k_bar"], self.k,
                                          block_size=self.block_size, forced_first=self.forced_first,
-                                         forced_last=self.forced_last, scale=scaling, out_dtype=query.dtype,
-                                         workspace=ws)
+                                         forced_last=self.forced_last, scale=scaling, scales=scales,
+                                         out_dtype=query.dtype, workspace=ws)
         return out.unsqueeze(1), None
 
 
