@@ -675,7 +675,8 @@ IA_API int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32_t o
  * score or logsumexp is no number or whose logits reach +infinity, offer nothing.  out_scores,
  * out_tokens and out_rows [batch, n]: score, token and row b * beams + j; where fewer than n
  * are offered, -infinity and the lowest continuations that were not.  beams and n at most 64.
- * The workspace needs no initialisation.
+ * The workspace must be zero-filled before its first use and then left to the library, used
+ * with one set of sizes; calls that share it must not overlap.
  */
 IA_API size_t ia_beam_select_workspace_size(int32_t batch, int32_t beams, int32_t vocab, int32_t n,
                                             int32_t logits_dtype);

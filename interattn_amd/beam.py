@@ -56,7 +56,7 @@ def beam_select(logits, scores, n=None, *, done=None, pad_token=0, workspace=Non
         need = lib.ia_beam_select_workspace_size(batch, beams, vocab, n, code)
         if not need:
             raise ValueError("beam_select: batch or vocabulary too large")
-        ws = workspace_tensor(workspace, key, (need,), device=dev, dtype=torch.uint8)
+        ws = workspace_tensor(workspace, key, (need,), device=dev, dtype=torch.uint8, zero=True)
     launch(lib.ia_beam_select, logits, logits.data_ptr(), code, logits.stride(0) if batch * beams > 1 else vocab,
            scores.data_ptr(), None if done is None else done.data_ptr(), int(pad_token), batch, beams, vocab, n,
            best.data_ptr(), tokens.data_ptr(), parents.data_ptr(), ws.data_ptr(), ws.numel())

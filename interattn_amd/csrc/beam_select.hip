@@ -2,16 +2,15 @@
 //
 //   key(j, v) = scores[j] + logits[j, v] - logsumexp(logits[j])
 //
-//   ia_beam_scan: one pass over the logits.  A wave takes a slice of a row, 16 bytes a lane,
-//     and keeps sum exp(x - M) against a reference M near its running maximum, and the slice's
-//     n best logits (the order inside a row is that of the keys).  A threshold T, below which
-//     nothing can be among them any more, makes the common chunk one comparison: the first
-//     chunk's T is the n-th largest of its lanes' maxima (found bit by bit with ballots), later
-//     ones follow the candidates held.  Candidates wait in LDS and are cut to the n best when
-//     they fill up.
-//   ia_beam_merge: a workgroup per batch entry joins the slices' sums, forms the candidates'
-//     keys in 64 bits (float32 keys of magnitude 10 would order equal what differs by 10^-6)
-//     and ranks those above a threshold.
+// ia_beam_scan, one launch, one pass over the logits.  A wave takes a slice of a row, groups of
+// four 16-byte loads a lane, and keeps sum exp(x - M) against a reference M near its running
+// maximum, and the slice's n best logits (the order inside a row is that of the keys).  What is
+// below the n-th largest of the lanes' running maxima (found bit by bit with ballots) cannot be
+// among them, so a group is one comparison unless it holds something better; candidates wait in
+// LDS and are cut to the n best when they fill up.  The workgroup that ends last of a batch entry
+// joins the slices' sums, forms the candidates' keys in 64 bits (float32 keys of magnitude 10
+// would order equal what differs by 10^-6) and ranks those above a threshold.  Slices are handed
+// over through memory at the device's coherence point (ia_common.hpp).
 //
 // Equal keys go to the lower beam * vocabulary + token.  Bound by reading the logits once.
 #include <algorithm>
@@ -23,13 +22,13 @@ namespace {
 
 constexpr int kScanThreads = 256;
 constexpr int kScanWaves = kScanThreads / 64;
-constexpr int kFly = 4;              // chunks in flight
+constexpr int kFly = 4;              // chunks of a group, and in flight
 constexpr int kHeld = 640;           // candidates a wave holds: a chunk's 512 and some
 constexpr int kTrim = 128;           // candidates at which they are cut to the n best
 constexpr int kMaxBeams = 64, kMaxBest = 64;
-constexpr int kMergeThreads = 256;
-constexpr int kMaxCandidates = 8192;  // of a batch entry
-constexpr int kNear = 1024;           // of those above the threshold, in LDS; more go through memory
+constexpr int kOwn = 8;              // candidates a merging thread keeps in registers
+constexpr int kMaxCandidates = kOwn * kScanThreads;  // of a batch entry, where a slice a row is fewer
+constexpr int kNear = 1024;          // of those above the threshold, in LDS; more go through memory
 constexpr int kTargetWaves = 4096;
 
 // Floats as integers of the same order (-0 before +0).
@@ -59,38 +58,49 @@ __device__ __forceinline__ u32 nth_of_lanes(u32 key, int n) {
   return k;
 }
 
-struct Candidate {
-  u32 key;  // order_key of the logit, -0 as +0
-  u32 at;   // token
-};
+// The least float above the one of key k.
+__device__ __forceinline__ float above(u32 k) { return order_value(k + 1); }
+
+// A candidate: order_key of the logit (-0 as +0) above the token.
+typedef unsigned long long Candidate;
+__device__ __forceinline__ u32 key_of(Candidate c) { return (u32)(c >> 32); }
+__device__ __forceinline__ u32 token_of(Candidate c) { return (u32)c; }
+constexpr Candidate kNoCandidate = 0xffffffffull;
 
 // The n best of cnt candidates (key descending, token ascending) to the front of `held`, in
 // any order; returns their least key.  cnt > n, one wave.
 __device__ u32 trim(Candidate* held, int cnt, int n, int lane) {
+  constexpr int kHere = 3;  // registers' worth; more only where very many are equal
+  Candidate mine[kHere];
+#pragma unroll
+  for (int i = 0; i < kHere; ++i) mine[i] = 64 * i + lane < cnt ? held[64 * i + lane] : 0ull;
   auto reach = [&](auto&& test) {
     int c = 0;
-    for (int i = 0; i < cnt; i += 64) c += __popcll(__ballot(i + lane < cnt && test(held[min(i + lane, cnt - 1)])));
+#pragma unroll
+    for (int i = 0; i < kHere; ++i) c += __popcll(__ballot(64 * i + lane < cnt && test(mine[i])));
+    for (int i = 64 * kHere; i < cnt; i += 64)
+      c += __popcll(__ballot(i + lane < cnt && test(held[min(i + lane, cnt - 1)])));
     return c;
   };
   u32 least = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const u32 t = least | 1u << bit;
-    if (reach([&](const Candidate& c) { return c.key >= t; }) >= n) least = t;
+    if (reach([&](Candidate c) { return key_of(c) >= t; }) >= n) least = t;
   }
   u32 last = 0xffffffffu;  // of those that have the least key, tokens up to `last` stay
-  const int above = reach([&](const Candidate& c) { return c.key > least; });
-  if (reach([&](const Candidate& c) { return c.key == least; }) > n - above) {
-    u32 below = 0;  // the largest bound below which fewer than n - above tokens lie
+  const int better = reach([&](Candidate c) { return key_of(c) > least; });
+  if (reach([&](Candidate c) { return key_of(c) == least; }) > n - better) {
+    u32 below = 0;  // the largest bound below which fewer than n - better tokens lie
     for (int bit = 31; bit >= 0; --bit) {
       const u32 t = below | 1u << bit;
-      if (reach([&](const Candidate& c) { return c.key == least && c.at < t; }) < n - above) below = t;
+      if (reach([&](Candidate c) { return key_of(c) == least && token_of(c) < t; }) < n - better) below = t;
     }
     last = below;
   }
   int kept = 0;
   for (int i = 0; i < cnt; i += 64) {
     const Candidate c = held[min(i + lane, cnt - 1)];
-    const bool keep = i + lane < cnt && (c.key > least || (c.key == least && c.at <= last));
+    const bool keep = i + lane < cnt && (key_of(c) > least || (key_of(c) == least && token_of(c) <= last));
     const unsigned long long m = __ballot(keep);
     wave_lds_sync();  // (read before it is written: entries move towards the front)
     if (keep) held[kept + __popcll(m & ((1ull << lane) - 1))] = c;
@@ -100,16 +110,23 @@ __device__ u32 trim(Candidate* held, int cnt, int n, int lane) {
   return least;
 }
 
-struct ScanParams {
+struct BeamParams {
   const char* logits;
   int64_t row_stride;  // bytes
+  const float* scores;  // [batch, beams]
   const uint8_t* done;  // null: none
-  int32_t vocab, n, slices, slice_chunks;
-  int64_t waves;  // rows * slices
-  // per slice: n candidates, the reference and the sum
+  int32_t beams, vocab, n, slices, slice_chunks, pad_token;
+  int32_t groups;  // workgroups of a batch entry
+  // per slice of a row: n candidates, the reference and the sum; per entry: workgroups that have
+  // ended (0 between calls), candidates' keys and places where kNear is too few
   Candidate* best;
-  double* sum;
+  unsigned long long* sum;  // (a double's bits)
   float* ref;
+  u32* ended;
+  unsigned long long* far;
+  float* out_scores;  // [batch, n]
+  int32_t* out_tokens;
+  int32_t* out_rows;
 };
 
 template <typename T>
@@ -117,23 +134,19 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // 16 bytes at any e
   u32x4_t w;
 };
 
+// One slice of one row: its candidates and sum, handed over.
 template <typename T>
-__global__ __launch_bounds__(kScanThreads) void ia_beam_scan(ScanParams p) {
+__device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held, int64_t row, int slice, int64_t id,
+                                           int lane) {
   constexpr int kVec = RowVec<T, kRowsPlain>::kVec, kChunk = 64 * kVec;
-  __shared__ Candidate all[kScanWaves][kHeld];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = (int64_t)blockIdx.x * kScanWaves + wave;
-  if (id >= p.waves) return;
-  const int64_t row = id / p.slices;
-  const int slice = (int)(id - row * p.slices);
-  if (p.done && p.done[row]) return;
-  Candidate* held = all[wave];
   const T* x0 = reinterpret_cast<const T*>(p.logits + row * p.row_stride);
   const int chunks = (p.vocab + kChunk - 1) / kChunk;
   const int c0 = slice * p.slice_chunks, c1 = min(c0 + p.slice_chunks, chunks);
   const int n = p.n;
 
-  float ref = kNegInf, limit = kNegInf;  // candidates are above `limit` (or any finite, to begin with)
+  float ref = kNegInf;
+  float lo = -3.402823466e38f;  // what is below cannot be among the n best
+  float seen = kNegInf;         // the lane's maximum so far
   double sum = 0.;
   int cnt = 0;
 
@@ -150,47 +163,72 @@ __global__ __launch_bounds__(kScanThreads) void ia_beam_scan(ScanParams p) {
     }
     return w;
   };
-  auto take = [&](const u32x4_t& w, int c) {
-    float x[kVec];
-    widen(w, x, T{});
+  auto take = [&](const u32x4_t* w, int c) {
+    float most[kFly], all = kNegInf;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) x[j] = fmaxf(x[j], kNegInf);  // NaN: never chosen, adds nothing
-    float most = x[0];
+    for (int i = 0; i < kFly; ++i) {
+      float x[kVec];
+      widen(w[i], x, T{});
+      most[i] = kNegInf;  // (a maximum passes over NaN)
 #pragma unroll
-    for (int j = 1; j < kVec; ++j) most = fmaxf(most, x[j]);
-    // (the reference is the maximum of a chunk that is well above the one before: exp stays
-    // below e^8 and few chunks pay for a new one)
-    if (__ballot(most > ref + 8.f)) {
-      const float to = wave_max(most);
+      for (int j = 0; j < kVec; ++j) most[i] = fmaxf(most[i], x[j]);
+      all = fmaxf(all, most[i]);
+    }
+    // (the reference is the maximum of a group that is well above the one before: exp stays
+    // below e^8 and few groups pay for a new one)
+    if (__ballot(all > ref + 8.f)) {
+      const float to = wave_max(all);
       if (ref != kNegInf) sum *= (double)__builtin_amdgcn_exp2f((ref - to) * kLog2e);
       ref = to;
     }
     const float base = ref == kNegInf ? 0.f : ref;
     float part = 0.f;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) part += __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
-    sum += (double)part;
-    const unsigned long long hits = __ballot(most > limit);
-    if (!hits) return;
-    float floor_ = kNegInf;  // what the chunk itself rules out
-    if (__popcll(hits) >= n) floor_ = order_value(nth_of_lanes(order_key(most + 0.f), n));
+    for (int i = 0; i < kFly; ++i) {
+      float x[kVec];
+      widen(w[i], x, T{});
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const bool in = x[j] > limit && x[j] >= floor_;
-      const unsigned long long m = __ballot(in);
-      if (m) {
-        if (in)
-          held[cnt + __popcll(m & ((1ull << lane) - 1))] =
-              Candidate{order_key(x[j] + 0.f), (u32)(c * kChunk + lane * kVec + j)};
-        cnt += __popcll(m);
+      for (int j = 0; j < kVec; ++j) part += __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+    }
+    if (part != part) {  // NaN adds nothing; +infinity leaves the sum NaN: the row offers nothing
+      part = 0.f;
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        float x[kVec];
+        widen(w[i], x, T{});
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) part += x[j] == x[j] ? __builtin_amdgcn_exp2f((x[j] - base) * kLog2e) : 0.f;
       }
     }
-    limit = fmaxf(limit, floor_);
-    wave_lds_sync();
-    if (cnt >= kTrim) {
-      limit = fmaxf(limit, order_value(trim(held, cnt, n, lane)));
-      cnt = n;
+    sum += (double)part;
+    if (!__ballot(all >= lo)) return;
+    seen = fmaxf(seen, all);
+    u32 floor_ = nth_of_lanes(order_key(seen + 0.f), n);  // n values of n lanes reach it
+    lo = fmaxf(lo, order_value(floor_));
+#pragma unroll
+    for (int i = 0; i < kFly; ++i) {
+      if (!__ballot(most[i] >= lo)) continue;
+      float x[kVec];
+      widen(w[i], x, T{});
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const bool in = x[j] >= lo;
+        const unsigned long long m = __ballot(in);
+        if (m) {
+          if (in)
+            held[cnt + __popcll(m & ((1ull << lane) - 1))] =
+                (Candidate)order_key(x[j] + 0.f) << 32 | (u32)((c + i) * kChunk + lane * kVec + j);
+          cnt += __popcll(m);
+        }
+      }
+      if (cnt >= kTrim) {
+        wave_lds_sync();
+        lo = fmaxf(lo, above(trim(held, cnt, n, lane)));
+        cnt = n;
+      }
     }
+    // n values at lower places reach the floor: from here on only what is above it counts
+    if (floor_ > order_key(-3.402823466e38f)) lo = fmaxf(lo, above(floor_));
   };
 
   u32x4_t cur[kFly], nxt[kFly];
@@ -199,172 +237,212 @@ __global__ __launch_bounds__(kScanThreads) void ia_beam_scan(ScanParams p) {
   for (int c = c0; c < c1; c += kFly) {
 #pragma unroll
     for (int i = 0; i < kFly; ++i) nxt[i] = load(c + kFly + i);
-#pragma unroll
-    for (int i = 0; i < kFly; ++i)
-      if (c + i < c1) take(cur[i], c + i);
+    take(cur, c);
 #pragma unroll
     for (int i = 0; i < kFly; ++i) cur[i] = nxt[i];
   }
+  wave_lds_sync();
   if (cnt > n) {
     trim(held, cnt, n, lane);
     cnt = n;
+    wave_lds_sync();
   }
-  wave_lds_sync();
   for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
-  if (lane < n) p.best[id * n + lane] = lane < cnt ? held[lane] : Candidate{0u, 0xffffffffu};
+  if (lane < n) st_agent_u64(p.best + id * n + lane, lane < cnt ? held[lane] : kNoCandidate);
   if (lane == 0) {
-    p.sum[id] = sum;
-    p.ref[id] = ref;
+    st_agent_u64(p.sum + id, (unsigned long long)__double_as_longlong(sum));
+    st_agent(p.ref + id, ref);
   }
 }
 
-struct MergeParams {
-  const float* scores;  // [batch, beams]
-  const uint8_t* done;
-  const Candidate* best;
-  const double* sum;
-  const float* ref;
-  unsigned long long* far;  // per batch entry: candidates' keys, then places, where kNear is too few
-  int32_t beams, vocab, n, slices, pad_token;
-  float* out_scores;  // [batch, n]
-  int32_t* out_tokens;
-  int32_t* out_rows;
+struct MergeLds {
+  unsigned long long keys[kNear], places[kNear];  // of those that stay
+  double log_sum[kMaxBeams];
+  float top[kMaxBeams];
+  u32 least[kScanWaves];
+  int rank[kNear];
+  int stay;
 };
 
-__global__ __launch_bounds__(kMergeThreads) void ia_beam_merge(MergeParams p) {
-  __shared__ unsigned long long near_keys[kNear], near_places[kNear];  // of those that stay
-  __shared__ double log_sum[kMaxBeams];
-  __shared__ float top[kMaxBeams];
-  __shared__ u32 wave_least[kMergeThreads / 64];
-  __shared__ int stay;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int total = p.beams * p.slices * p.n;
+// The n best of a batch entry's candidates, by the whole workgroup.
+__device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per_beam = p.slices * p.n, total = p.beams * per_beam;
+  const int64_t row0 = (int64_t)b * p.beams;
   unsigned long long* far_keys = p.far + 2 * (size_t)b * total;
   unsigned long long* far_places = far_keys + total;
+  Candidate own[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i)
+    own[i] = i * kScanThreads + tid < total ? ld_agent_u64(p.best + row0 * per_beam + i * kScanThreads + tid) : kNoCandidate;
   // each beam's reference and log of its sum; +infinity where the beam has nothing to offer
-  for (int j = wave; j < p.beams; j += kMergeThreads / 64) {
-    const int64_t row = (int64_t)b * p.beams + j;
+  for (int j = wave; j < p.beams; j += kScanWaves) {
+    const int64_t at = (row0 + j) * p.slices;
+    const bool ended = p.done && p.done[row0 + j];
     float m = kNegInf;
-    const bool ended = p.done && p.done[row];
     if (!ended)
-      for (int s = lane; s < p.slices; s += 64) m = fmaxf(m, p.ref[row * p.slices + s]);
+      for (int s = lane; s < p.slices; s += 64) m = fmaxf(m, ld_agent(p.ref + at + s));
     m = wave_max(m);
-    double l = 0.;
+    double t = 0.;
     if (!ended && m != kNegInf)
       for (int s = lane; s < p.slices; s += 64) {
-        const float r = p.ref[row * p.slices + s];
-        if (r != kNegInf) l += p.sum[row * p.slices + s] * exp((double)r - (double)m);
+        const float r = ld_agent(p.ref + at + s);
+        // (a reference of -infinity: nothing was added)
+        if (r != kNegInf) t += __longlong_as_double((long long)ld_agent_u64(p.sum + at + s)) * exp((double)r - (double)m);
       }
-    for (int s = 32; s > 0; s >>= 1) l += __shfl_xor(l, s, 64);
+    for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s, 64);
     if (lane == 0) {
-      top[j] = m;
-      log_sum[j] = l > 0. ? log(l) : (double)__builtin_huge_valf();
+      l.top[j] = m;
+      l.log_sum[j] = t > 0. ? log(t) : (double)__builtin_huge_valf();
     }
   }
-  if (tid == 0) stay = 0;
+  if (tid == 0) l.stay = 0;
   __syncthreads();
   const unsigned long long none = order_key64((double)kNegInf);
-  auto candidate = [&](int i, unsigned long long* place) {
-    const int j = i / (p.slices * p.n);
-    const int64_t row = (int64_t)b * p.beams + j;
+  // key of candidate i (0: cannot be chosen) and its place
+  auto key_place = [&](int i, Candidate c, unsigned long long* place) {
+    const int j = i / per_beam;
     double key = (double)kNegInf;
-    u32 at = 0;
-    if (p.done && p.done[row]) {
-      if (i == j * p.slices * p.n) {
-        key = (double)p.scores[row];
-        at = (u32)p.pad_token;
-      }
-    } else {
-      const Candidate c = p.best[row * p.slices * p.n + (i - j * p.slices * p.n)];
+    u32 at = token_of(c);
+    if (p.done && p.done[row0 + j]) {
+      at = (u32)p.pad_token;
+      if (i == j * per_beam) key = (double)p.scores[row0 + j];
+    } else if (c != kNoCandidate) {
       // (x - top is exact: rows that differ by a constant have the same keys)
-      if (c.at != 0xffffffffu)
-        key = (double)p.scores[row] + (((double)order_value(c.key) - (double)top[j]) - log_sum[j]);
-      at = c.at;
+      key = (double)p.scores[row0 + j] + (((double)order_value(key_of(c)) - (double)l.top[j]) - l.log_sum[j]);
     }
-    *place = (unsigned long long)j * (u32)p.vocab + at;
+    *place = (unsigned long long)j << 32 | at;
     const unsigned long long k = key == key ? order_key64(key + 0.) : none;
-    return k <= none ? 0ull : k;  // (nothing is below -infinity: 0 marks what cannot be chosen)
+    return k <= none ? 0ull : k;
   };
   // a threshold on the keys' upper halves that n candidates of some wave reach
+  unsigned long long own_key[kOwn], own_place[kOwn];
   u32 mine = 0;
-  for (int i = tid; i < total; i += kMergeThreads) {
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    own_key[i] = 0;
+    if (i * kScanThreads + tid < total) own_key[i] = key_place(i * kScanThreads + tid, own[i], &own_place[i]);
+    mine = max(mine, (u32)(own_key[i] >> 32));
+  }
+  for (int i = kMaxCandidates + tid; i < total; i += kScanThreads) {
     unsigned long long place;
-    mine = max(mine, (u32)(candidate(i, &place) >> 32));
+    mine = max(mine, (u32)(key_place(i, ld_agent_u64(p.best + row0 * per_beam + i), &place) >> 32));
   }
   const u32 least = nth_of_lanes(mine, p.n);
-  if (lane == 0) wave_least[wave] = least;
+  if (lane == 0) l.least[wave] = least;
   __syncthreads();
   u32 limit = 0;
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 64; ++w) limit = max(limit, wave_least[w]);
-  for (int i = tid; i < total; i += kMergeThreads) {
-    unsigned long long place;
-    const unsigned long long k = candidate(i, &place);
-    if (k == 0 || (u32)(k >> 32) < limit) continue;
-    const int at = atomicAdd(&stay, 1);
+  for (int w = 0; w < kScanWaves; ++w) limit = max(limit, l.least[w]);
+  auto keep = [&](unsigned long long k, unsigned long long place) {
+    if (k == 0 || (u32)(k >> 32) < limit) return;
+    const int at = atomicAdd(&l.stay, 1);
     if (at < kNear) {
-      near_keys[at] = k;
-      near_places[at] = place;
+      l.keys[at] = k;
+      l.places[at] = place;
+      l.rank[at] = 0;
     }
     far_keys[at] = k;
     far_places[at] = place;
+  };
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) keep(own_key[i], own_place[i]);
+  for (int i = kMaxCandidates + tid; i < total; i += kScanThreads) {
+    unsigned long long place;
+    const unsigned long long k = key_place(i, ld_agent_u64(p.best + row0 * per_beam + i), &place);
+    keep(k, place);
   }
-  __threadfence();
+  __threadfence_block();
   __syncthreads();
   // ranks: better keys, and equal ones at lower places
-  const int count = stay;
-  auto rank_all = [&](const unsigned long long* keys, const unsigned long long* places) {
-    for (int i = tid; i < count; i += kMergeThreads) {
-      const unsigned long long k = keys[i], at = places[i];
-      int rank = 0;
-      for (int o = 0; o < count; ++o) rank += keys[o] > k || (keys[o] == k && places[o] < at);
-      if (rank >= p.n) continue;
-      const int64_t to = (int64_t)b * p.n + rank;
-      const int j = (int)(at / (u32)p.vocab);
-      p.out_scores[to] = (float)order_value64(k);
-      p.out_tokens[to] = (int32_t)(at - (unsigned long long)j * (u32)p.vocab);
-      p.out_rows[to] = b * p.beams + j;
-    }
+  const int count = l.stay;
+  auto put = [&](int rank, double score, unsigned long long place) {
+    const int64_t to = (int64_t)b * p.n + rank;
+    p.out_scores[to] = (float)score;
+    p.out_tokens[to] = (int32_t)(u32)place;
+    p.out_rows[to] = (int)(row0 + (int64_t)(place >> 32));
   };
-  if (count <= kNear)
-    rank_all(near_keys, near_places);
-  else
-    rank_all(far_keys, far_places);
+  if (count <= kNear) {
+    // a wave counts for every candidate against a quarter of them
+    for (int i = lane; i < count; i += 64) {
+      const unsigned long long k = l.keys[i], at = l.places[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int o = wave; o < count; o += kScanWaves) rank += l.keys[o] > k || (l.keys[o] == k && l.places[o] < at);
+      atomicAdd(&l.rank[i], rank);
+    }
+    __syncthreads();
+    for (int i = tid; i < count; i += kScanThreads)
+      if (l.rank[i] < p.n) put(l.rank[i], order_value64(l.keys[i]), l.places[i]);
+  } else {
+    for (int i = tid; i < count; i += kScanThreads) {
+      const unsigned long long k = far_keys[i], at = far_places[i];
+      int rank = 0;
+      for (int o = 0; o < count; ++o) rank += far_keys[o] > k || (far_keys[o] == k && far_places[o] < at);
+      if (rank < p.n) put(rank, order_value64(k), at);
+    }
+  }
   // fewer candidates than places: -infinity, the lowest ones that are none
   if (count < p.n && tid == 0) {
-    unsigned long long at = 0;
-    for (int r = count; r < p.n; ++at) {
+    int j = 0, v = 0;
+    for (int r = count; r < p.n;) {
+      const unsigned long long place = (unsigned long long)j << 32 | (u32)v;
       bool is = false;
-      for (int o = 0; o < count; ++o) is |= near_places[o] == at;
-      if (is) continue;
-      const int64_t to = (int64_t)b * p.n + r++;
-      const int j = (int)(at / (u32)p.vocab);
-      p.out_scores[to] = kNegInf;
-      p.out_tokens[to] = (int32_t)(at - (unsigned long long)j * (u32)p.vocab);
-      p.out_rows[to] = b * p.beams + j;
+      for (int o = 0; o < count; ++o) is |= l.places[o] == place;
+      if (!is) put(r++, (double)kNegInf, place);
+      if (++v == p.vocab) {
+        v = 0;
+        ++j;
+      }
     }
   }
 }
 
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void ia_beam_scan(BeamParams p) {
+  __shared__ union {
+    Candidate held[kScanWaves][kHeld];
+    MergeLds merge;
+  } lds;
+  __shared__ u32 before;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.x / p.groups, local = (blockIdx.x - b * p.groups) * kScanWaves + wave;
+  if (local < p.beams * p.slices) {
+    const int j = local / p.slices, slice = local - j * p.slices;
+    const int64_t row = (int64_t)b * p.beams + j;
+    if (!p.done || !p.done[row]) scan_slice<T>(p, lds.held[wave], row, slice, row * p.slices + slice, lane);
+  }
+  // the workgroup that ends last merges
+  wait_memory();
+  __syncthreads();
+  if (threadIdx.x == 0) before = fetch_add_agent_u32(p.ended + b, 1);
+  __syncthreads();
+  if (before != (u32)p.groups - 1) return;
+  if (threadIdx.x == 0) st_agent_u32(p.ended + b, 0);
+  merge_entry(p, lds.merge, b);
+}
+
 struct BeamPlan {
-  int64_t rows, waves;
-  int slices, slice_chunks;
-  size_t best, sum, ref, far, total;  // offsets in the workspace
+  int64_t waves;
+  int slices, slice_chunks, groups;
+  size_t ended, best, sum, ref, far, total;  // offsets in the workspace
 };
 
 // Slices of a row: about kTargetWaves waves in all, two chunks each at least, and no more
-// candidates for a batch entry than the merge holds.
+// candidates for a batch entry than a merging workgroup holds in registers.
 BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
   BeamPlan r{};
-  r.rows = batch * beams;
+  const int64_t rows = batch * beams;
   const int64_t chunk = 64 * (16 / elem_bytes), chunks = (vocab + chunk - 1) / chunk;
-  int64_t s = std::max<int64_t>(1, kTargetWaves / std::max<int64_t>(r.rows, 1));
+  int64_t s = std::max<int64_t>(1, kTargetWaves / std::max<int64_t>(rows, 1));
   s = std::min<int64_t>(s, std::max<int64_t>(1, chunks / 2));
   s = std::min<int64_t>(s, std::max(1, kMaxCandidates / (beams * n)));
   r.slice_chunks = (int)((chunks + s - 1) / s);
   r.slices = (int)((chunks + r.slice_chunks - 1) / r.slice_chunks);
-  r.waves = r.rows * r.slices;
-  r.best = 0;
+  r.groups = (beams * r.slices + kScanWaves - 1) / kScanWaves;
+  r.waves = rows * r.slices;
+  r.ended = 0;
+  r.best = align_up(r.ended + 4 * (size_t)batch, 256);
   r.sum = align_up(r.best + sizeof(Candidate) * (size_t)r.waves * n, 256);
   r.ref = align_up(r.sum + sizeof(double) * (size_t)r.waves, 256);
   r.far = align_up(r.ref + sizeof(float) * (size_t)r.waves, 256);
@@ -373,7 +451,7 @@ BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
 }
 
 bool beam_sizes(int64_t batch, int beams, int vocab, int n, int dtype) {
-  return batch >= 0 && batch <= (1 << 22) && beams >= 1 && beams <= kMaxBeams && n >= 1 && n <= kMaxBest && vocab >= 1 &&
+  return batch >= 0 && batch <= (1 << 20) && beams >= 1 && beams <= kMaxBeams && n >= 1 && n <= kMaxBest && vocab >= 1 &&
          vocab <= 1 << 30 && n <= (int64_t)beams * vocab && (dtype == IA_F32 || dtype == IA_BF16);
 }
 
@@ -407,31 +485,33 @@ int ia_beam_select(const void* logits, int32_t logits_dtype, int64_t row_stride,
   if (!workspace || workspace_bytes < plan.total || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(IA_ERR_WORKSPACE, "workspace missing, too small or not 256-byte aligned");
   char* ws = static_cast<char*>(workspace);
-  ScanParams s{};
-  s.logits = static_cast<const char*>(logits);
-  s.row_stride = row_stride * eb;
-  s.done = done;
-  s.vocab = vocab;
-  s.n = n;
-  s.slices = plan.slices;
-  s.slice_chunks = plan.slice_chunks;
-  s.waves = plan.waves;
-  s.best = reinterpret_cast<Candidate*>(ws + plan.best);
-  s.sum = reinterpret_cast<double*>(ws + plan.sum);
-  s.ref = reinterpret_cast<float*>(ws + plan.ref);
+  BeamParams p{};
+  p.logits = static_cast<const char*>(logits);
+  p.row_stride = row_stride * eb;
+  p.scores = scores;
+  p.done = done;
+  p.beams = beams;
+  p.vocab = vocab;
+  p.n = n;
+  p.slices = plan.slices;
+  p.slice_chunks = plan.slice_chunks;
+  p.pad_token = pad_token;
+  p.groups = plan.groups;
+  p.best = reinterpret_cast<Candidate*>(ws + plan.best);
+  p.sum = reinterpret_cast<unsigned long long*>(ws + plan.sum);
+  p.ref = reinterpret_cast<float*>(ws + plan.ref);
+  p.ended = reinterpret_cast<u32*>(ws + plan.ended);
+  p.far = reinterpret_cast<unsigned long long*>(ws + plan.far);
+  p.out_scores = out_scores;
+  p.out_tokens = out_tokens;
+  p.out_rows = out_rows;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)((plan.waves + kScanWaves - 1) / kScanWaves));
+  const dim3 grid((unsigned)(batch * plan.groups));
   if (logits_dtype == IA_F32)
-    hipLaunchKernelGGL(ia_beam_scan<float>, grid, dim3(kScanThreads), 0, st, s);
+    hipLaunchKernelGGL(ia_beam_scan<float>, grid, dim3(kScanThreads), 0, st, p);
   else
-    hipLaunchKernelGGL(ia_beam_scan<bf16_t>, grid, dim3(kScanThreads), 0, st, s);
-  const int rc = check_launch("beam scan");
-  if (rc) return rc;
-  const MergeParams m{scores, done,        s.best,    s.sum,      s.ref,      reinterpret_cast<unsigned long long*>(ws + plan.far),
-                      beams,  vocab,       n,         plan.slices, pad_token, out_scores,
-                      out_tokens, out_rows};
-  hipLaunchKernelGGL(ia_beam_merge, dim3(batch), dim3(kMergeThreads), 0, st, m);
-  return check_launch("beam merge");
+    hipLaunchKernelGGL(ia_beam_scan<bf16_t>, grid, dim3(kScanThreads), 0, st, p);
+  return check_launch("beam select");
 }
 
 }  // extern "C"

@@ -4,7 +4,9 @@ Bar of a score: exp in float32 is off by 2^-22 relative at most (its argument's 
 2^-24 |x - M| log2 e for the terms that count, and the instruction's last place), so the log of a
 sum by 2^-21; a returned score is rounded once more, 2^-24 of itself.  Tokens are equal unless two
 keys are closer than that bar, which no listed case is by chance: equal keys are made so on
-purpose, and go to the lower place."""
+purpose, and go to the lower place.  That holds inside a row and between rows that hold the same
+values in the same order (up to a constant); two rows of the same values in another order have
+logs of sums that are each off by up to 2^-21, so which of them comes first is not theirs to say."""
 
 import math
 
@@ -38,7 +40,12 @@ def check(got, logits, scores, n, done=None, pad=0):
     # a place differs only where the keys do not tell (never equal ones)
     mine = np.take_along_axis(keys, at, 1)
     differ = at != place
-    assert not (differ & (mine == want)).any(), "equal keys go to the lower place"
+    x = logits.double().cpu().numpy().reshape(batch, beams, vocab)
+    with np.errstate(invalid="ignore"):
+        x = x - x.max(-1, keepdims=True)
+    for b, i in np.argwhere(differ & (mine == want)):
+        j, k = at[b, i] // vocab, place[b, i] // vocab
+        assert not np.array_equal(x[b, j], x[b, k], equal_nan=True), "equal keys go to the lower place"
     assert (np.abs(mine[differ] - want[differ]) <= 2.0 ** -20).all()
     assert all(len(set(r)) == n for r in at)
 
