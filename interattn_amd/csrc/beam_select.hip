@@ -25,6 +25,8 @@ constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kFly = 4;              // chunks of a group, and in flight
 constexpr int kHeld = 640;           // candidates a wave holds: a chunk's 512 and some
 constexpr int kTrim = 128;           // candidates at which they are cut to the n best
+constexpr int kWorthFloor = 8;       // lanes with something better for which the floor is raised
+constexpr int kMaxSlices = 64;       // of a row: a lane each in the merge
 constexpr int kMaxBeams = 64, kMaxBest = 64;
 constexpr int kOwn = 8;              // candidates a merging thread keeps in registers
 constexpr int kMaxCandidates = kOwn * kScanThreads;  // of a batch entry, where a slice a row is fewer
@@ -47,11 +49,13 @@ __device__ __forceinline__ double order_value64(unsigned long long k) {
   return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k));
 }
 
-// The n-th largest of the lanes' keys (n <= 64): the largest K that n keys reach.
+// The n-th largest of the lanes' keys (n <= 64), its lower bits cut off: the largest K of BITS
+// leading bits that n keys reach.
+template <int BITS>
 __device__ __forceinline__ u32 nth_of_lanes(u32 key, int n) {
   u32 k = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit > 31 - BITS; --bit) {
     const u32 t = k | 1u << bit;
     if (__popcll(__ballot(key >= t)) >= n) k = t;
   }
@@ -150,18 +154,16 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
   double sum = 0.;
   int cnt = 0;
 
-  auto load = [&](int c) {
+  // a chunk past the slice or the row's end: what is there, -infinity for the rest
+  auto load_some = [&](int c) {
     const int at = c * kChunk + lane * kVec;
-    u32x4_t w;
-    if (c < c1 && at + kVec <= p.vocab) {
-      w = __builtin_nontemporal_load(&reinterpret_cast<const Loose<T>*>(x0 + at)->w);
-    } else {
-      float y[kVec];
+    float y[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = c < c1 && at + j < p.vocab ? to_f32(x0[at + j]) : kNegInf;
-      w = narrow(y, T{});
-    }
-    return w;
+    for (int j = 0; j < kVec; ++j) y[j] = c < c1 && at + j < p.vocab ? to_f32(x0[at + j]) : kNegInf;
+    return narrow(y, T{});
+  };
+  auto load = [&](int c) {
+    return __builtin_nontemporal_load(&reinterpret_cast<const Loose<T>*>(x0 + (c * kChunk + lane * kVec))->w);
   };
   auto take = [&](const u32x4_t* w, int c) {
     float most[kFly], all = kNegInf;
@@ -201,10 +203,15 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
       }
     }
     sum += (double)part;
-    if (!__ballot(all >= lo)) return;
+    const unsigned long long hits = __ballot(all >= lo);
+    if (!hits) return;
     seen = fmaxf(seen, all);
-    u32 floor_ = nth_of_lanes(order_key(seen + 0.f), n);  // n values of n lanes reach it
-    lo = fmaxf(lo, order_value(floor_));
+    // n values of n lanes reach the floor; a few better values are not worth a new one
+    u32 floor_ = 0;
+    if (__popcll(hits) >= kWorthFloor) {
+      floor_ = nth_of_lanes<16>(order_key(seen + 0.f), n);
+      lo = fmaxf(lo, order_value(floor_));
+    }
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
       if (!__ballot(most[i] >= lo)) continue;
@@ -231,15 +238,26 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
     if (floor_ > order_key(-3.402823466e38f)) lo = fmaxf(lo, above(floor_));
   };
 
+  // whole groups, one ahead (the last is loaded twice: a load under a condition would make every
+  // group wait for the one behind it), then what is left
+  const int whole = max(min(c1, p.vocab / kChunk) - c0, 0) / kFly;
   u32x4_t cur[kFly], nxt[kFly];
+  if (whole > 0) {
 #pragma unroll
-  for (int i = 0; i < kFly; ++i) cur[i] = load(c0 + i);
-  for (int c = c0; c < c1; c += kFly) {
+    for (int i = 0; i < kFly; ++i) cur[i] = load(c0 + i);
+    for (int g = 0; g < whole; ++g) {
+      const int next = c0 + min(g + 1, whole - 1) * kFly;
 #pragma unroll
-    for (int i = 0; i < kFly; ++i) nxt[i] = load(c + kFly + i);
-    take(cur, c);
+      for (int i = 0; i < kFly; ++i) nxt[i] = load(next + i);
+      take(cur, c0 + g * kFly);
 #pragma unroll
-    for (int i = 0; i < kFly; ++i) cur[i] = nxt[i];
+      for (int i = 0; i < kFly; ++i) cur[i] = nxt[i];
+    }
+  }
+  if (c0 + whole * kFly < c1) {
+#pragma unroll
+    for (int i = 0; i < kFly; ++i) cur[i] = load_some(c0 + whole * kFly + i);
+    take(cur, c0 + whole * kFly);
   }
   wave_lds_sync();
   if (cnt > n) {
@@ -275,25 +293,31 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
 #pragma unroll
   for (int i = 0; i < kOwn; ++i)
     own[i] = i * kScanThreads + tid < total ? ld_agent_u64(p.best + row0 * per_beam + i * kScanThreads + tid) : kNoCandidate;
-  // each beam's reference and log of its sum; +infinity where the beam has nothing to offer
-  for (int j = wave; j < p.beams; j += kScanWaves) {
-    const int64_t at = (row0 + j) * p.slices;
-    const bool ended = p.done && p.done[row0 + j];
-    float m = kNegInf;
-    if (!ended)
-      for (int s = lane; s < p.slices; s += 64) m = fmaxf(m, ld_agent(p.ref + at + s));
-    m = wave_max(m);
-    double t = 0.;
-    if (!ended && m != kNegInf)
-      for (int s = lane; s < p.slices; s += 64) {
-        const float r = ld_agent(p.ref + at + s);
-        // (a reference of -infinity: nothing was added)
-        if (r != kNegInf) t += __longlong_as_double((long long)ld_agent_u64(p.sum + at + s)) * exp((double)r - (double)m);
+  // each beam's reference and log of its sum; +infinity where the beam has nothing to offer.
+  // The slices of four beams are in flight together.
+  for (int j0 = wave; j0 < p.beams; j0 += 4 * kScanWaves) {
+    float r[4];
+    double t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * kScanWaves;
+      const int64_t at = (row0 + j) * p.slices + lane;
+      const bool there = j < p.beams && lane < p.slices && !(p.done && p.done[row0 + j]);
+      r[i] = there ? ld_agent(p.ref + at) : kNegInf;
+      t[i] = there ? __longlong_as_double((long long)ld_agent_u64(p.sum + at)) : 0.;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * kScanWaves;
+      if (j >= p.beams) break;
+      const float m = wave_max(r[i]);
+      // (a reference of -infinity: nothing was added)
+      double x = r[i] == kNegInf ? 0. : t[i] * exp((double)r[i] - (double)m);
+      for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s, 64);
+      if (lane == 0) {
+        l.top[j] = m;
+        l.log_sum[j] = x > 0. ? log(x) : (double)__builtin_huge_valf();
       }
-    for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s, 64);
-    if (lane == 0) {
-      l.top[j] = m;
-      l.log_sum[j] = t > 0. ? log(t) : (double)__builtin_huge_valf();
     }
   }
   if (tid == 0) l.stay = 0;
@@ -328,7 +352,7 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
     unsigned long long place;
     mine = max(mine, (u32)(key_place(i, ld_agent_u64(p.best + row0 * per_beam + i), &place) >> 32));
   }
-  const u32 least = nth_of_lanes(mine, p.n);
+  const u32 least = nth_of_lanes<24>(mine, p.n);
   if (lane == 0) l.least[wave] = least;
   __syncthreads();
   u32 limit = 0;
@@ -428,16 +452,16 @@ struct BeamPlan {
   size_t ended, best, sum, ref, far, total;  // offsets in the workspace
 };
 
-// Slices of a row: about kTargetWaves waves in all, two chunks each at least, and no more
+// Slices of a row: about kTargetWaves waves in all, a group each at least, and no more
 // candidates for a batch entry than a merging workgroup holds in registers.
 BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
   BeamPlan r{};
   const int64_t rows = batch * beams;
   const int64_t chunk = 64 * (16 / elem_bytes), chunks = (vocab + chunk - 1) / chunk;
   int64_t s = std::max<int64_t>(1, kTargetWaves / std::max<int64_t>(rows, 1));
-  s = std::min<int64_t>(s, std::max<int64_t>(1, chunks / 2));
-  s = std::min<int64_t>(s, std::max(1, kMaxCandidates / (beams * n)));
-  r.slice_chunks = (int)((chunks + s - 1) / s);
+  s = std::min<int64_t>(s, (chunks + kFly - 1) / kFly);
+  s = std::min<int64_t>(s, std::max(1, std::min(kMaxSlices, kMaxCandidates / (beams * n))));
+  r.slice_chunks = (int)align_up((chunks + s - 1) / s, kFly);
   r.slices = (int)((chunks + r.slice_chunks - 1) / r.slice_chunks);
   r.groups = (beams * r.slices + kScanWaves - 1) / kScanWaves;
   r.waves = rows * r.slices;
