@@ -65,53 +65,65 @@ __device__ __forceinline__ u32 nth_of_lanes(u32 key, int n) {
 // The least float above the one of key k.
 __device__ __forceinline__ float above(u32 k) { return order_value(k + 1); }
 
-// A candidate: order_key of the logit (-0 as +0) above the token.
+// A candidate: order_key of the logit (-0 as +0) above the token's complement, so that the
+// better of two is the larger number.  0: none.
 typedef unsigned long long Candidate;
 __device__ __forceinline__ u32 key_of(Candidate c) { return (u32)(c >> 32); }
-__device__ __forceinline__ u32 token_of(Candidate c) { return (u32)c; }
-constexpr Candidate kNoCandidate = 0xffffffffull;
+__device__ __forceinline__ u32 token_of(Candidate c) { return ~(u32)c; }
+__device__ __forceinline__ Candidate candidate(float x, u32 token) { return (Candidate)order_key(x + 0.f) << 32 | ~token; }
 
-// The n best of cnt candidates (key descending, token ascending) to the front of `held`, in
-// any order; returns their least key.  cnt > n, one wave.
+// c of another lane (the same for all)
+__device__ __forceinline__ Candidate of_lane(Candidate c, int lane) {
+  return (Candidate)(u32)__builtin_amdgcn_readlane((int)(c >> 32), lane) << 32 |
+         (u32)__builtin_amdgcn_readlane((int)(u32)c, lane);
+}
+
+// The n best of cnt candidates to the front of `held`; returns the least key that stays.
+// n < cnt <= kHeld, one wave.
 __device__ u32 trim(Candidate* held, int cnt, int n, int lane) {
-  constexpr int kHere = 3;  // registers' worth; more only where very many are equal
-  Candidate mine[kHere];
-#pragma unroll
-  for (int i = 0; i < kHere; ++i) mine[i] = 64 * i + lane < cnt ? held[64 * i + lane] : 0ull;
-  auto reach = [&](auto&& test) {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < kHere; ++i) c += __popcll(__ballot(64 * i + lane < cnt && test(mine[i])));
-    for (int i = 64 * kHere; i < cnt; i += 64)
-      c += __popcll(__ballot(i + lane < cnt && test(held[min(i + lane, cnt - 1)])));
-    return c;
-  };
-  u32 least = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const u32 t = least | 1u << bit;
-    if (reach([&](Candidate c) { return key_of(c) >= t; }) >= n) least = t;
-  }
-  u32 last = 0xffffffffu;  // of those that have the least key, tokens up to `last` stay
-  const int better = reach([&](Candidate c) { return key_of(c) > least; });
-  if (reach([&](Candidate c) { return key_of(c) == least; }) > n - better) {
-    u32 below = 0;  // the largest bound below which fewer than n - better tokens lie
-    for (int bit = 31; bit >= 0; --bit) {
-      const u32 t = below | 1u << bit;
-      if (reach([&](Candidate c) { return key_of(c) == least && token_of(c) < t; }) < n - better) below = t;
+  wave_lds_sync();
+  Candidate edge;  // the least that stays
+  Candidate a = lane < cnt ? held[lane] : 0ull, b = 64 + lane < cnt ? held[64 + lane] : 0ull;
+  if (cnt <= 128) {  // ranks, by counting what is better (bit by bit as below: 4 us, 32 dependent steps)
+    int ra = 0, rb = 0;
+    const int first = min(cnt, 64);
+#pragma unroll 8
+    for (int o = 0; o < first; ++o) {
+      const Candidate x = of_lane(a, o);
+      ra += x > a;
+      rb += x > b;
     }
-    last = below;
-  }
-  int kept = 0;
-  for (int i = 0; i < cnt; i += 64) {
-    const Candidate c = held[min(i + lane, cnt - 1)];
-    const bool keep = i + lane < cnt && (key_of(c) > least || (key_of(c) == least && token_of(c) <= last));
-    const unsigned long long m = __ballot(keep);
-    wave_lds_sync();  // (read before it is written: entries move towards the front)
-    if (keep) held[kept + __popcll(m & ((1ull << lane) - 1))] = c;
-    kept += __popcll(m);
+#pragma unroll 8
+    for (int o = 0; o < cnt - 64; ++o) {
+      const Candidate x = of_lane(b, o);
+      ra += x > a;
+      rb += x > b;
+    }
     wave_lds_sync();
+    if (lane < cnt && ra < n) held[ra] = a;
+    if (64 + lane < cnt && rb < n) held[rb] = b;
+    wave_lds_sync();
+    edge = held[n - 1];
+  } else {  // (many equal ones) the n-th largest number bit by bit: key, then token
+    edge = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const Candidate t = edge | 1ull << bit;
+      int c = 0;
+      for (int i = 0; i < cnt; i += 64) c += __popcll(__ballot(i + lane < cnt && held[min(i + lane, cnt - 1)] >= t));
+      if (c >= n) edge = t;
+    }
+    int kept = 0;
+    for (int i = 0; i < cnt; i += 64) {
+      const Candidate c = held[min(i + lane, cnt - 1)];
+      const bool keep = i + lane < cnt && c >= edge;
+      const unsigned long long m = __ballot(keep);
+      wave_lds_sync();  // (read before it is written: entries move towards the front)
+      if (keep) held[kept + __popcll(m & ((1ull << lane) - 1))] = c;
+      kept += __popcll(m);
+      wave_lds_sync();
+    }
   }
-  return least;
+  return key_of(edge);
 }
 
 struct BeamParams {
@@ -224,12 +236,11 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
         if (m) {
           if (in)
             held[cnt + __popcll(m & ((1ull << lane) - 1))] =
-                (Candidate)order_key(x[j] + 0.f) << 32 | (u32)((c + i) * kChunk + lane * kVec + j);
+                candidate(x[j], (u32)((c + i) * kChunk + lane * kVec + j));
           cnt += __popcll(m);
         }
       }
       if (cnt >= kTrim) {
-        wave_lds_sync();
         lo = fmaxf(lo, above(trim(held, cnt, n, lane)));
         cnt = n;
       }
@@ -263,10 +274,9 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
   if (cnt > n) {
     trim(held, cnt, n, lane);
     cnt = n;
-    wave_lds_sync();
   }
   for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
-  if (lane < n) st_agent_u64(p.best + id * n + lane, lane < cnt ? held[lane] : kNoCandidate);
+  if (lane < n) st_agent_u64(p.best + id * n + lane, lane < cnt ? held[lane] : 0ull);
   if (lane == 0) {
     st_agent_u64(p.sum + id, (unsigned long long)__double_as_longlong(sum));
     st_agent(p.ref + id, ref);
@@ -292,7 +302,7 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
   Candidate own[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i)
-    own[i] = i * kScanThreads + tid < total ? ld_agent_u64(p.best + row0 * per_beam + i * kScanThreads + tid) : kNoCandidate;
+    own[i] = i * kScanThreads + tid < total ? ld_agent_u64(p.best + row0 * per_beam + i * kScanThreads + tid) : 0ull;
   // each beam's reference and log of its sum; +infinity where the beam has nothing to offer.
   // The slices of four beams are in flight together.
   for (int j0 = wave; j0 < p.beams; j0 += 4 * kScanWaves) {
@@ -331,7 +341,7 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
     if (p.done && p.done[row0 + j]) {
       at = (u32)p.pad_token;
       if (i == j * per_beam) key = (double)p.scores[row0 + j];
-    } else if (c != kNoCandidate) {
+    } else if (c != 0) {
       // (x - top is exact: rows that differ by a constant have the same keys)
       key = (double)p.scores[row0 + j] + (((double)order_value(key_of(c)) - (double)l.top[j]) - l.log_sum[j]);
     }
