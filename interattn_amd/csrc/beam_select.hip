@@ -31,7 +31,7 @@ constexpr int kMaxBeams = 64, kMaxBest = 64;
 constexpr int kOwn = 8;              // candidates a merging thread keeps in registers
 constexpr int kMaxCandidates = kOwn * kScanThreads;  // of a batch entry, where a slice a row is fewer
 constexpr int kNear = 1024;          // of those above the threshold, in LDS; more go through memory
-constexpr int kTargetWaves = 4096;
+constexpr int kWaves = 2048;         // of a call, where slices are long
 
 // Floats as integers of the same order (-0 before +0).
 __device__ __forceinline__ u32 order_key(float x) {
@@ -86,18 +86,22 @@ __device__ u32 trim(Candidate* held, int cnt, int n, int lane) {
   Candidate a = lane < cnt ? held[lane] : 0ull, b = 64 + lane < cnt ? held[64 + lane] : 0ull;
   if (cnt <= 128) {  // ranks, by counting what is better (bit by bit as below: 4 us, 32 dependent steps)
     int ra = 0, rb = 0;
-    const int first = min(cnt, 64);
-#pragma unroll 8
-    for (int o = 0; o < first; ++o) {
-      const Candidate x = of_lane(a, o);
-      ra += x > a;
-      rb += x > b;
-    }
-#pragma unroll 8
-    for (int o = 0; o < cnt - 64; ++o) {
-      const Candidate x = of_lane(b, o);
-      ra += x > a;
-      rb += x > b;
+    if (cnt <= 64) {
+#pragma unroll 4
+      for (int o = 0; o < cnt; ++o) ra += of_lane(a, o) > a;
+    } else {
+#pragma unroll 4
+      for (int o = 0; o < 64; ++o) {
+        const Candidate x = of_lane(a, o);
+        ra += x > a;
+        rb += x > b;
+      }
+#pragma unroll 4
+      for (int o = 0; o < cnt - 64; ++o) {
+        const Candidate x = of_lane(b, o);
+        ra += x > a;
+        rb += x > b;
+      }
     }
     wave_lds_sync();
     if (lane < cnt && ra < n) held[ra] = a;
@@ -133,6 +137,7 @@ struct BeamParams {
   const uint8_t* done;  // null: none
   int32_t beams, vocab, n, slices, slice_chunks, pad_token;
   int32_t groups;  // workgroups of a batch entry
+  unsigned long long per_beam_inverse;  // of slices * n, 2^32 times, rounded up
   // per slice of a row: n candidates, the reference and the sum; per entry: workgroups that have
   // ended (0 between calls), candidates' keys and places where kNear is too few
   Candidate* best;
@@ -171,7 +176,10 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
     const int at = c * kChunk + lane * kVec;
     float y[kVec];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) y[j] = c < c1 && at + j < p.vocab ? to_f32(x0[at + j]) : kNegInf;
+    for (int j = 0; j < kVec; ++j) {
+      const float x = to_f32(x0[min(at + j, p.vocab - 1)]);  // (loaded by every lane: no branch a value)
+      y[j] = c < c1 && at + j < p.vocab ? x : kNegInf;
+    }
     return narrow(y, T{});
   };
   auto load = [&](int c) {
@@ -275,8 +283,8 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
     trim(held, cnt, n, lane);
     cnt = n;
   }
-  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
   if (lane < n) st_agent_u64(p.best + id * n + lane, lane < cnt ? held[lane] : 0ull);
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
   if (lane == 0) {
     st_agent_u64(p.sum + id, (unsigned long long)__double_as_longlong(sum));
     st_agent(p.ref + id, ref);
@@ -286,9 +294,9 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
 struct MergeLds {
   unsigned long long keys[kNear], places[kNear];  // of those that stay
   double log_sum[kMaxBeams];
-  float top[kMaxBeams];
-  u32 least[kScanWaves];
-  int rank[kNear];
+  float top[kMaxBeams], score[kMaxBeams];
+  int ended[kMaxBeams];
+  u32 least[2][kScanWaves];
   int stay;
 };
 
@@ -312,7 +320,12 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + i * kScanWaves;
       const int64_t at = (row0 + j) * p.slices + lane;
-      const bool there = j < p.beams && lane < p.slices && !(p.done && p.done[row0 + j]);
+      const bool ended = j < p.beams && p.done && p.done[row0 + j];
+      const bool there = j < p.beams && lane < p.slices && !ended;
+      if (j < p.beams && lane == 0) {
+        l.score[j] = p.scores[row0 + j];
+        l.ended[j] = ended;
+      }
       r[i] = there ? ld_agent(p.ref + at) : kNegInf;
       t[i] = there ? __longlong_as_double((long long)ld_agent_u64(p.sum + at)) : 0.;
     }
@@ -335,21 +348,22 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
   const unsigned long long none = order_key64((double)kNegInf);
   // key of candidate i (0: cannot be chosen) and its place
   auto key_place = [&](int i, Candidate c, unsigned long long* place) {
-    const int j = i / per_beam;
+    const int j = (int)((u32)i * p.per_beam_inverse >> 32);
     double key = (double)kNegInf;
     u32 at = token_of(c);
-    if (p.done && p.done[row0 + j]) {
+    if (l.ended[j]) {
       at = (u32)p.pad_token;
-      if (i == j * per_beam) key = (double)p.scores[row0 + j];
+      if (i == j * per_beam) key = (double)l.score[j];
     } else if (c != 0) {
       // (x - top is exact: rows that differ by a constant have the same keys)
-      key = (double)p.scores[row0 + j] + (((double)order_value(key_of(c)) - (double)l.top[j]) - l.log_sum[j]);
+      key = (double)l.score[j] + (((double)order_value(key_of(c)) - (double)l.top[j]) - l.log_sum[j]);
     }
     *place = (unsigned long long)j << 32 | at;
     const unsigned long long k = key == key ? order_key64(key + 0.) : none;
     return k <= none ? 0ull : k;
   };
-  // a threshold on the keys' upper halves that n candidates of some wave reach
+  // a threshold on the keys' upper halves that n candidates reach: n of some wave, or each wave's
+  // share of n
   unsigned long long own_key[kOwn], own_place[kOwn];
   u32 mine = 0;
 #pragma unroll
@@ -362,22 +376,29 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
     unsigned long long place;
     mine = max(mine, (u32)(key_place(i, ld_agent_u64(p.best + row0 * per_beam + i), &place) >> 32));
   }
-  const u32 least = nth_of_lanes<24>(mine, p.n);
-  if (lane == 0) l.least[wave] = least;
+  const u32 least = nth_of_lanes<24>(mine, p.n), share = nth_of_lanes<24>(mine, (p.n + kScanWaves - 1) / kScanWaves);
+  if (lane == 0) {
+    l.least[0][wave] = least;
+    l.least[1][wave] = share;
+  }
   __syncthreads();
-  u32 limit = 0;
+  u32 limit = 0, shares = 0xffffffffu;
 #pragma unroll
-  for (int w = 0; w < kScanWaves; ++w) limit = max(limit, l.least[w]);
+  for (int w = 0; w < kScanWaves; ++w) {
+    limit = max(limit, l.least[0][w]);
+    shares = min(shares, l.least[1][w]);
+  }
+  limit = max(limit, shares);
   auto keep = [&](unsigned long long k, unsigned long long place) {
     if (k == 0 || (u32)(k >> 32) < limit) return;
     const int at = atomicAdd(&l.stay, 1);
     if (at < kNear) {
       l.keys[at] = k;
       l.places[at] = place;
-      l.rank[at] = 0;
+    } else {
+      far_keys[at] = k;
+      far_places[at] = place;
     }
-    far_keys[at] = k;
-    far_places[at] = place;
   };
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) keep(own_key[i], own_place[i]);
@@ -396,23 +417,28 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
     p.out_tokens[to] = (int32_t)(u32)place;
     p.out_rows[to] = (int)(row0 + (int64_t)(place >> 32));
   };
-  if (count <= kNear) {
-    // a wave counts for every candidate against a quarter of them
-    for (int i = lane; i < count; i += 64) {
-      const unsigned long long k = l.keys[i], at = l.places[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int o = wave; o < count; o += kScanWaves) rank += l.keys[o] > k || (l.keys[o] == k && l.places[o] < at);
-      atomicAdd(&l.rank[i], rank);
+  if (count <= 128) {  // a candidate a lane, the others read across the wave
+    const int i = tid;
+    const unsigned long long k = i < count ? l.keys[i] : 0ull, at = i < count ? l.places[i] : 0ull;
+    int rank = 0;
+    for (int o0 = 0; o0 < count && wave * 64 < count; o0 += 64) {
+      const unsigned long long ok = o0 + lane < count ? l.keys[o0 + lane] : 0ull;
+      const unsigned long long oa = o0 + lane < count ? l.places[o0 + lane] : 0ull;
+      const int many = min(count - o0, 64);
+#pragma unroll 8
+      for (int o = 0; o < many; ++o) {
+        const unsigned long long x = of_lane(ok, o), y = of_lane(oa, o);
+        rank += x > k || (x == k && y < at);
+      }
     }
-    __syncthreads();
-    for (int i = tid; i < count; i += kScanThreads)
-      if (l.rank[i] < p.n) put(l.rank[i], order_value64(l.keys[i]), l.places[i]);
+    if (i < count && rank < p.n) put(rank, order_value64(k), at);
   } else {
+    auto key_at = [&](int o) { return o < kNear ? l.keys[o] : far_keys[o]; };
+    auto place_at = [&](int o) { return o < kNear ? l.places[o] : far_places[o]; };
     for (int i = tid; i < count; i += kScanThreads) {
-      const unsigned long long k = far_keys[i], at = far_places[i];
+      const unsigned long long k = key_at(i), at = place_at(i);
       int rank = 0;
-      for (int o = 0; o < count; ++o) rank += far_keys[o] > k || (far_keys[o] == k && far_places[o] < at);
+      for (int o = 0; o < count; ++o) rank += key_at(o) > k || (key_at(o) == k && place_at(o) < at);
       if (rank < p.n) put(rank, order_value64(k), at);
     }
   }
@@ -462,14 +488,19 @@ struct BeamPlan {
   size_t ended, best, sum, ref, far, total;  // offsets in the workspace
 };
 
-// Slices of a row: about kTargetWaves waves in all, a group each at least, and no more
-// candidates for a batch entry than a merging workgroup holds in registers.
+// Slices of a row: up to kWaves waves in all with two groups a slice, up to half as many with
+// one, and no more candidates for a batch entry than a merging workgroup holds in registers.  A
+// wave's first group and its last cut of the candidates cost about 4 us, so that more waves are
+// not faster: 512 rows of 128,000 take 42 us in 2,048 waves, 43 in 4,096, 67 in 8,192 and 68 in
+// 1,024, where too few loads are in flight; 512 of 16,384 19 in 2,048 and 23 in 4,096; 80 of
+// 50,021 14.8 with two groups a slice and 16.7 with one.
 BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
   BeamPlan r{};
   const int64_t rows = batch * beams;
   const int64_t chunk = 64 * (16 / elem_bytes), chunks = (vocab + chunk - 1) / chunk;
-  int64_t s = std::max<int64_t>(1, kTargetWaves / std::max<int64_t>(rows, 1));
-  s = std::min<int64_t>(s, (chunks + kFly - 1) / kFly);
+  const int64_t per_row = kWaves / std::max<int64_t>(rows, 1);
+  int64_t s = std::max(std::min(per_row, chunks / (2 * kFly)), std::min(per_row / 2, (chunks + kFly - 1) / kFly));
+  s = std::max<int64_t>(s, 1);
   s = std::min<int64_t>(s, std::max(1, std::min(kMaxSlices, kMaxCandidates / (beams * n))));
   r.slice_chunks = (int)align_up((chunks + s - 1) / s, kFly);
   r.slices = (int)((chunks + r.slice_chunks - 1) / r.slice_chunks);
@@ -531,6 +562,7 @@ int ia_beam_select(const void* logits, int32_t logits_dtype, int64_t row_stride,
   p.slice_chunks = plan.slice_chunks;
   p.pad_token = pad_token;
   p.groups = plan.groups;
+  p.per_beam_inverse = ((1ull << 32) + plan.slices * n - 1) / (plan.slices * n);
   p.best = reinterpret_cast<Candidate*>(ws + plan.best);
   p.sum = reinterpret_cast<unsigned long long*>(ws + plan.sum);
   p.ref = reinterpret_cast<float*>(ws + plan.ref);
