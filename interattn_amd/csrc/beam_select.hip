@@ -159,7 +159,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // 16 bytes at any e
 template <typename T>
 __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held, int64_t row, int slice, int64_t id,
                                            int lane) {
-  constexpr int kVec = RowVec<T, kRowsPlain>::kVec, kChunk = 64 * kVec;
+  constexpr int kVec = RowVec<T>::kVec, kChunk = 64 * kVec;
   const T* x0 = reinterpret_cast<const T*>(p.logits + row * p.row_stride);
   const int chunks = (p.vocab + kChunk - 1) / kChunk;
   const int c0 = slice * p.slice_chunks, c1 = min(c0 + p.slice_chunks, chunks);

@@ -43,7 +43,7 @@ struct ReadChunk;
 
 template <typename T>
 struct ReadChunk<T, T> {
-  static constexpr int kElems = RowVec<T, kRowsPlain>::kVec;
+  static constexpr int kElems = RowVec<T>::kVec;
   static __device__ __forceinline__ void put(T* to, const u32x4_t& w, float) { *reinterpret_cast<u32x4_t*>(to) = w; }
 };
 template <>
@@ -77,7 +77,7 @@ struct ReadChunk<fp8_t, OutT> {
     for (int i = 0; i < 4; ++i) fp8x4_to_f32(w[i], x + 4 * i);
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] *= s;
-    constexpr int kVec = RowVec<OutT, kRowsPlain>::kVec;
+    constexpr int kVec = RowVec<OutT>::kVec;
 #pragma unroll
     for (int j = 0; j < 16; j += kVec) *reinterpret_cast<u32x4_t*>(to + j) = narrow(x + j, OutT{});
   }

@@ -36,7 +36,7 @@ struct RotParams {
   int heads[2];
   const int32_t* pos;
   RotaryArgs rot;
-  int n_tokens, units, tile, heads_per_wg;
+  int n_tokens, head_dim, units, tile, heads_per_wg;
 };
 
 template <typename T, int LAYOUT>
@@ -46,8 +46,8 @@ __global__ __launch_bounds__(kRotThreads) void ia_rotary_turn(RotParams p) {
   const int64_t tok = (int64_t)blockIdx.x * p.tile + local;
   if (local >= p.tile || tok >= p.n_tokens) return;
   float cs[kVec], sn[kVec];
-  const int turns = unit_turns<kVec>(p.rot.rot, u);
-  unit_angles<kVec>(p.rot, p.pos[tok], u, turns, cs, sn);
+  const typename RowUnit<T, LAYOUT>::Turns turns(u, p.rot.rot, p.head_dim);
+  unit_angles<LAYOUT, kVec>(p.rot, p.pos[tok], turns, cs, sn);
   const int all = p.heads[0] + p.heads[1];
   const int h0 = blockIdx.y * p.heads_per_wg, h1 = min(h0 + p.heads_per_wg, all);
 #pragma unroll
@@ -61,13 +61,13 @@ __global__ __launch_bounds__(kRotThreads) void ia_rotary_turn(RotParams p) {
       RowUnit<T, LAYOUT> x[kRotFly];
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
-        if (h + i < b) x[i].load(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot);
+        if (h + i < b) x[i].load(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot, p.head_dim);
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
         if (h + i < b) {
           float y[2 * kVec];
           x[i].turned(cs, sn, turns, y);
-          store_unit<T, LAYOUT>(reinterpret_cast<T*>(out + (h + i) * t.out_head), u, p.rot.rot, y);
+          store_unit<T, LAYOUT>(reinterpret_cast<T*>(out + (h + i) * t.out_head), u, p.rot.rot, p.head_dim, y);
         }
     }
   }
@@ -79,10 +79,8 @@ void launch_rotary(int layout, dim3 grid, hipStream_t st, const RotParams& p) {
     hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalf>), grid, dim3(kRotThreads), 0, st, p);
   else if (layout == kRowsInterleaved)
     hipLaunchKernelGGL((ia_rotary_turn<T, kRowsInterleaved>), grid, dim3(kRotThreads), 0, st, p);
-  else if (layout == kRowsHalfOdd)
-    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalfOdd>), grid, dim3(kRotThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsPlain>), grid, dim3(kRotThreads), 0, st, p);
+    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalfOdd>), grid, dim3(kRotThreads), 0, st, p);
 }
 
 }  // namespace
@@ -123,6 +121,7 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
   p.rot = RotaryArgs{reinterpret_cast<const unsigned long long*>(rotary->turns), rotary->dim, rotary->factor,
                      inverse ? -1.f : 1.f};
   p.n_tokens = n_tokens;
+  p.head_dim = head_dim;
   const int layout = rotary_layout(rotary, eb);
   p.units = layout == kRowsHalfOdd ? head_dim / 2 : head_dim * eb / 32;
   p.tile = kRotThreads / p.units;

@@ -36,17 +36,17 @@ __device__ __forceinline__ void rotary_sincos(u32 turn, float* sn, float* cs) {
   *cs = (quarter + 1) & 2 ? -b : b;
 }
 
-// How a head's D elements are taken as D / 2 pairs.  A lane holds VEC neighbouring pairs, unit
-// u the pairs u * VEC ...; pairs past rot / 2 are not turned.  VEC fills 16 bytes but in the
-// last layout.
-//   kRowsPlain        no pairs: 2 * VEC elements in a row, never turned
-//   kRowsHalf         (i, i + rot / 2): two 16-byte chunks; rot a multiple of 2 * VEC
-//   kRowsInterleaved  (2 i, 2 i + 1): 2 * VEC elements in a row
+// How a head's D elements are taken as D / 2 pairs.  A lane holds a unit of VEC pairs: two
+// chunks of VEC elements, so that neighbouring lanes read neighbouring chunks.  VEC fills 16
+// bytes but in the last layout.
+//   kRowsHalf         pair (i, i + rot / 2): a chunk of each half; rot a multiple of 2 * VEC
+//   kRowsInterleaved  pair (2 i, 2 i + 1): chunks u and u + D / (2 VEC), VEC / 2 pairs in each
 //   kRowsHalfOdd      as kRowsHalf for any even rot: one pair a lane, so that a wave's accesses
 //                     are neighbours though the halves begin anywhere
-enum RowLayout { kRowsPlain = 0, kRowsHalf = 1, kRowsInterleaved = 2, kRowsHalfOdd = 3 };
+// Channels past rot are not turned; rot 0 (values) is a row of plain chunks in any layout.
+enum RowLayout { kRowsHalf = 0, kRowsInterleaved = 1, kRowsHalfOdd = 2 };
 
-template <typename T, int LAYOUT>
+template <typename T, int LAYOUT = kRowsHalf>
 struct RowVec {
   static constexpr int kVec = LAYOUT == kRowsHalfOdd ? 1 : 16 / (int)sizeof(T);
 };
@@ -79,16 +79,30 @@ __device__ __forceinline__ u32x4_t narrow(const float* x, float) {
 
 // Elements at which a unit's two chunks begin.
 template <int LAYOUT, int VEC>
-__device__ __forceinline__ void unit_chunks(int u, int rot, int* a, int* b) {
-  if constexpr (LAYOUT == kRowsHalf || LAYOUT == kRowsHalfOdd) {
-    const int turned = rot / (2 * VEC);  // units that turn; the rest are pairs of neighbours
-    *a = u < turned ? u * VEC : u * 2 * VEC;
-    *b = u < turned ? rot / 2 + u * VEC : *a + VEC;
-  } else {
-    *a = u * 2 * VEC;
-    *b = *a + VEC;
-  }
+__device__ __forceinline__ void unit_chunks(int u, int rot, int d, int* a, int* b) {
+  if constexpr (LAYOUT == kRowsInterleaved) rot = 0;  // (its chunks lie as those of a plain row)
+  const int turned = rot / (2 * VEC);
+  *a = u < turned ? u * VEC : rot + (u - turned) * VEC;
+  *b = *a + (u < turned ? rot : d - rot) / 2;
 }
+
+// Pair j of unit u; pairs from rot / 2 on are not turned.
+template <int LAYOUT, int VEC>
+__device__ __forceinline__ int unit_pair(int u, int j, int d) {
+  if constexpr (LAYOUT == kRowsInterleaved) return (u * VEC + (j < VEC / 2 ? 0 : d / 2 - VEC)) / 2 + j;
+  return u * VEC + j;
+}
+
+// Which pairs of a unit turn: all, none, or (interleaved) those below `end`.
+template <int LAYOUT, int VEC>
+struct UnitTurns {
+  int unit, d, end;
+  bool all;
+  __device__ __forceinline__ UnitTurns(int u, int rot, int d_) : unit(u), d(d_), end(rot / 2) {
+    all = unit_pair<LAYOUT, VEC>(u, VEC - 1, d) < end;  // (the last pair is the unit's highest)
+  }
+  __device__ __forceinline__ bool turns(int j) const { return all || unit_pair<LAYOUT, VEC>(unit, j, d) < end; }
+};
 
 // One unit of a row as it lies in memory.
 template <typename T, int LAYOUT>
@@ -96,31 +110,28 @@ struct RowUnit {
   static constexpr int kVec = RowVec<T, LAYOUT>::kVec;
   static constexpr int kA = LAYOUT == kRowsInterleaved ? 2 : 1;      // pair j is x[kA j]
   static constexpr int kB = LAYOUT == kRowsInterleaved ? 1 : kVec;  // and x[kA j + kB]
+  using Turns = UnitTurns<LAYOUT, kVec>;
   u32x4_t w0, w1;
 
-  __device__ __forceinline__ void load(const T* row, int u, int rot) {
+  __device__ __forceinline__ void load(const T* row, int u, int rot, int d) {
     int a, b;
-    unit_chunks<LAYOUT, kVec>(u, rot, &a, &b);
+    unit_chunks<LAYOUT, kVec>(u, rot, d, &a, &b);
     w0 = ld_stream16(row + a);
     w1 = ld_stream16(row + b);
   }
 
-  __device__ __forceinline__ void zero() { w0 = w1 = u32x4_t{0u, 0u, 0u, 0u}; }
-
-  // x[0 .. VEC) and x[VEC .. 2 VEC): the elements of the two chunks, the unit's first n pairs
-  // turned (the others as they are, whatever their neighbour holds)
-  __device__ __forceinline__ void turned(const float* cs, const float* sn, int n, float* x) const {
+  // x[0 .. VEC) and x[VEC .. 2 VEC): the elements of the two chunks, turned where `t` says so
+  // (the others as they are, whatever their neighbour holds)
+  __device__ __forceinline__ void turned(const float* cs, const float* sn, const Turns& t, float* x) const {
     widen(w0, x, T{});
     widen(w1, x + kVec, T{});
-    if constexpr (LAYOUT != kRowsPlain) {
-      if (n == kVec) {
+    if (t.all) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
-      } else if constexpr (LAYOUT == kRowsInterleaved) {
+      for (int j = 0; j < kVec; ++j) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
+    } else if constexpr (LAYOUT == kRowsInterleaved) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (j < n) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
-      }
+      for (int j = 0; j < kVec; ++j)
+        if (t.turns(j)) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
     }
   }
 
@@ -134,19 +145,19 @@ struct RowUnit {
 template <typename T>
 struct RowUnit<T, kRowsHalfOdd> {
   static constexpr int kVec = 1;
+  using Turns = UnitTurns<kRowsHalfOdd, 1>;
   T e0, e1;
 
-  __device__ __forceinline__ void load(const T* row, int u, int rot) {
+  __device__ __forceinline__ void load(const T* row, int u, int rot, int d) {
     int a, b;
-    unit_chunks<kRowsHalfOdd, 1>(u, rot, &a, &b);
+    unit_chunks<kRowsHalfOdd, 1>(u, rot, d, &a, &b);
     e0 = row[a];
     e1 = row[b];
   }
-  __device__ __forceinline__ void zero() { e0 = e1 = T{}; }
-  __device__ __forceinline__ void turned(const float* cs, const float* sn, int n, float* x) const {
+  __device__ __forceinline__ void turned(const float* cs, const float* sn, const Turns& t, float* x) const {
     x[0] = to_f32(e0);
     x[1] = to_f32(e1);
-    if (n) RowUnit<T, kRowsHalf>::turn(x[0], x[1], cs[0], sn[0]);
+    if (t.all) RowUnit<T, kRowsHalf>::turn(x[0], x[1], cs[0], sn[0]);
   }
 };
 
@@ -155,10 +166,10 @@ __device__ __forceinline__ void put_one(float* to, float x) { *to = x; }
 
 // The unit's elements to a row of T.
 template <typename T, int LAYOUT>
-__device__ __forceinline__ void store_unit(T* row, int u, int rot, const float* x) {
+__device__ __forceinline__ void store_unit(T* row, int u, int rot, int d, const float* x) {
   constexpr int kVec = RowVec<T, LAYOUT>::kVec;
   int a, b;
-  unit_chunks<LAYOUT, kVec>(u, rot, &a, &b);
+  unit_chunks<LAYOUT, kVec>(u, rot, d, &a, &b);
   if constexpr (LAYOUT == kRowsHalfOdd) {
     put_one(row + a, x[0]);
     put_one(row + b, x[1]);
@@ -176,19 +187,14 @@ struct RotaryArgs {
   float sign;  // -1: the transposed rotation
 };
 
-// How many of unit u's VEC pairs turn.
-template <int VEC>
-__device__ __forceinline__ int unit_turns(int rot, int u) {
-  return min(max(rot / 2 - u * VEC, 0), VEC);
-}
-
-// Cosines and sines, times the factor, of a unit's first n pairs at position t.
-template <int VEC>
-__device__ __forceinline__ void unit_angles(const RotaryArgs& r, int t, int u, int n, float* cs, float* sn) {
+// Cosines and sines, times the factor, of unit u's pairs at position t.
+template <int LAYOUT, int VEC>
+__device__ __forceinline__ void unit_angles(const RotaryArgs& r, int t, const UnitTurns<LAYOUT, VEC>& turns, float* cs,
+                                            float* sn) {
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
     float s = 0.f, c = 1.f;
-    if (j < n) rotary_sincos(rotary_turn(t, r.w[u * VEC + j]), &s, &c);
+    if (turns.turns(j)) rotary_sincos(rotary_turn(t, r.w[unit_pair<LAYOUT, VEC>(turns.unit, j, turns.d)]), &s, &c);
     cs[j] = c * r.factor;
     sn[j] = s * (r.factor * r.sign);
   }
@@ -198,7 +204,7 @@ int check_rotary(const ia_rotary* r, int head_dim);  // rotary.hip
 
 // The layout whose loads fit: kRowsHalfOdd where the halves are no whole chunks.
 inline int rotary_layout(const ia_rotary* r, int elem_bytes) {
-  if (!r || r->dim == 0) return kRowsPlain;
+  if (!r || r->dim == 0) return kRowsHalf;
   if (r->interleaved) return kRowsInterleaved;
   return r->dim % (2 * (16 / elem_bytes)) ? kRowsHalfOdd : kRowsHalf;
 }

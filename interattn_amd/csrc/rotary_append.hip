@@ -2,11 +2,13 @@
 // the write side of a serving step, into bf16, f32 and fp8 pages.
 //
 // A workgroup per (sequence, page its new tokens touch, slice of heads).  A wave takes one
-// head's rows of the page, 16 at a time, as units of VEC pairs: lane = (row, unit), so that the
-// angles of its rows are computed once and serve every head, and a pair turns inside a lane.
+// head's rows of the page, 16 at a time (a part), as units of VEC pairs: lane = (row, unit), so
+// that the angles of its rows are computed once and serve every head, and a pair turns inside a
+// lane.  Pages of up to four parts give each part a wave of its own.
 //
-// fp8 pages have one float32 scale per (page, kv head).  The wave that holds the page's new
-// rows takes the largest magnitude a of its finite values (a reduction inside the wave) and
+// fp8 pages have one float32 scale per (page, kv head).  The waves that hold the page's new
+// rows take the largest magnitude a of its finite values (a reduction inside a wave, and over
+// its parts through LDS) and
 //   s = 2^ceil(log2(a / 448)), at least 2^-126;
 // a page that holds earlier tokens keeps its scale s0 where a <= 448 s0, else its earlier codes
 // c become e4m3(c * s0 / s).  A power of two costs e4m3 no relative precision (only up to one
@@ -105,92 +107,100 @@ __device__ void recode(char* rows, int64_t tok_stride, int n, float s0, float s,
 
 // One page of one sequence, as all of its tasks see it.
 struct WritePage {
-  int64_t page;    // -1: none
-  int64_t tok;     // packed row of page row 0 (may lie before the first row)
-  int lo, hi;      // the new rows' places in the page
-  int sub0, sub1;  // 16-row parts that hold them
+  int64_t page;  // -1: none
+  int64_t tok;   // packed row of page row 0 (may lie before the first row)
+  int lo, hi;    // the new rows' places in the page
 };
 
-// Rows of T, 16 of a page at a time, by one wave.
+// 16 rows of a page by one wave.  Lanes without a new row hold the nearest one: loads need no
+// condition (a branch around one would make every load wait for all before it), a maximum is
+// the same, and only stores ask.
 template <typename T, int D, int LAYOUT>
 struct PageRows {
   using Unit = RowUnit<T, LAYOUT>;
+  using Turns = typename Unit::Turns;
   static constexpr int kVec = Unit::kVec;
   static constexpr int kUnits = D / (2 * kVec);  // of a row
   static constexpr int kRows = 64 / kUnits;      // a wave's rows at once
   static constexpr int kGroups = kSub / kRows;   // of 16 rows
+  static constexpr int kFly = kGroups >= 4 ? 1 : 4 / kGroups;  // heads whose loads are in flight together
   static_assert(kRows >= 1 && kRows <= kSub, "a wave holds 1 to 16 rows, a unit a lane");
 
   const WriteParams& p;
   const WritePage& w;
-  int unit, row, turns;
+  int unit, row;
+  Turns turns;  // of q and k
+  Turns none;   // of v
   float cs[kGroups][kVec], sn[kGroups][kVec];
 
   __device__ __forceinline__ PageRows(const WriteParams& p_, const WritePage& w_, int lane)
-      : p(p_), w(w_), unit(lane % kUnits), row(lane / kUnits), turns(unit_turns<kVec>(p_.rot.rot, lane % kUnits)) {}
+      : p(p_), w(w_), unit(lane % kUnits), row(lane / kUnits), turns(lane % kUnits, p_.rot.rot, D), none(lane % kUnits, 0, D) {}
 
   __device__ __forceinline__ int place(int sub, int g) const { return sub * kSub + g * kRows + row; }
   __device__ __forceinline__ bool mine(int at) const { return at >= w.lo && at < w.hi; }
+  __device__ __forceinline__ int64_t token(int at) const { return w.tok + min(max(at, w.lo), w.hi - 1); }
 
-  __device__ __forceinline__ void angles(int sub, int64_t pos0) {
-    if constexpr (LAYOUT != kRowsPlain) {
+  __device__ __forceinline__ void angles(int sub, int64_t shift) {
+    if (p.rot.rot == 0) return;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int at = place(sub, g);
-        const int t = !mine(at) ? 0 : p.positions ? p.positions[w.tok + at] : (int)(pos0 + at);
-        unit_angles<kVec>(p.rot, t, unit, turns, cs[g], sn[g]);
-      }
+    for (int g = 0; g < kGroups; ++g) {
+      const int64_t tok = token(place(sub, g));
+      unit_angles<LAYOUT, kVec>(p.rot, p.positions ? p.positions[tok] : (int)(tok + shift), turns, cs[g], sn[g]);
     }
   }
 
   __device__ __forceinline__ void load(Unit* x, const char* rows, int64_t tok_stride, int sub) const {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int at = place(sub, g);
-      if (mine(at)) x[g].load(reinterpret_cast<const T*>(rows + (w.tok + at) * tok_stride), unit, p.rot.rot);
-      else x[g].zero();
-    }
+    for (int g = 0; g < kGroups; ++g)
+      x[g].load(reinterpret_cast<const T*>(rows + token(place(sub, g)) * tok_stride), unit, p.rot.rot, D);
   }
 
   // as rows of T, row0 the row of the page's first place
-  __device__ __forceinline__ void put(const Unit* x, char* rows, int64_t tok_stride, int64_t row0, int sub) const {
+  __device__ __forceinline__ void put(const Unit* x, const Turns& t, char* rows, int64_t tok_stride, int64_t row0,
+                                      int sub) const {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int at = place(sub, g);
-      if (!mine(at)) continue;
       float y[2 * kVec];
-      x[g].turned(cs[g], sn[g], turns, y);
-      store_unit<T, LAYOUT>(reinterpret_cast<T*>(rows + (row0 + at) * tok_stride), unit, p.rot.rot, y);
+      x[g].turned(cs[g], sn[g], t, y);
+      if (mine(at)) store_unit<T, LAYOUT>(reinterpret_cast<T*>(rows + (row0 + at) * tok_stride), unit, p.rot.rot, D, y);
     }
   }
 
-  // largest finite magnitude of the 16 places' new rows, in every lane
-  __device__ __forceinline__ float largest(const Unit* x) const {
+  // largest finite magnitude of the rows, in every lane
+  __device__ __forceinline__ float largest(const Unit* x, const Turns& t) const {
     float a = 0.f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       float y[2 * kVec];
-      x[g].turned(cs[g], sn[g], turns, y);
+      x[g].turned(cs[g], sn[g], t, y);
 #pragma unroll
       for (int j = 0; j < 2 * kVec; ++j) a = fmaxf(a, finite(y[j]) ? fabsf(y[j]) : 0.f);
     }
     return wave_max(a);
   }
 
-  // as e4m3 codes over the scale s; inv is its reciprocal where that is exact, else 0
-  __device__ __forceinline__ void put_codes(const Unit* x, char* rows, int64_t tok_stride, int sub, float s,
-                                            float inv) const {
+  // as e4m3 codes over the scale s
+  __device__ __forceinline__ void put_codes(const Unit* x, const Turns& t, char* rows, int64_t tok_stride, int sub,
+                                            float s) const {
+    // (a power of two is divided by exactly through its reciprocal)
+    const float inv = (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
+    int a, b;
+    unit_chunks<LAYOUT, kVec>(unit, p.rot.rot, D, &a, &b);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int at = place(sub, g);
-      if (!mine(at)) continue;
       float y[2 * kVec];
-      x[g].turned(cs[g], sn[g], turns, y);
+      x[g].turned(cs[g], sn[g], t, y);
+      if (inv != 0.f) {
 #pragma unroll
-      for (int j = 0; j < 2 * kVec; ++j) y[j] = inv != 0.f ? y[j] * inv : y[j] / s;
+        for (int j = 0; j < 2 * kVec; ++j) y[j] *= inv;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2 * kVec; ++j) y[j] /= s;
+      }
+      if (!mine(at)) continue;
       char* to = rows + at * tok_stride;
-      int a, b;
-      unit_chunks<LAYOUT, kVec>(unit, p.rot.rot, &a, &b);
       if constexpr (kVec == 8) {
         *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(y), fp8_codes(y + 4)};
         *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(y + 8), fp8_codes(y + 12)};
@@ -205,43 +215,45 @@ struct PageRows {
       }
     }
   }
-
-  // One head's new rows into its fp8 page.
-  __device__ __forceinline__ void quantise(const char* from, int64_t from_tok, char* rows, int64_t tok, float* scale,
-                                           int64_t pos0, int lane) {
-    const bool one = w.sub1 - w.sub0 == 1;  // the rows stay in registers between scale and codes
-    Unit x[kGroups];
-    float a = 0.f;
-    for (int sub = w.sub0; sub < w.sub1; ++sub) {
-      load(x, from, from_tok, sub);
-      if (!one) angles(sub, pos0);
-      a = fmaxf(a, largest(x));
-    }
-    float s = page_scale(a);
-    if (w.lo > 0) {  // earlier tokens: their scale, or their codes follow
-      const float s0 = *scale;
-      if (finite(s0) && s0 >= kLeastScale && a <= kLargestCode * s0)
-        s = s0;
-      else
-        recode<D>(rows, tok, w.lo, s0, s, lane);
-    }
-    if (lane == 0) *scale = s;
-    const float inv = (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
-    for (int sub = w.sub0; sub < w.sub1; ++sub) {
-      if (!one) {
-        load(x, from, from_tok, sub);
-        angles(sub, pos0);
-      }
-      put_codes(x, rows, tok, sub, s, inv);
-    }
-  }
 };
+
+// A head's tensor of the page's tasks: queries first, then keys, then values.
+struct WriteTask {
+  const char* from;
+  int64_t from_tok;
+  char* rows;  // page row 0
+  int64_t tok;
+  float* scale;
+  bool value;
+};
+
+__device__ __forceinline__ WriteTask kv_task(const WriteParams& p, int64_t page, int kv0, int n_kv, int i) {
+  const bool value = i >= n_kv;
+  const int64_t h = kv0 + (value ? i - n_kv : i);
+  WriteTask t;
+  t.value = value;
+  t.from = value ? p.v_new + h * p.vn_head : p.k_new + h * p.kn_head;
+  t.from_tok = value ? p.vn_tok : p.kn_tok;
+  t.rows = value ? p.v + page * p.v_page + h * p.v_head : p.k + page * p.k_page + h * p.k_head;
+  t.tok = value ? p.v_tok : p.k_tok;
+  t.scale = value ? p.v_scale + page * p.scale_page + h : p.k_scale + page * p.scale_page + h;
+  return t;
+}
+
+// The scale for new values of magnitude a of a page whose scale was s0; keeps: the earlier
+// codes stay as they are.
+__device__ __forceinline__ float settle(float a, bool begun, float s0, bool* keeps) {
+  *keeps = begun && finite(s0) && s0 >= kLeastScale && a <= kLargestCode * s0;
+  return *keeps ? s0 : page_scale(a);
+}
 
 template <typename T, bool FP8, int D, int LAYOUT>
 __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p) {
-  using Turned = PageRows<T, D, LAYOUT>;
-  using Plain = PageRows<T, D, kRowsPlain>;
+  using Rows = PageRows<T, D, LAYOUT>;
+  using Unit = typename Rows::Unit;
+  constexpr int kFly = Rows::kFly, kGroups = Rows::kGroups;
   __shared__ int first_gap;
+  __shared__ float parts[2][kFly][kWriteMaxThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = blockDim.x >> 6;
   int b, first, count;
@@ -289,45 +301,100 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   w.tok = first + (base - start);
   w.lo = (int)(start > base ? start - base : 0);
   w.hi = (int)(start + count - base < p.page_rows ? start + count - base : p.page_rows);
-  w.sub0 = w.lo / kSub;
-  w.sub1 = (w.hi + kSub - 1) / kSub;
-  const int64_t pos0 = base + (past < 0 ? past : 0);
-  const int kv0 = blockIdx.y * p.kv_heads_per_wg, kv1 = min(kv0 + p.kv_heads_per_wg, p.n_kv_heads);
-  Turned turned(p, w, lane);
-  Plain plain(p, w, lane);
-  const int n_kv = kv1 - kv0, n_q = p.q ? n_kv * p.group : 0;
-  for (int sub = w.sub0; sub < w.sub1; ++sub) {
-    turned.angles(sub, pos0);
-    for (int i = wave; i < n_q; i += waves) {
-      const int64_t h = (int64_t)kv0 * p.group + i;
-      typename Turned::Unit x[Turned::kGroups];
-      turned.load(x, p.q + h * p.q_head, p.q_tok, sub);
-      turned.put(x, p.q_out + h * p.qo_head, p.qo_tok, w.tok, sub);
+  const int64_t shift = past - first;  // a token's position less its packed row
+  const int kv0 = blockIdx.y * p.kv_heads_per_wg, n_kv = min(kv0 + p.kv_heads_per_wg, p.n_kv_heads) - kv0;
+  const int n_q = p.q ? n_kv * p.group : 0;
+
+  // parts with new rows: 1, 2 or up to 4 waves share a head's page, each with a part of its own;
+  // with more parts each wave goes through several
+  const int sub0 = w.lo / kSub, subs = (w.hi + kSub - 1) / kSub - sub0;
+  const int share = subs == 1 || waves < 2 ? 1 : subs == 2 || waves < 4 ? 2 : 4;
+  const int step = waves / share, slot = wave / share, part = wave % share;
+  const int turns_each = (subs + share - 1) / share;
+  Rows rows(p, w, lane);
+  for (int k = 0; k < turns_each; ++k) {
+    const int sub = sub0 + part + k * share;
+    rows.angles(sub, shift);
+    for (int i = slot; i < n_q; i += kFly * step) {
+      Unit x[kFly][kGroups];
+#pragma unroll
+      for (int f = 0; f < kFly; ++f)
+        rows.load(x[f], p.q + ((int64_t)kv0 * p.group + min(i + f * step, n_q - 1)) * p.q_head, p.q_tok, sub);
+#pragma unroll
+      for (int f = 0; f < kFly; ++f)
+        if (i + f * step < n_q)
+          rows.put(x[f], rows.turns, p.q_out + ((int64_t)kv0 * p.group + i + f * step) * p.qo_head, p.qo_tok, w.tok, sub);
     }
     if (FP8 || w.page < 0) continue;
-    for (int i = wave; i < 2 * n_kv; i += waves) {
-      const int64_t h = kv0 + (i < n_kv ? i : i - n_kv);
-      if (i < n_kv) {
-        typename Turned::Unit x[Turned::kGroups];
-        turned.load(x, p.k_new + h * p.kn_head, p.kn_tok, sub);
-        turned.put(x, p.k + w.page * p.k_page + h * p.k_head, p.k_tok, 0, sub);
-      } else {
-        typename Plain::Unit x[Plain::kGroups];
-        plain.load(x, p.v_new + h * p.vn_head, p.vn_tok, sub);
-        plain.put(x, p.v + w.page * p.v_page + h * p.v_head, p.v_tok, 0, sub);
+    for (int i = slot; i < 2 * n_kv; i += kFly * step) {
+      Unit x[kFly][kGroups];
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min(i + f * step, 2 * n_kv - 1));
+        rows.load(x[f], t.from, t.from_tok, sub);
+      }
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        if (i + f * step >= 2 * n_kv) break;
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, i + f * step);
+        rows.put(x[f], t.value ? rows.none : rows.turns, t.rows, t.tok, 0, sub);
       }
     }
   }
   if constexpr (FP8) {
     if (w.page < 0) return;
-    for (int i = wave; i < 2 * n_kv; i += waves) {
-      const int64_t h = kv0 + (i < n_kv ? i : i - n_kv);
-      if (i < n_kv)
-        turned.quantise(p.k_new + h * p.kn_head, p.kn_tok, p.k + w.page * p.k_page + h * p.k_head, p.k_tok,
-                        p.k_scale + w.page * p.scale_page + h, pos0, lane);
-      else
-        plain.quantise(p.v_new + h * p.vn_head, p.vn_tok, p.v + w.page * p.v_page + h * p.v_head, p.v_tok,
-                       p.v_scale + w.page * p.scale_page + h, pos0, lane);
+    // (every wave runs every round: the barriers are the workgroup's)
+    for (int round = 0; round * kFly * step < 2 * n_kv; ++round) {
+      Unit x[kFly][kGroups];
+      float s0[kFly], a[kFly];
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min((round * kFly + f) * step + slot, 2 * n_kv - 1));
+        s0[f] = w.lo > 0 ? *t.scale : 0.f;
+        rows.load(x[f], t.from, t.from_tok, sub0 + part);
+        a[f] = 0.f;
+      }
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min((round * kFly + f) * step + slot, 2 * n_kv - 1));
+        for (int k = 0; k < turns_each; ++k) {
+          const int sub = sub0 + part + k * share;
+          if (turns_each > 1) {
+            rows.load(x[f], t.from, t.from_tok, sub);
+            rows.angles(sub, shift);
+          }
+          a[f] = fmaxf(a[f], rows.largest(x[f], t.value ? rows.none : rows.turns));
+        }
+      }
+      if (share > 1) {
+#pragma unroll
+        for (int f = 0; f < kFly; ++f)
+          if (lane == 0) parts[round & 1][f][wave] = a[f];
+        __syncthreads();  // (and the earlier scale has been read by every wave)
+#pragma unroll
+        for (int f = 0; f < kFly; ++f)
+          for (int o = 0; o < share; ++o) a[f] = fmaxf(a[f], parts[round & 1][f][slot * share + o]);
+      }
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        const int i = (round * kFly + f) * step + slot;
+        if (i >= 2 * n_kv) break;
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, i);
+        bool keeps;
+        const float s = settle(a[f], w.lo > 0, s0[f], &keeps);
+        if (part == 0) {
+          if (w.lo > 0 && !keeps) recode<D>(t.rows, t.tok, w.lo, s0[f], s, lane);
+          if (lane == 0) *t.scale = s;
+        }
+        for (int k = 0; k < turns_each; ++k) {
+          const int sub = sub0 + part + k * share;
+          if (turns_each > 1) {
+            rows.load(x[f], t.from, t.from_tok, sub);
+            rows.angles(sub, shift);
+          }
+          rows.put_codes(x[f], t.value ? rows.none : rows.turns, t.rows, t.tok, sub, s);
+        }
+      }
     }
   }
 }
@@ -338,10 +405,8 @@ void launch_write(int layout, dim3 grid, dim3 block, hipStream_t st, const Write
     hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalf>), grid, block, 0, st, p);
   else if (layout == kRowsInterleaved)
     hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsInterleaved>), grid, block, 0, st, p);
-  else if (layout == kRowsHalfOdd)
-    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalfOdd>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsPlain>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalfOdd>), grid, block, 0, st, p);
 }
 
 template <typename T, bool FP8>
@@ -443,7 +508,7 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   p.kv_heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
   if (in_place) {
     p.kv_heads_per_wg = n_kv_heads;
-    threads = std::min(kWriteMaxThreads, 64 * (2 + (q ? p.group : 0)) * n_kv_heads);
+    threads = (2 + (q ? p.group : 0)) * n_kv_heads > 4 ? kWriteMaxThreads : kWriteThreads;
   }
   const int64_t ny = (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg;
   if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
