@@ -93,7 +93,7 @@ __device__ __forceinline__ int unit_pair(int u, int j, int d) {
   return u * VEC + j;
 }
 
-// Which pairs of a unit turn: all, none, or (interleaved) those below `end`.
+// Which pairs of a unit turn: those below `end`; in half layouts all or none.
 template <int LAYOUT, int VEC>
 struct UnitTurns {
   int unit, d, end;
@@ -101,7 +101,10 @@ struct UnitTurns {
   __device__ __forceinline__ UnitTurns(int u, int rot, int d_) : unit(u), d(d_), end(rot / 2) {
     all = unit_pair<LAYOUT, VEC>(u, VEC - 1, d) < end;  // (the last pair is the unit's highest)
   }
-  __device__ __forceinline__ bool turns(int j) const { return all || unit_pair<LAYOUT, VEC>(unit, j, d) < end; }
+  __device__ __forceinline__ bool turns(int j) const {
+    if constexpr (LAYOUT == kRowsInterleaved) return unit_pair<LAYOUT, VEC>(unit, j, d) < end;
+    return all;
+  }
 };
 
 // One unit of a row as it lies in memory.
@@ -125,13 +128,19 @@ struct RowUnit {
   __device__ __forceinline__ void turned(const float* cs, const float* sn, const Turns& t, float* x) const {
     widen(w0, x, T{});
     widen(w1, x + kVec, T{});
-    if (t.all) {
+    if constexpr (LAYOUT == kRowsInterleaved) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        float a = x[kA * j], b = x[kA * j + kB];
+        turn(a, b, cs[j], sn[j]);
+        if (t.turns(j)) {
+          x[kA * j] = a;
+          x[kA * j + kB] = b;
+        }
+      }
+    } else if (t.all) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
-    } else if constexpr (LAYOUT == kRowsInterleaved) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (t.turns(j)) turn(x[kA * j], x[kA * j + kB], cs[j], sn[j]);
     }
   }
 

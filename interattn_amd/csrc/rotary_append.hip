@@ -29,6 +29,7 @@ int check_kv(const ia_paged_kv* kv, int d);
 namespace {
 
 constexpr int kWriteThreads = 256, kWriteMaxThreads = 512;
+constexpr int kWriteBytes = 96 << 10;
 constexpr int kSub = 16;  // rows of a page taken at a time
 constexpr float kLargestCode = 448.f;
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
@@ -502,10 +503,15 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
                      rotary ? rotary->dim : 0, rotary ? rotary->factor : 1.f, 1.f};
   const int64_t tiles = cu_seqlens ? (int64_t)n_tokens / p.page_rows + 2 * (int64_t)n_seq : n_seq;
   if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
-  // few tiles: a workgroup for each kv head.  Lengths that advance in place are read by one
+  // A workgroup takes about kWriteBytes of rows: with 8 kv heads of 128 bf16 and groups of 4,
+  // pages of 16 (36k tokens into fp8) took 193 us with all heads to a workgroup, 183 with half
+  // of them and 220 with a quarter; pages of 64 227, 217 and 210; heads of 64 99, 119 and 176.
+  // Few tiles: a workgroup for each kv head.  Lengths that advance in place are read by one
   // workgroup only, of as many waves as it has tasks.
   int threads = kWriteThreads;
-  p.kv_heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
+  const int64_t head_rows = (int64_t)p.page_rows * (2 + (q ? p.group : 0)) * head_dim * eb;
+  const int64_t slices = tiles >= 2 * device_cus() ? std::max<int64_t>(1, n_kv_heads * head_rows / kWriteBytes) : n_kv_heads;
+  p.kv_heads_per_wg = (int)((n_kv_heads + std::min<int64_t>(slices, n_kv_heads) - 1) / std::min<int64_t>(slices, n_kv_heads));
   if (in_place) {
     p.kv_heads_per_wg = n_kv_heads;
     threads = (2 + (q ? p.group : 0)) * n_kv_heads > 4 ? kWriteMaxThreads : kWriteThreads;
