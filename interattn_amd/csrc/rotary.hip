@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kRotThreads) void ia_rotary_turn(RotParams p) {
       RowUnit<T, LAYOUT> x[kRotFly];
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
-        if (h + i < b) x[i].load(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot, p.head_dim);
+        if (h + i < b) x[i].template load<true>(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot, p.head_dim);
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
         if (h + i < b) {

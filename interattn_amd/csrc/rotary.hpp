@@ -116,11 +116,13 @@ struct RowUnit {
   using Turns = UnitTurns<LAYOUT, kVec>;
   u32x4_t w0, w1;
 
+  // STREAM: past the caches (rows larger than they hold)
+  template <bool STREAM>
   __device__ __forceinline__ void load(const T* row, int u, int rot, int d) {
     int a, b;
     unit_chunks<LAYOUT, kVec>(u, rot, d, &a, &b);
-    w0 = ld_stream16(row + a);
-    w1 = ld_stream16(row + b);
+    w0 = STREAM ? ld_stream16(row + a) : *reinterpret_cast<const u32x4_t*>(row + a);
+    w1 = STREAM ? ld_stream16(row + b) : *reinterpret_cast<const u32x4_t*>(row + b);
   }
 
   // x[0 .. VEC) and x[VEC .. 2 VEC): the elements of the two chunks, turned where `t` says so
@@ -157,6 +159,7 @@ struct RowUnit<T, kRowsHalfOdd> {
   using Turns = UnitTurns<kRowsHalfOdd, 1>;
   T e0, e1;
 
+  template <bool STREAM>
   __device__ __forceinline__ void load(const T* row, int u, int rot, int d) {
     int a, b;
     unit_chunks<kRowsHalfOdd, 1>(u, rot, d, &a, &b);

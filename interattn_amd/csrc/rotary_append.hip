@@ -153,7 +153,7 @@ struct PageRows {
   __device__ __forceinline__ void load(Unit* x, const char* rows, int64_t tok_stride, int sub) const {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g)
-      x[g].load(reinterpret_cast<const T*>(rows + token(place(sub, g)) * tok_stride), unit, p.rot.rot, D);
+      x[g].template load<false>(reinterpret_cast<const T*>(rows + token(place(sub, g)) * tok_stride), unit, p.rot.rot, D);
   }
 
   // as rows of T, row0 the row of the page's first place
