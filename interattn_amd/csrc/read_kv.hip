@@ -1,9 +1,9 @@
 // Cached rows as packed tensors for gfx950: the way back from the paged pool.
 //
 //   ia_read_kv_rows: a workgroup per tile of one sequence's tokens; a thread's token, page and
-//   16-byte chunk are fixed, and it goes through the heads of its slice with the K and V loads
-//   of a pass in flight.  fp8 codes are widened exactly, times their page's scale, rounded
-//   once.  Bound by HBM.
+//   16-byte chunk of the output row are fixed (so that a wave's stores are whole lines), and it
+//   goes through the heads of its slice with the K and V loads of a pass in flight.  fp8 codes
+//   are widened exactly, times their page's scale, rounded once.  Bound by HBM.
 #include <algorithm>
 
 #include "packed_rows.hpp"
@@ -33,57 +33,74 @@ struct ReadParams {
   const int32_t* starts;
   const int32_t* cu;
   int32_t n_seq, n_tokens, n_kv_heads, heads_per_wg;
-  int32_t chunks;  // 16-byte chunks of a pool row
+  int32_t chunks;  // 16-byte chunks of an output row
   int32_t tile;    // tokens of a tile
 };
 
-// One chunk of a pool row as OutT's elements.
-template <typename PoolT, typename OutT>
-struct ReadChunk;
-
-template <typename T>
-struct ReadChunk<T, T> {
-  static constexpr int kElems = RowVec<T>::kVec;
-  static __device__ __forceinline__ void put(T* to, const u32x4_t& w, float) { *reinterpret_cast<u32x4_t*>(to) = w; }
-};
-template <>
-struct ReadChunk<bf16_t, float> {
-  static constexpr int kElems = 8;
-  static __device__ __forceinline__ void put(float* to, const u32x4_t& w, float) {
-    float x[8];
-    widen(w, x, bf16_t{});
-    reinterpret_cast<u32x4_t*>(to)[0] = narrow(x, float{});
-    reinterpret_cast<u32x4_t*>(to)[1] = narrow(x + 4, float{});
-  }
-};
-template <>
-struct ReadChunk<float, bf16_t> {
-  static constexpr int kElems = 4;
-  static __device__ __forceinline__ void put(bf16_t* to, const u32x4_t& w, float) {
-    float x[4];
-    widen(w, x, float{});
-    *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-  }
-};
 struct fp8_t {
   unsigned char bits;
 };
-template <typename OutT>
-struct ReadChunk<fp8_t, OutT> {
-  static constexpr int kElems = 16;
-  static __device__ __forceinline__ void put(OutT* to, const u32x4_t& w, float s) {
-    float x[16];
+
+// What of a pool row becomes 16 bytes of OutT.
+template <typename PoolT, typename OutT>
+struct ReadChunk {
+  static constexpr int kElems = 16 / (int)sizeof(OutT), kBytes = kElems * (int)sizeof(PoolT), kWords = kBytes / 4;
+  u32 w[kWords];
+
+  __device__ __forceinline__ void load(const char* at) {
+    if constexpr (kWords == 1) {
+      w[0] = ld_stream4(at);
+    } else if constexpr (kWords == 2) {
+      const u32x2_t x = ld_stream8(at);
+      w[0] = x[0];
+      w[1] = x[1];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fp8x4_to_f32(w[i], x + 4 * i);
+      for (int i = 0; i < kWords; i += 4) {
+        const u32x4_t x = ld_stream16(at + 4 * i);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] *= s;
-    constexpr int kVec = RowVec<OutT>::kVec;
+        for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int j = 0; j < 16; j += kVec) *reinterpret_cast<u32x4_t*>(to + j) = narrow(x + j, OutT{});
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ u32x4_t out(float s) const {
+    if constexpr (sizeof(PoolT) == sizeof(OutT)) {
+      return u32x4_t{w[0], w[1], w[2], w[3]};
+    } else {
+      float x[kElems];
+      if constexpr (sizeof(PoolT) == 1) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) fp8x4_to_f32(w[i], x + 4 * i);
+#pragma unroll
+        for (int j = 0; j < kElems; ++j) x[j] *= s;
+      } else if constexpr (sizeof(PoolT) == 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          x[2 * i] = bf16_lo(w[i]);
+          x[2 * i + 1] = bf16_hi(w[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) x[i] = __uint_as_float(w[i]);
+      }
+      return narrow(x, OutT{});
+    }
   }
 };
 
-template <typename PoolT, typename OutT>
+template <bool STREAM>
+__device__ __forceinline__ void put16(char* to, const u32x4_t& w) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(to));
+  else
+    *reinterpret_cast<u32x4_t*>(to) = w;
+}
+
+template <typename PoolT, typename OutT, bool STREAM>
 __global__ __launch_bounds__(kReadThreads) void ia_read_kv_rows(ReadParams p) {
   using C = ReadChunk<PoolT, OutT>;
   constexpr bool kScaled = sizeof(PoolT) == 1;
@@ -103,22 +120,21 @@ __global__ __launch_bounds__(kReadThreads) void ia_read_kv_rows(ReadParams p) {
   const bool held = pg >= 0;
   if (!held) pg = 0;
   const int h0 = blockIdx.y * p.heads_per_wg, h1 = min(h0 + p.heads_per_wg, p.n_kv_heads);
-  const char* ks = p.k + pg * p.k_page + in * p.k_tok + chunk * 16;
-  const char* vs = p.v + pg * p.v_page + in * p.v_tok + chunk * 16;
-  const int64_t row = (int64_t)p.chunks * C::kElems;
-  const int64_t out = ((int64_t)(t.tok0 + tok) * p.n_kv_heads) * row + chunk * C::kElems;
-  OutT* kd = reinterpret_cast<OutT*>(p.k_out) + out;
-  OutT* vd = reinterpret_cast<OutT*>(p.v_out) + out;
+  const char* ks = p.k + pg * p.k_page + in * p.k_tok + chunk * C::kBytes;
+  const char* vs = p.v + pg * p.v_page + in * p.v_tok + chunk * C::kBytes;
+  const int64_t row = (int64_t)p.chunks * 16;
+  const int64_t out = (int64_t)(t.tok0 + tok) * p.n_kv_heads * row + chunk * 16;
   for (int h = h0; h < h1; h += kReadHeads) {
-    u32x4_t a[kReadHeads], b[kReadHeads];
+    C a[kReadHeads], b[kReadHeads];
     float sa[kReadHeads], sb[kReadHeads];
 #pragma unroll
     for (int i = 0; i < kReadHeads; ++i) {
-      a[i] = b[i] = u32x4_t{0u, 0u, 0u, 0u};
+      a[i].zero();
+      b[i].zero();
       sa[i] = sb[i] = 1.f;
       if (held && h + i < h1) {
-        a[i] = ld_stream16(ks + (h + i) * p.k_head);
-        b[i] = ld_stream16(vs + (h + i) * p.v_head);
+        a[i].load(ks + (h + i) * p.k_head);
+        b[i].load(vs + (h + i) * p.v_head);
         if constexpr (kScaled) {
           sa[i] = p.k_scale[pg * p.scale_page + h + i];
           sb[i] = p.v_scale[pg * p.scale_page + h + i];
@@ -128,18 +144,26 @@ __global__ __launch_bounds__(kReadThreads) void ia_read_kv_rows(ReadParams p) {
 #pragma unroll
     for (int i = 0; i < kReadHeads; ++i)
       if (h + i < h1) {
-        C::put(kd + (h + i) * row, a[i], sa[i]);
-        C::put(vd + (h + i) * row, b[i], sb[i]);
+        put16<STREAM>(p.k_out + out + (h + i) * row, a[i].out(sa[i]));
+        put16<STREAM>(p.v_out + out + (h + i) * row, b[i].out(sb[i]));
       }
   }
 }
 
-template <typename PoolT>
-void launch_read(int out_dtype, dim3 grid, hipStream_t st, const ReadParams& p) {
-  if (out_dtype == IA_F32)
-    hipLaunchKernelGGL((ia_read_kv_rows<PoolT, float>), grid, dim3(kReadThreads), 0, st, p);
+template <typename PoolT, typename OutT>
+void launch_read(bool past_caches, dim3 grid, hipStream_t st, const ReadParams& p) {
+  if (past_caches)
+    hipLaunchKernelGGL((ia_read_kv_rows<PoolT, OutT, true>), grid, dim3(kReadThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((ia_read_kv_rows<PoolT, bf16_t>), grid, dim3(kReadThreads), 0, st, p);
+    hipLaunchKernelGGL((ia_read_kv_rows<PoolT, OutT, false>), grid, dim3(kReadThreads), 0, st, p);
+}
+
+template <typename PoolT>
+void launch_read_as(int out_dtype, bool past_caches, dim3 grid, hipStream_t st, const ReadParams& p) {
+  if (out_dtype == IA_F32)
+    launch_read<PoolT, float>(past_caches, grid, st, p);
+  else
+    launch_read<PoolT, bf16_t>(past_caches, grid, st, p);
 }
 
 }  // namespace
@@ -183,7 +207,8 @@ extern "C" int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32
   p.n_seq = n_seq;
   p.n_tokens = n_tokens;
   p.n_kv_heads = n_kv_heads;
-  p.chunks = head_dim * eb / 16;
+  const int ob = out_dtype == IA_F32 ? 4 : 2;
+  p.chunks = head_dim * ob / 16;
   p.tile = kReadThreads / p.chunks;
   const int64_t tiles = (int64_t)n_tokens / p.tile + n_seq;
   if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
@@ -192,11 +217,13 @@ extern "C" int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32
   if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
   const dim3 grid((unsigned)tiles, (unsigned)ny);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  // outputs larger than the L2s are written past them, as stream_rows says
+  const bool past = stream_rows(nullptr, kRowsHalf, (int64_t)n_tokens * n_kv_heads * head_dim * ob, ob);
   if (kv->dtype == IA_F32)
-    launch_read<float>(out_dtype, grid, st, p);
+    launch_read_as<float>(out_dtype, past, grid, st, p);
   else if (kv->dtype == IA_BF16)
-    launch_read<bf16_t>(out_dtype, grid, st, p);
+    launch_read_as<bf16_t>(out_dtype, past, grid, st, p);
   else
-    launch_read<fp8_t>(out_dtype, grid, st, p);
+    launch_read_as<fp8_t>(out_dtype, past, grid, st, p);
   return check_launch("read kv");
 }

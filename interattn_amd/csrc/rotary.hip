@@ -39,7 +39,7 @@ struct RotParams {
   int n_tokens, head_dim, units, tile, heads_per_wg;
 };
 
-template <typename T, int LAYOUT>
+template <typename T, int LAYOUT, bool STREAM>
 __global__ __launch_bounds__(kRotThreads) void ia_rotary_turn(RotParams p) {
   constexpr int kVec = RowVec<T, LAYOUT>::kVec;
   const int u = threadIdx.x % p.units, local = threadIdx.x / p.units;
@@ -61,26 +61,34 @@ __global__ __launch_bounds__(kRotThreads) void ia_rotary_turn(RotParams p) {
       RowUnit<T, LAYOUT> x[kRotFly];
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
-        if (h + i < b) x[i].template load<true>(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot, p.head_dim);
+        if (h + i < b) x[i].template load<STREAM>(reinterpret_cast<const T*>(in + (h + i) * t.in_head), u, p.rot.rot, p.head_dim);
 #pragma unroll
       for (int i = 0; i < kRotFly; ++i)
         if (h + i < b) {
           float y[2 * kVec];
           x[i].turned(cs, sn, turns, y);
-          store_unit<T, LAYOUT>(reinterpret_cast<T*>(out + (h + i) * t.out_head), u, p.rot.rot, p.head_dim, y);
+          store_unit<T, LAYOUT, STREAM>(reinterpret_cast<T*>(out + (h + i) * t.out_head), u, p.rot.rot, p.head_dim, y);
         }
     }
   }
 }
 
-template <typename T>
-void launch_rotary(int layout, dim3 grid, hipStream_t st, const RotParams& p) {
-  if (layout == kRowsHalf)
-    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalf>), grid, dim3(kRotThreads), 0, st, p);
-  else if (layout == kRowsInterleaved)
-    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsInterleaved>), grid, dim3(kRotThreads), 0, st, p);
+template <typename T, int LAYOUT>
+void launch_layout(bool stream, dim3 grid, hipStream_t st, const RotParams& p) {
+  if (stream)
+    hipLaunchKernelGGL((ia_rotary_turn<T, LAYOUT, true>), grid, dim3(kRotThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalfOdd>), grid, dim3(kRotThreads), 0, st, p);
+    hipLaunchKernelGGL((ia_rotary_turn<T, LAYOUT, false>), grid, dim3(kRotThreads), 0, st, p);
+}
+
+template <typename T>
+void launch_rotary(int layout, bool stream, dim3 grid, hipStream_t st, const RotParams& p) {
+  if (layout == kRowsHalf)
+    launch_layout<T, kRowsHalf>(stream, grid, st, p);
+  else if (layout == kRowsInterleaved)
+    launch_layout<T, kRowsInterleaved>(stream, grid, st, p);
+  else
+    hipLaunchKernelGGL((ia_rotary_turn<T, kRowsHalfOdd, false>), grid, dim3(kRotThreads), 0, st, p);
 }
 
 }  // namespace
@@ -134,9 +142,10 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
   if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
   const dim3 grid((unsigned)tiles, (unsigned)ny);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool stream_them = stream_rows(rotary, layout, n_tokens * all * head_dim * eb, eb);
   if (dtype == IA_F32)
-    launch_rotary<float>(layout, grid, st, p);
+    launch_rotary<float>(layout, stream_them, grid, st, p);
   else
-    launch_rotary<bf16_t>(layout, grid, st, p);
+    launch_rotary<bf16_t>(layout, stream_them, grid, st, p);
   return check_launch("rotary");
 }

@@ -58,6 +58,7 @@ struct WriteParams {
   const int32_t* positions;  // null: the place in the sequence
   int32_t n_seq, n_tokens, n_kv_heads, group, kv_heads_per_wg;
   RotaryArgs rot;
+  bool stream;  // the queries' rows are written past the caches
 };
 
 __device__ __forceinline__ int64_t write_page(const WriteParams& p, int b, int64_t lp) {
@@ -157,14 +158,23 @@ struct PageRows {
   }
 
   // as rows of T, row0 the row of the page's first place
-  __device__ __forceinline__ void put(const Unit* x, const Turns& t, char* rows, int64_t tok_stride, int64_t row0,
-                                      int sub) const {
+  __device__ __forceinline__ void put(const Unit* x, const Turns& t, char* rows, int64_t tok_stride, int64_t row0, int sub,
+                                      bool stream) const {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int at = place(sub, g);
       float y[2 * kVec];
       x[g].turned(cs[g], sn[g], t, y);
-      if (mine(at)) store_unit<T, LAYOUT>(reinterpret_cast<T*>(rows + (row0 + at) * tok_stride), unit, p.rot.rot, D, y);
+      if (!mine(at)) continue;
+      T* to = reinterpret_cast<T*>(rows + (row0 + at) * tok_stride);
+      if (stream) {
+        // (the asm keeps the two branches' stores from being made one, without the hint)
+        asm volatile("");
+        store_unit<T, LAYOUT, true>(to, unit, p.rot.rot, D, y);
+        asm volatile("");
+      } else {
+        store_unit<T, LAYOUT, false>(to, unit, p.rot.rot, D, y);
+      }
     }
   }
 
@@ -324,7 +334,8 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
 #pragma unroll
       for (int f = 0; f < kFly; ++f)
         if (i + f * step < n_q)
-          rows.put(x[f], rows.turns, p.q_out + ((int64_t)kv0 * p.group + i + f * step) * p.qo_head, p.qo_tok, w.tok, sub);
+          rows.put(x[f], rows.turns, p.q_out + ((int64_t)kv0 * p.group + i + f * step) * p.qo_head, p.qo_tok, w.tok, sub,
+                   p.stream);
     }
     if (FP8 || w.page < 0) continue;
     for (int i = slot; i < 2 * n_kv; i += kFly * step) {
@@ -338,7 +349,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
       for (int f = 0; f < kFly; ++f) {
         if (i + f * step >= 2 * n_kv) break;
         const WriteTask t = kv_task(p, w.page, kv0, n_kv, i + f * step);
-        rows.put(x[f], t.value ? rows.none : rows.turns, t.rows, t.tok, 0, sub);
+        rows.put(x[f], t.value ? rows.none : rows.turns, t.rows, t.tok, 0, sub, p.stream);
       }
     }
   }
@@ -521,6 +532,7 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   const dim3 grid((unsigned)tiles, (unsigned)ny), block((unsigned)threads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int layout = rotary_layout(rotary, eb);
+  p.stream = stream_rows(rotary, layout, (int64_t)n_tokens * p.group * n_kv_heads * head_dim * eb, eb);
   if (rows->dtype == IA_BF16)
     fp8 ? launch_write_d<bf16_t, true>(head_dim, layout, grid, block, st, p)
         : launch_write_d<bf16_t, false>(head_dim, layout, grid, block, st, p);
