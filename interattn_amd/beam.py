@@ -44,9 +44,9 @@ def beam_select(logits, scores, n=None, *, done=None, pad_token=0, workspace=Non
                              or not done.is_contiguous()):
         raise ValueError("done must be contiguous bool [batch, beams]")
     dev, code = logits.device, _LOGITS[logits.dtype]
-    best = torch.empty((batch, n), device=dev, dtype=torch.float32)
-    tokens = torch.empty((batch, n), device=dev, dtype=torch.int32)
-    parents = torch.empty((batch, n), device=dev, dtype=torch.int32)
+    best = scores.new_empty((batch, n))
+    tokens = scores.new_empty((batch, n), dtype=torch.int32)
+    parents = torch.empty_like(tokens)
     if batch == 0:
         return best, tokens, parents
     lib = N.lib()

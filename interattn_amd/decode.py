@@ -296,6 +296,9 @@ class PagedTopkDecodeRunner:
         self.k_bar_dtype = k_bar_dtype or self.dtype
         if self.block_size % 16 or self.page_size % 16:
             raise ValueError("block_size and page_size must be multiples of 16")
+        if self.kv_dtype != self.dtype and self.block_size % self.page_size:
+            # (a page whose scale rises rounds its earlier tokens again: its block is summed anew)
+            raise ValueError("an fp8 cache (kv_dtype) needs a page_size that divides block_size")
         self.nb_max = -(-self.max_seq_len // self.block_size)
         pages_per_seq = -(-self.max_seq_len // self.page_size)
         gen = torch.Generator(device="cpu").manual_seed(int(seed))

@@ -211,7 +211,8 @@ def update_block_summaries(summ, pool_k, pool_v, block_table, old_seq_lens, seq_
     """Refresh ``summ`` (a ``build_block_summaries`` dict, holding the summaries at
     ``old_seq_lens``) in place for sequences grown to ``seq_lens``; only the blocks
     the new tokens touch are recomputed (``max_new_tokens`` bounds the growth).
-    Equal to a full rebuild at ``seq_lens``."""
+    Equal to a full rebuild at ``seq_lens`` (in fp8 pools whose pages are larger than a
+    block, writing can round a page's tokens of an earlier block again: rebuild then)."""
     kv, keep = paged_kv(pool_k, pool_v, block_table, scales)
     _require_cuda(old_seq_lens, seq_lens)
     _check_i32(old_seq_lens, "old_seq_lens")

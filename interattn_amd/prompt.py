@@ -284,14 +284,11 @@ def read_kv(pool_k, pool_v, block_table, starts, cu_seqlens, n_tokens, *, scales
     if out_dtype not in (_F32, _BF16):
         raise ValueError("out_dtype must be float32 or bfloat16")
     shape = (int(n_tokens), hkv, d)
-    outs = []
     for out in (k_out, v_out):
-        if out is None:
-            out = torch.empty(shape, device=pool_k.device, dtype=out_dtype)
-        elif out.shape != shape or out.dtype != out_dtype or not out.is_contiguous():
+        if out is not None and (out.shape != shape or out.dtype != out_dtype or not out.is_contiguous()):
             raise ValueError(f"k_out and v_out must be contiguous {list(shape)} tensors of out_dtype")
-        outs.append(out)
-    k, v = outs
+    k = pool_k.new_empty(shape, dtype=out_dtype) if k_out is None else k_out
+    v = torch.empty_like(k) if v_out is None else v_out
     launch(N.lib().ia_read_kv, pool_k, kv, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[out_dtype], starts.data_ptr(),
            cu_seqlens.data_ptr(), n_seq, shape[0], hkv, d)
     return k, v

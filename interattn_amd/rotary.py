@@ -19,6 +19,7 @@ from .prompt import check_ints, device_of, launch, packed_rows, pool_of, prompt_
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16)
 LAYOUTS = ("half", "interleaved")
+_TWO_ROWS = N.RotaryRows * 2
 
 
 class RotaryPlan:
@@ -127,13 +128,16 @@ def _heads(shape, stride, dtype, what):
 
 def _rows(x, out, what):
     """``RotaryRows`` of ``x`` and its output (made where None), and the output."""
-    heads, d, tok, head = _heads(x.shape[1:], x.stride(), x.dtype, what)
+    shape = x.shape
+    heads, d, tok, head = _heads(shape[1:], x.stride(), x.dtype, what)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError(f"{what}_out must have {what}'s shape and dtype")
-    _, _, o_tok, o_head = _heads(out.shape[1:], out.stride(), out.dtype, what + "_out")
-    if x.shape[0] <= 1:
+        out = x.new_empty(shape)
+        o_tok, o_head = heads * d, d
+    else:
+        if out.shape != shape or out.dtype != x.dtype:
+            raise ValueError(f"{what}_out must have {what}'s shape and dtype")
+        _, _, o_tok, o_head = _heads(shape[1:], out.stride(), out.dtype, what + "_out")
+    if shape[0] <= 1:
         tok = o_tok = 0  # (any stride means nothing then)
     return N.RotaryRows(x.data_ptr(), out.data_ptr(), tok, head, o_tok, o_head, heads), out
 
@@ -146,18 +150,21 @@ def apply_rotary(q, k, positions, plan, *, inverse=False, q_out=None, k_out=None
     themselves.  ``inverse``: angles negated (the gradient; a rotation by position differences
     moves cached keys)."""
     device_of(q, k, positions, plan.turns if plan.dim else None, q_out, k_out)
-    tokens = check_ints(positions, "positions", q.shape[0] if q.dim() else None)
+    shape = q.shape
+    tokens = check_ints(positions, "positions", shape[0] if len(shape) else None)
     q_rows, q_out = _rows(q, q_out, "q")
-    d = q.shape[2]
+    d = shape[2]
     n = 1
-    rows = (N.RotaryRows * 2)(q_rows)
     if k is not None:
-        if k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
+        of_k = k.shape
+        if len(of_k) != 3 or of_k[0] != tokens or of_k[2] != d or k.dtype != q.dtype:
             raise ValueError("k must have q's tokens, head_dim and dtype")
-        rows[1], k_out = _rows(k, k_out, "k")
-        n = 2
-    elif k_out is not None:
-        raise ValueError("k_out is given without k")
+        k_rows, k_out = _rows(k, k_out, "k")
+        rows, n = _TWO_ROWS(q_rows, k_rows), 2
+    else:
+        if k_out is not None:
+            raise ValueError("k_out is given without k")
+        rows = _TWO_ROWS(q_rows)
     if tokens:
         launch(N.lib().ia_apply_rotary, q, plan.native, rows, n, _DTYPE_CODE[q.dtype], d, positions.data_ptr(), tokens,
                int(inverse))
@@ -203,14 +210,15 @@ def rotary_append_kv(q, k_new, v_new, plan, pool_k, pool_v, block_table, seq_len
         check_ints(positions, "positions", tokens)
     q_rows = None
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != d or q.dtype != k_new.dtype:
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != d or q.dtype != k_new.dtype:
             raise ValueError("q must be [tokens, Hq, D] with k_new's tokens, head_dim and dtype")
-        if q.shape[1] == 0 or q.shape[1] % hkv:
+        if shape[1] == 0 or shape[1] % hkv:
             raise ValueError("n_q_heads must be a multiple of n_kv_heads (grouped query attention)")
         q_rows, q_out = _rows(q, q_out, "q")
     elif q_out is not None:
         raise ValueError("q_out is given without q")
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch(N.lib().ia_rotary_append_kv, k_new, None if plan is None else plan.native, q_rows, rows, kv, p(cu_seqlens),
-           seq_lens.data_ptr(), new_seq_lens.data_ptr(), p(positions), n_seq, tokens, hkv, d)
+    launch(N.lib().ia_rotary_append_kv, k_new, None if plan is None else plan.native, q_rows, rows, kv,
+           None if cu_seqlens is None else cu_seqlens.data_ptr(), seq_lens.data_ptr(), new_seq_lens.data_ptr(),
+           None if positions is None else positions.data_ptr(), n_seq, tokens, hkv, d)
     return q_out, new_seq_lens

@@ -245,3 +245,6 @@ def test_the_paged_runner_on_an_8_bit_cache(device):
     for refused, kv in ((model, torch.float16), (_model(device), torch.float8_e4m3fn)):
         with pytest.raises(ValueError, match="kv_dtype"):
             PagedTopkDecodeRunner(model=refused, batch_size=2, max_seq_len=128, block_size=32, k=8, kv_dtype=kv)
+    with pytest.raises(ValueError, match="divides block_size"):
+        PagedTopkDecodeRunner(model=model, batch_size=2, max_seq_len=128, block_size=16, page_size=32, k=8,
+                              kv_dtype=torch.float8_e4m3fn)
