@@ -77,15 +77,15 @@ __device__ __forceinline__ float page_scale(float a) {
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Four floats, already divided by their scale, as e4m3 codes; not finite: NaN.
+// Four floats, already divided by their scale, as e4m3 codes.
 __device__ __forceinline__ u32 fp8_codes(const float* x) {
-  float y[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = finite(x[j]) ? x[j] : __uint_as_float(0x7fc00000u);
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
   return (u32)w;
 }
+
+// Not finite: NaN, which has a code (infinity has none).
+__device__ __forceinline__ float or_nan(float x) { return finite(x) ? x : __uint_as_float(0x7fc00000u); }
 
 // The earlier rows [0, n) of one head's page from scale s0 to s.
 template <int D>
@@ -100,7 +100,7 @@ __device__ void recode(char* rows, int64_t tok_stride, int n, float s0, float s,
       float x[4];
       fp8x4_to_f32(w[i], x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= ratio;
+      for (int j = 0; j < 4; ++j) x[j] = or_nan(x[j] * ratio);
       w[i] = fp8_codes(x);
     }
     *at = w;
@@ -178,22 +178,42 @@ struct PageRows {
     }
   }
 
-  // largest finite magnitude of the rows, in every lane
-  __device__ __forceinline__ float largest(const Unit* x, const Turns& t) const {
-    float a = 0.f;
+  using Values = float[kGroups][2 * kVec];
+
+  __device__ __forceinline__ void turn(const Unit* x, const Turns& t, Values& y) const {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      float y[2 * kVec];
-      x[g].turned(cs[g], sn[g], t, y);
+    for (int g = 0; g < kGroups; ++g) x[g].turned(cs[g], sn[g], t, y[g]);
+  }
+
+  // Largest finite magnitude of the rows, in every lane; what is not finite becomes NaN.  As
+  // integers, floats of either sign rise with their magnitude, and what is not finite is above
+  // all others: one maximum of each sign finds both.
+  __device__ __forceinline__ float largest(Values& y) const {
+    int plus = 0;
+    u32 minus = 0;
 #pragma unroll
-      for (int j = 0; j < 2 * kVec; ++j) a = fmaxf(a, finite(y[j]) ? fabsf(y[j]) : 0.f);
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int j = 0; j < 2 * kVec; ++j) {
+        plus = max(plus, __float_as_int(y[g][j]));
+        minus = max(minus, __float_as_uint(y[g][j]));
+      }
+    float a = __uint_as_float(max((u32)plus, minus & 0x7fffffffu));
+    if (!finite(a)) {
+      a = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int j = 0; j < 2 * kVec; ++j) {
+          y[g][j] = or_nan(y[g][j]);
+          a = fmaxf(a, fabsf(y[g][j]));  // (a maximum passes over NaN)
+        }
     }
     return wave_max(a);
   }
 
   // as e4m3 codes over the scale s
-  __device__ __forceinline__ void put_codes(const Unit* x, const Turns& t, char* rows, int64_t tok_stride, int sub,
-                                            float s) const {
+  __device__ __forceinline__ void put_codes(const Values& y, char* rows, int64_t tok_stride, int sub, float s) const {
     // (a power of two is divided by exactly through its reciprocal)
     const float inv = (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
     int a, b;
@@ -201,25 +221,23 @@ struct PageRows {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int at = place(sub, g);
-      float y[2 * kVec];
-      x[g].turned(cs[g], sn[g], t, y);
+      float z[2 * kVec < 4 ? 4 : 2 * kVec] = {};
       if (inv != 0.f) {
 #pragma unroll
-        for (int j = 0; j < 2 * kVec; ++j) y[j] *= inv;
+        for (int j = 0; j < 2 * kVec; ++j) z[j] = y[g][j] * inv;
       } else {
 #pragma unroll
-        for (int j = 0; j < 2 * kVec; ++j) y[j] /= s;
+        for (int j = 0; j < 2 * kVec; ++j) z[j] = y[g][j] / s;
       }
       if (!mine(at)) continue;
       char* to = rows + at * tok_stride;
       if constexpr (kVec == 8) {
-        *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(y), fp8_codes(y + 4)};
-        *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(y + 8), fp8_codes(y + 12)};
+        *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(z), fp8_codes(z + 4)};
+        *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(z + 8), fp8_codes(z + 12)};
       } else if constexpr (kVec == 4) {
-        *reinterpret_cast<u32*>(to + a) = fp8_codes(y);
-        *reinterpret_cast<u32*>(to + b) = fp8_codes(y + 4);
+        *reinterpret_cast<u32*>(to + a) = fp8_codes(z);
+        *reinterpret_cast<u32*>(to + b) = fp8_codes(z + 4);
       } else {
-        const float z[4] = {y[0], y[1], 0.f, 0.f};
         const u32 c = fp8_codes(z);
         to[a] = (char)(c & 0xff);
         to[b] = (char)(c >> 8 & 0xff);
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   using Unit = typename Rows::Unit;
   constexpr int kFly = Rows::kFly, kGroups = Rows::kGroups;
   __shared__ int first_gap;
-  __shared__ float parts[2][kFly][kWriteMaxThreads / 64];
+  __shared__ float parts[2][kWriteMaxThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = blockDim.x >> 6;
   int b, first, count;
@@ -356,44 +374,40 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   if constexpr (FP8) {
     if (w.page < 0) return;
     // (every wave runs every round: the barriers are the workgroup's)
-    for (int round = 0; round * kFly * step < 2 * n_kv; ++round) {
+    int exchange = 0;
+    for (int i0 = slot; i0 - slot < 2 * n_kv; i0 += kFly * step) {
       Unit x[kFly][kGroups];
-      float s0[kFly], a[kFly];
+      float s0[kFly];
 #pragma unroll
       for (int f = 0; f < kFly; ++f) {
-        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min((round * kFly + f) * step + slot, 2 * n_kv - 1));
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min(i0 + f * step, 2 * n_kv - 1));
         s0[f] = w.lo > 0 ? *t.scale : 0.f;
         rows.load(x[f], t.from, t.from_tok, sub0 + part);
-        a[f] = 0.f;
       }
 #pragma unroll
       for (int f = 0; f < kFly; ++f) {
-        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min((round * kFly + f) * step + slot, 2 * n_kv - 1));
+        const int i = i0 + f * step;
+        const WriteTask t = kv_task(p, w.page, kv0, n_kv, min(i, 2 * n_kv - 1));
+        const typename Rows::Turns& turns = t.value ? rows.none : rows.turns;
+        typename Rows::Values y;
+        float a = 0.f;
         for (int k = 0; k < turns_each; ++k) {
-          const int sub = sub0 + part + k * share;
           if (turns_each > 1) {
-            rows.load(x[f], t.from, t.from_tok, sub);
-            rows.angles(sub, shift);
+            rows.load(x[f], t.from, t.from_tok, sub0 + part + k * share);
+            rows.angles(sub0 + part + k * share, shift);
           }
-          a[f] = fmaxf(a[f], rows.largest(x[f], t.value ? rows.none : rows.turns));
+          rows.turn(x[f], turns, y);
+          a = fmaxf(a, rows.largest(y));
         }
-      }
-      if (share > 1) {
-#pragma unroll
-        for (int f = 0; f < kFly; ++f)
-          if (lane == 0) parts[round & 1][f][wave] = a[f];
-        __syncthreads();  // (and the earlier scale has been read by every wave)
-#pragma unroll
-        for (int f = 0; f < kFly; ++f)
-          for (int o = 0; o < share; ++o) a[f] = fmaxf(a[f], parts[round & 1][f][slot * share + o]);
-      }
-#pragma unroll
-      for (int f = 0; f < kFly; ++f) {
-        const int i = (round * kFly + f) * step + slot;
-        if (i >= 2 * n_kv) break;
-        const WriteTask t = kv_task(p, w.page, kv0, n_kv, i);
+        if (share > 1) {
+          float* mine = parts[exchange++ & 1];
+          if (lane == 0) mine[wave] = a;
+          __syncthreads();  // (and the earlier scale has been read by every wave)
+          for (int o = 0; o < share; ++o) a = fmaxf(a, mine[slot * share + o]);
+        }
+        if (i >= 2 * n_kv) continue;
         bool keeps;
-        const float s = settle(a[f], w.lo > 0, s0[f], &keeps);
+        const float s = settle(a, w.lo > 0, s0[f], &keeps);
         if (part == 0) {
           if (w.lo > 0 && !keeps) recode<D>(t.rows, t.tok, w.lo, s0[f], s, lane);
           if (lane == 0) *t.scale = s;
@@ -403,8 +417,10 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
           if (turns_each > 1) {
             rows.load(x[f], t.from, t.from_tok, sub);
             rows.angles(sub, shift);
+            rows.turn(x[f], turns, y);
+            rows.largest(y);  // (what is not finite)
           }
-          rows.put_codes(x[f], t.value ? rows.none : rows.turns, t.rows, t.tok, sub, s);
+          rows.put_codes(y, t.rows, t.tok, sub, s);
         }
       }
     }
