@@ -761,7 +761,8 @@ IA_API int ia_reserve_pages(const ia_page_state* state, const int32_t* new_token
  * Pages that no row holds afterwards are free (before the copies take theirs).  A parent
  * outside [0, rows) leaves the row empty.  ok[row] is 1, or 0 and the row empty: where the
  * partly filled page is not mapped, the length does not fit the table, or no page is free.
- * workspace: ia_reorder_workspace_size bytes.
+ * workspace: ia_reorder_workspace_size bytes, zero-filled before its first use and then left to
+ * the library; calls that share it must not overlap.
  */
 IA_API size_t ia_reorder_workspace_size(int32_t rows, int32_t cols);
 IA_API int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,

@@ -343,18 +343,19 @@ struct ReorderPlan {
   int32_t* to;     // [rows]
   int32_t* list;   // [rows]
   int32_t* table;  // [rows, cols] its pages
+  u32* ended;      // workgroups of ia_reorder_take that have ended (0 between calls)
 };
 enum { kRowStays = 0, kRowChanges = 1, kRowEmpty = 2 };
 
-// A workgroup per row and stretch of columns: the row's new pages and their counts.  The table
-// itself is read only; the counts change by sums, whose order does not matter.
-__global__ __launch_bounds__(kCopyThreads) void ia_reorder_take(Table t, ReorderPlan r, int span) {
-  const int i = blockIdx.x, tid = threadIdx.x, src = r.parents[i];
+// The row's new pages and their counts, by one workgroup a stretch of columns.  The table itself
+// is read only; the counts change by sums, whose order does not matter.
+__device__ void reorder_row(const Table& t, const ReorderPlan& r, int i, int c0, int c1, bool first) {
+  const int tid = threadIdx.x, src = r.parents[i];
   const bool exists = src >= 0 && src < t.rows;
   bool heir = src == i;
   if (exists && !heir) {
     int before = r.parents[src] == src;
-    for (int j = tid; j < i && !before; j += kCopyThreads) before = r.parents[j] == src;
+    for (int j = tid; j < i && !before; j += kPlanThreads) before = r.parents[j] == src;
     heir = !__syncthreads_or(before);
   }
   int kind = src == i ? kRowStays : exists ? kRowChanges : kRowEmpty, ok = 1, len = 0, whole = 0, from = -1;
@@ -374,15 +375,15 @@ __global__ __launch_bounds__(kCopyThreads) void ia_reorder_take(Table t, Reorder
       }
     }
   }
-  if (blockIdx.y == 0 && tid == 0) {
-    r.ok[i] = ok;
+  if (first && tid == 0) {
     r.kind[i] = kind;
     r.len[i] = len;
-    r.from[i] = from;
+    // (read by the workgroup that plans)
+    st_agent_u32(reinterpret_cast<u32*>(r.ok + i), (u32)ok);
+    st_agent_u32(reinterpret_cast<u32*>(r.from + i), (u32)from);
   }
   if (kind == kRowStays) return;
-  const int c0 = blockIdx.y * span, c1 = min(c0 + span, t.cols);
-  for (int c = c0 + tid; c < c1; c += kCopyThreads) {
+  for (int c = c0 + tid; c < c1; c += kPlanThreads) {
     const int old = t.table[i * t.stride + c];
     int pg = -1;
     if (kind == kRowChanges && (heir || c < whole)) pg = t.table[src * t.stride + c];
@@ -394,13 +395,12 @@ __global__ __launch_bounds__(kCopyThreads) void ia_reorder_take(Table t, Reorder
 }
 
 // Pages for the copies, in the rows' order.
-__global__ __launch_bounds__(kPlanThreads) void ia_reorder_plan(Table t, ReorderPlan r) {
-  __shared__ int scratch[kPlanWaves];
+__device__ void reorder_pages(const Table& t, const ReorderPlan& r, int* scratch) {
   const int tid = threadIdx.x;
   int base = 0;
   for (int i0 = 0; i0 < t.rows; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    const int need = i < t.rows && r.from[i] >= 0;
+    const int need = i < t.rows && (int)ld_agent_u32(reinterpret_cast<const u32*>(r.from + i)) >= 0;
     const int upto = wave_inclusive_scan(need);
     int before, total;
     wave_prefix(__builtin_amdgcn_readlane(upto, 63), scratch, &before, &total);
@@ -419,6 +419,25 @@ __global__ __launch_bounds__(kPlanThreads) void ia_reorder_plan(Table t, Reorder
     r.to[i] = r.list[rank];
     t.refs[r.list[rank]] = 1;
   }
+}
+
+// A workgroup per row and stretch of columns; the one that ends last plans the copies (a launch
+// of its own for that costs 3 us more).  What it reads of the others' work is stored at the
+// device's coherence point, and the counts are agent-scope atomics: no fence over a whole L2 (one
+// in every workgroup took 38 us).
+__global__ __launch_bounds__(kPlanThreads) void ia_reorder_take(Table t, ReorderPlan r, int span) {
+  __shared__ int scratch[kPlanWaves];
+  __shared__ u32 before;
+  const int c0 = blockIdx.y * span;
+  reorder_row(t, r, blockIdx.x, c0, min(c0 + span, t.cols), blockIdx.y == 0);
+  wait_memory();
+  __syncthreads();
+  if (threadIdx.x == 0) before = fetch_add_agent_u32(r.ended, 1);
+  __syncthreads();
+  if (before != gridDim.x * gridDim.y - 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  if (threadIdx.x == 0) st_agent_u32(r.ended, 0);
+  reorder_pages(t, r, scratch);
 }
 
 // y = 0: the table rows and lengths; y > 0: tensor y - 1's partly filled page
@@ -659,7 +678,7 @@ int ia_reserve_pages(const ia_page_state* state, const int32_t* new_tokens, int3
 }
 
 size_t ia_reorder_workspace_size(int32_t rows, int32_t cols) {
-  return rows > 0 && cols >= 0 ? 4 * (size_t)rows * (5 + (size_t)cols) : 0;
+  return rows > 0 && cols >= 0 ? 4 * (1 + (size_t)rows * (5 + (size_t)cols)) : 0;
 }
 
 int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tensors, int32_t n_tensors,
@@ -676,17 +695,16 @@ int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tenso
   if (!workspace || workspace_bytes < ia_reorder_workspace_size(t.rows, t.cols) ||
       reinterpret_cast<uintptr_t>(workspace) % 4)
     return fail(IA_ERR_WORKSPACE, "workspace missing or too small");
-  int32_t* w = static_cast<int32_t*>(workspace);
+  int32_t* w = static_cast<int32_t*>(workspace) + 1;
   const size_t n = t.rows;
-  const ReorderPlan r{parents, ok, w, w + n, w + 2 * n, w + 3 * n, w + 4 * n, w + 5 * n};
+  const ReorderPlan r{parents,   ok,        w,         w + n, w + 2 * n, w + 3 * n, w + 4 * n, w + 5 * n,
+                      static_cast<u32*>(workspace)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   // (a row's length and counts are written even where the table has no column)
-  const int span = 4 * kCopyThreads, spans = std::max(1, (t.cols + span - 1) / span);
-  hipLaunchKernelGGL(ia_reorder_take, dim3(t.rows, spans), dim3(kCopyThreads), 0, st, t, r, span);
+  const int span = 4 * kPlanThreads, spans = std::max(1, (t.cols + span - 1) / span);
+  if (spans > 65535) return fail(IA_ERR_UNSUPPORTED, "the table has too many columns");
+  hipLaunchKernelGGL(ia_reorder_take, dim3(t.rows, spans), dim3(kPlanThreads), 0, st, t, r, span);
   rc = check_launch("reorder");
-  if (rc) return rc;
-  hipLaunchKernelGGL(ia_reorder_plan, dim3(1), dim3(kPlanThreads), 0, st, t, r);
-  rc = check_launch("reorder plan");
   for (int at = 0; !rc && (at == 0 || at < n_tensors); at += kMaxTensors) {
     const Tensors ts = some_tensors(tensors, n_tensors, at);
     const int with_table = at == 0;

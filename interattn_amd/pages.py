@@ -11,13 +11,19 @@ Calls launch on the current stream of the tensors' device, never synchronise and
 captured.  One state's calls must be ordered (one stream).
 """
 
+import ctypes
 import functools
+import operator
+import struct
 
 import torch
 
 from . import _native as N
 from .ops import workspace_tensor
 from .prompt import check_ints, device_of, launch
+
+
+_TAIL_BYTES = ctypes.sizeof(N.PageTensor) - 8
 
 
 @functools.lru_cache(maxsize=512)
@@ -57,28 +63,32 @@ def _struct_tail(shape, stride, dtype, word):
 
 def _page_tensors(tensors, n_pages, ref):
     """C array of page tensors; ``n_pages`` None takes the first tensor's."""
-    parts, dev, last, tails = [], ref.get_device(), None, {}
-    for t in tensors:
-        shape, at = t.shape, t.data_ptr()
-        layout = (shape, t.stride(), t.dtype)
-        if layout != last:  # (a model's pools are alike)
-            if n_pages is None:
-                n_pages = shape[0] if len(shape) else 0
-            if len(shape) < 2 or shape[0] != n_pages:
-                raise ValueError(f"page tensors must be [n_pages, ...] with {n_pages} pages")
-            last, tails = layout, {}
-        word = 4 if at & 15 else 16
-        tail = tails.get(word)
-        if tail is None:
-            tail = tails[word] = _struct_tail(*layout, word)
-        if at & 3:
-            raise ValueError("pages must be 4-byte aligned")
+    dev, at = ref.get_device(), [t.data_ptr() for t in tensors]
+    if not at:
+        return None, 0, 0
+    low = functools.reduce(operator.or_, at) & 15
+    if low & 3:
+        raise ValueError("pages must be 4-byte aligned")
+    parts, known, last, tail = [], [], None, None
+    for t, p in zip(tensors, at):
+        layout = (t.shape, t.stride(), t.dtype)
+        if layout != last or low:  # (a model's pools are alike)
+            for last, tail in known if not low else ():
+                if layout == last:
+                    break
+            else:
+                shape = layout[0]
+                if n_pages is None:
+                    n_pages = shape[0] if len(shape) else 0
+                if len(shape) < 2 or shape[0] != n_pages:
+                    raise ValueError(f"page tensors must be [n_pages, ...] with {n_pages} pages")
+                last, tail = layout, _struct_tail(*layout, 4 if p & 15 else 16)
+                known.append((last, tail))
         if t.get_device() != dev:
             raise ValueError(f"page tensors must be on {ref.device}, got {t.device}")
-        parts.append(at.to_bytes(8, "little") + tail)
-    if not parts:
-        return None, 0, 0
-    return (N.PageTensor * len(parts)).from_buffer_copy(b"".join(parts)), len(parts), n_pages
+        parts += p, tail
+    n = len(at)
+    return (N.PageTensor * n).from_buffer_copy(struct.pack(f"Q{_TAIL_BYTES}s" * n, *parts)), n, n_pages
 
 
 def _state(block_table, seq_lens, refs, page_size, *others):
@@ -173,7 +183,7 @@ def reorder_sequences(tensors, block_table, seq_lens, refs, parents, *, page_siz
     ok = torch.empty_like(parents)
     lib = N.lib()
     need = max(lib.ia_reorder_workspace_size(state.rows, state.cols), 4)
-    ws = workspace_tensor(workspace, ("reorder_scratch", need), (need,), device=refs.device, dtype=torch.uint8)
+    ws = workspace_tensor(workspace, ("reorder_scratch", state.rows, state.cols), (need,), device=refs.device, dtype=torch.uint8, zero=True)
     launch(lib.ia_reorder_sequences, refs, state, desc, n_t, parents.data_ptr(), ok.data_ptr(), ws.data_ptr(),
            ws.numel())
     return ok
