@@ -17,7 +17,9 @@ import torch
 from . import _native as N
 from .ops import _DTYPE_CODE, _code, _stream, paged_kv, workspace_tensor
 
-_F32, _BF16 = torch.float32, torch.bfloat16
+_F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
+# (as ops._raw_stream: not public, and a torch without it takes the public one)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def device_of(ref, *others):
@@ -33,11 +35,9 @@ def device_of(ref, *others):
 
 def check_ints(t, name, length=None):
     """A contiguous int32 vector; returns its length."""
-    if t.dtype != torch.int32 or t.dim() != 1:
+    if t.dtype != _I32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector")
-    n = t.shape[0]
-    if n > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be a contiguous int32 vector")
+    n = t.numel()
     if length is not None and n != length:
         raise ValueError(f"{name} must have {length} entries, got {n}")
     return n
@@ -45,11 +45,13 @@ def check_ints(t, name, length=None):
 
 def launch(fn, ref, *args):
     """Call an entry point on the current stream of ``ref``'s device, with it current."""
-    if torch.cuda.current_device() == ref.get_device():
-        N.check(fn(*args, _stream(ref)))
+    if _current_device() == ref.get_device():
+        rc = fn(*args, _stream(ref))
     else:
         with torch.cuda.device(ref.device):
-            N.check(fn(*args, _stream(ref)))
+            rc = fn(*args, _stream(ref))
+    if rc:
+        N.check(rc)
 
 
 # What follows from shapes, strides and types alone is checked once per combination and kept
@@ -113,7 +115,7 @@ _POOLS = {}  # layouts of pools -> (PagedKV bytes, n_kv_heads, D)
 
 def pool_of(pool_k, pool_v, block_table, scales, n_seq):
     """``(PagedKV, n_kv_heads, D)``: ``ops.paged_kv``'s struct, its table of ``n_seq`` rows."""
-    key = [pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype]
+    key = (pool_k.shape, pool_k.stride(), pool_k.dtype, pool_v.shape, pool_v.stride(), pool_v.dtype)
     if block_table is not None:
         rows = block_table.shape
         if rows[0] != n_seq:
@@ -123,7 +125,6 @@ def pool_of(pool_k, pool_v, block_table, scales, n_seq):
     if scales is not None:
         ks, vs = scales[:2]
         key += (ks.shape, ks.stride(), ks.dtype, vs.shape, vs.stride(), vs.dtype)
-    key = tuple(key)
     held = _POOLS.get(key)
     if held is None:
         kv, _ = paged_kv(pool_k, pool_v, block_table, scales if ks is None else (ks, vs))
