@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   }
   const int64_t start = past < 0 ? 0 : past;  // (a negative length: the queries only)
   const int64_t lp = start / p.page_rows + local, base = lp * p.page_rows;
-  if (base >= start + count) return;
+  if (count == 0 || base >= start + count) return;  // (no rows: none to hold in their place either)
   WritePage w;
   w.page = past < 0 ? -1 : write_page(p, b, lp);
   w.tok = first + (base - start);

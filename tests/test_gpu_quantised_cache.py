@@ -294,6 +294,35 @@ def test_single_tokens_with_and_without_cu(device, kv):
         assert all(torch.equal(x, y) for x, y in zip(r, results[0]))
 
 
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_sequences_without_new_rows(device, kv):
+    """A begun page of a sequence that gets no rows keeps its codes and its scale, whatever the
+    rows before and behind its place in the batch are; a batch of no rows at all."""
+    announce(f"write, sequences without rows {kv}")
+    hkv, d, page = 2, 64, 16
+    past, counts = [5, 0, 8, 16, 3], [0, 3, 0, 2, 0]
+    g, pk, pv, table, scales = setup(device, 9, 5, hkv, page, d, 2, False, FP8 if kv == "fp8" else BF16)
+    if scales:
+        for s in scales:
+            s.fill_(2.0 ** -6)
+    total = sum(counts)
+    k, v, q = (torch.full((total + 1, hkv, d), 1e4, device=device, dtype=BF16)[1:] for _ in "kvq")
+    seq = torch.tensor(past, device=device, dtype=torch.int32)
+    idle = [b for b, n in enumerate(counts) if n == 0]
+    mine = table[idle].flatten().long()
+    state = [pk.view(torch.uint8), pv.view(torch.uint8), *(scales or ())]
+    before = [x.clone() for x in state]
+    plan = ia.rotary_plan(d, device=device)
+    _, lens = ia.rotary_append_kv(q, k, v, plan, pk, pv, table, seq, cu_of(counts, device), scales=scales)
+    torch.cuda.synchronize()
+    assert lens.tolist() == [a + b for a, b in zip(past, counts)]
+    assert all(torch.equal(x[mine], y[mine]) for x, y in zip(state, before))
+    before = [x.clone() for x in state]
+    _, lens = ia.rotary_append_kv(q[:0], k[:0], v[:0], plan, pk, pv, table, seq, cu_of([0] * 5, device), scales=scales)
+    torch.cuda.synchronize()
+    assert lens.tolist() == past and all(torch.equal(x, y) for x, y in zip(state, before))
+
+
 def test_missing_pages(device):
     """A position without a page is skipped, the length counts up to the first of them, and
     queries are turned all the same."""
