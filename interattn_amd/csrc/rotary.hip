@@ -116,6 +116,8 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
     const int64_t strides[4] = {x.in_token_stride, x.in_head_stride, x.out_token_stride, x.out_head_stride};
     for (int64_t s : strides)
       if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
+    if ((n_tokens > 1 && x.out_token_stride < head_dim) || (x.n_heads > 1 && x.out_head_stride < head_dim))
+      return fail(IA_ERR_INVALID, "output rows must not overlap");
     if ((reinterpret_cast<uintptr_t>(x.in) | reinterpret_cast<uintptr_t>(x.out)) % 16)
       return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
     p.t[i] = RotTensor{static_cast<const char*>(x.in), static_cast<char*>(x.out), x.in_token_stride * eb,
@@ -134,6 +136,7 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
   p.units = layout == kRowsHalfOdd ? head_dim / 2 : head_dim * eb / 32;
   p.tile = kRotThreads / p.units;
   const int64_t tiles = ((int64_t)n_tokens + p.tile - 1) / p.tile;
+  if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
   // few tokens: the heads over as many workgroups as the device runs at once
   const int64_t slices = std::min<int64_t>((all + kRotFly - 1) / kRotFly,
                                            std::max<int64_t>(1, 4 * (int64_t)device_cus() / tiles));

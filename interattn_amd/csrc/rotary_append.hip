@@ -477,6 +477,12 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   const bool in_place = n_seq > 0 && new_seq_lens == seq_lens;
   if (in_place && cu_seqlens)
     return fail(IA_ERR_INVALID, "lengths advance in place for single tokens only (cu_seqlens null)");
+  if (n_seq > 0 && positions) {
+    // (lengths are written while other waves still look for their positions)
+    const uintptr_t a = reinterpret_cast<uintptr_t>(positions), b = reinterpret_cast<uintptr_t>(new_seq_lens);
+    if (a < b + 4 * (uintptr_t)n_seq && b < a + 4 * (uintptr_t)n_tokens)
+      return fail(IA_ERR_INVALID, "positions must not overlap new_seq_lens");
+  }
   WriteParams p{};
   p.group = 1;
   if (q) {
@@ -486,6 +492,8 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
     const int64_t qs[4] = {q->in_token_stride, q->in_head_stride, q->out_token_stride, q->out_head_stride};
     for (int64_t s : qs)
       if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
+    if ((n_tokens > 1 && q->out_token_stride < head_dim) || (q->n_heads > 1 && q->out_head_stride < head_dim))
+      return fail(IA_ERR_INVALID, "output rows must not overlap");
     if ((reinterpret_cast<uintptr_t>(q->in) | reinterpret_cast<uintptr_t>(q->out)) % 16)
       return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
     p.q = static_cast<const char*>(q->in);

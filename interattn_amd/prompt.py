@@ -279,8 +279,8 @@ def read_kv(pool_k, pool_v, block_table, starts, cu_seqlens, n_tokens, *, scales
     n_seq = _n_seq(cu_seqlens)
     check_ints(starts, "starts", n_seq)
     kv, hkv, d = pool_of(pool_k, pool_v, block_table, scales, n_seq)
-    if n_tokens < 0:
-        raise ValueError("n_tokens must be >= 0")
+    if not 0 <= n_tokens < 1 << 31:
+        raise ValueError("n_tokens must be >= 0, below 2^31")
     out_dtype = out_dtype or (pool_k.dtype if pool_k.dtype in (_F32, _BF16) else _BF16)
     if out_dtype not in (_F32, _BF16):
         raise ValueError("out_dtype must be float32 or bfloat16")

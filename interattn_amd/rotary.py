@@ -178,8 +178,8 @@ def rotary_append_kv(q, k_new, v_new, plan, pool_k, pool_v, block_table, seq_len
 
     ``q [tokens, Hq, D]`` (or None), ``k_new, v_new [tokens, Hkv, D]`` packed; sequence b's rows
     ``cu_seqlens[b] ..`` are the positions ``seq_lens[b], seq_lens[b] + 1, ...`` of the pool, and
-    what they are turned to, unless ``positions [tokens] int32`` says otherwise.  ``plan`` None
-    turns nothing.  Pools are bf16 or float32 as the rows are, or fp8 with ``scales=(k_scale,
+    what they are turned to, unless ``positions [tokens] int32`` (not the tensor the lengths are
+    written to) says otherwise.  ``plan`` None turns nothing.  Pools are bf16 or float32 as the rows are, or fp8 with ``scales=(k_scale,
     v_scale)``, which the call sets: every page gets the least power of two that brings its
     largest finite magnitude down to 448; a page with earlier tokens keeps its scale while that
     is enough, else its codes are rewritten with it (exact, but for what turns subnormal).  A

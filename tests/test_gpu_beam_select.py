@@ -95,6 +95,17 @@ def test_equal_keys_go_to_the_lower_place(device, dtype):
         check(ia.beam_select(rising, scores, n), rising, scores, n)
 
 
+def test_more_equal_keys_than_fit(device):
+    """64 beams of equal rows, the best 64: thousands of keys reach the threshold."""
+    announce("beam select, 64 equal beams")
+    g = torch.Generator(device=device)
+    g.manual_seed(6)
+    scores = torch.full((2, 64), -3.0, device=device)
+    row = torch.randn((1, 3000), device=device, generator=g)
+    for logits in (row.expand(128, 3000), torch.zeros((128, 3000), device=device), row.bfloat16().repeat(128, 1)):
+        check(ia.beam_select(logits, scores, 64), logits, scores, 64)
+
+
 def test_what_offers_nothing(device):
     """-inf and NaN logits, beams of -inf or NaN scores, rows that reach +inf, rows of -inf."""
     announce("beam select, nothing offered")
@@ -162,13 +173,17 @@ def test_a_captured_selection(device):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = ia.beam_select(logits, scores, 8, workspace=ws)
+    alone = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(alone):  # (with memory of its own)
+        out += ia.beam_select(logits, scores, 8)
     for _ in range(3):
         logits.normal_(generator=g)
         scores.normal_(generator=g)
         want = ia.beam_select(logits, scores, 8)
         graph.replay()
+        alone.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(out, want * 2))
 
 
 def test_refusals(device):

@@ -196,6 +196,9 @@ def test_one_by_one_is_all_at_once(device):
     (64, 32, 32, "interleaved", 4, 2, [100, 0], [50, 33], True),
     (128, 64, 70, "half", 1, 3, [60], [75], False),
     (64, 16, 10, "interleaved", 1, 1, [0, 1], [0, 17], False),
+    (128, 128, 128, "half", 2, 1, [100, 0], [60, 128], False),        # pages of more parts than waves
+    (64, 256, 26, "half", 1, 2, [7, 250], [500, 30], False),
+    (128, 256, 64, "interleaved", 1, 1, [200], [300], True),
 ])
 def test_turned_keys_and_queries(device, kv, dtype, d, page, rot, layout, hkv, group, past, counts, paired):
     announce(f"turned write {kv} {dtype} {d} {page} {rot} {layout}")
@@ -439,6 +442,10 @@ def test_write_and_read_refusals(device):
         lambda: ia.rotary_append_kv(q, rows, rows, plan, pk, pv, table, seq, cu, scales=scales, positions=seq[:1]),
         lambda: ia.rotary_append_kv(None, rows, rows, plan, pk, pv, table, seq, cu, scales=scales, q_out=q),
         lambda: ia.rotary_append_kv(q, rows, rows, ia.rotary_plan(128, device=device), pk, pv, table, seq, cu, scales=scales),
+        lambda: ia.rotary_append_kv(q, rows, rows, plan, pk, pv, table, seq, scales=scales, positions=seq),
+        lambda: ia.rotary_append_kv(q, rows, rows, plan, pk, pv, table, seq, cu, scales=scales, positions=cu[1:], new_seq_lens=cu[1:]),
+        lambda: ia.rotary_append_kv(q, rows, rows, plan, pk, pv, table, seq, cu, scales=scales, q_out=q[:1].expand(2, 4, 64)),
+        lambda: ia.read_kv(pk, pv, table, seq, cu, 1 << 31, scales=scales),
         lambda: ia.append_prompt_kv(f32, f32, table, seq, rows, rows, cu, scales=scales),
         lambda: ia.append_kv(f32, f32, table, seq, rows, rows, scales=scales),
         lambda: ia.append_prompt_kv(pk, pv, table, seq, rows, rows, cu),

@@ -151,6 +151,28 @@ def test_strided_tables_many_tensors_no_columns(device):
     assert ok.shape == (0,)
 
 
+@pytest.mark.parametrize("rows,cols,longest", [(4, 9001, 144000), (1500, 3, 40), (2, 4097, 65552)])
+def test_wide_tables_and_many_rows(device, rows, cols, longest):
+    """Tables wider than a workgroup's stretch of columns, more rows than a workgroup's threads."""
+    announce(f"reorder, {rows} rows of {cols} pages")
+    rng = np.random.default_rng(rows)
+    lens = rng.integers(0, longest + 1, rows).tolist()
+    lens[0] = longest
+    n_pages = sum(-(-n // 16) for n in lens) + rows
+    g = torch.Generator(device=device)
+    g.manual_seed(rows)
+    table, free = np.full((rows, cols), -1, np.int32), rng.permutation(n_pages)
+    for i, n in enumerate(lens):
+        need = -(-n // 16)
+        table[i, :need], free = free[:need], free[need:]
+    refs = np.bincount(table[table >= 0], minlength=n_pages).astype(np.int32)
+    tensors = [torch.randint(0, 256, (n_pages, 1, 16, 4), device=device, generator=g).to(torch.uint8) for _ in "kv"]
+    state = [torch.from_numpy(x).to(device) for x in (table, np.array(lens, np.int32), refs)]
+    ws = {}
+    for parents in ([0] * rows, list(range(rows))[::-1], rng.integers(0, rows, rows).tolist()):
+        run(device, tensors, state, parents, 16, ws)
+
+
 def test_captured(device):
     announce("reorder, captured")
     tensors, state = make(device, 4, 6, 4, 16, [37, 20, 16, 40, 1, 33], 60)
@@ -164,13 +186,16 @@ def test_captured(device):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         ok = ia.reorder_sequences(tensors, *state, parents, page_size=16, workspace=ws)
+    alone = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(alone):  # (with memory of its own)
+        ok_too = ia.reorder_sequences(tensors, *state, parents, page_size=16)
     rng = np.random.default_rng(0)
-    for _ in range(4):
+    for step in range(4):
         parents.copy_(torch.from_numpy(rng.integers(0, 6, 6).astype(np.int32)))
         want = B.reorder(*(x.cpu().numpy() for x in state), parents.cpu().numpy(), 16)
-        graph.replay()
+        (alone if step % 2 else graph).replay()
         torch.cuda.synchronize()
-        for got, w in zip((*state, ok), want[:4]):
+        for got, w in zip((*state, ok_too if step % 2 else ok), want[:4]):
             assert np.array_equal(got.cpu().numpy(), w)
 
 

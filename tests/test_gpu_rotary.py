@@ -199,6 +199,8 @@ def test_refusals(device):
                 lambda: ia.apply_rotary(x, x[:3], pos, plan), lambda: ia.apply_rotary(x[..., :32], None, pos, plan),
                 lambda: ia.apply_rotary(x, None, pos, plan, q_out=x.bfloat16()),
                 lambda: ia.apply_rotary(x, None, pos, plan, k_out=x),
+                lambda: ia.apply_rotary(x, None, pos, plan, q_out=torch.empty_like(x[:1]).expand(4, 2, 64)),
+                lambda: ia.apply_rotary(x, None, pos, plan, q_out=torch.empty_like(x[:, :1]).expand(4, 2, 64)),
                 lambda: ia.apply_rotary(x.transpose(1, 2), None, pos, plan),
                 lambda: ia.apply_rotary(x, None, pos, ia.rotary_plan(64, device="cpu"))):
         with pytest.raises(ValueError):
