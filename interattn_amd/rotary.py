@@ -40,24 +40,30 @@ def _known(scaling, *keys):
     missing = [k for k in ("factor", "original_max_position_embeddings") if k in keys and scaling.get(k) is None]
     if missing:
         raise ValueError(f"scaling needs {missing}")
-    if scaling["factor"] <= 0:
+    if "factor" in keys and scaling["factor"] <= 0:
         raise ValueError("the scaling factor must be positive")
 
 
-def rotary_frequencies(dim, *, base=10000.0, scaling=None):
-    """``(radians per position of each pair, factor)``, in 64 bits.  ``scaling`` is a model
-    config's entry: ``rope_type`` ``"default"``, ``"linear"`` (``factor``), ``"yarn"`` (``factor``,
+def rotary_frequencies(dim, *, base=None, scaling=None):
+    """``(radians per position of each pair, factor)``, in 64 bits.  ``base`` is 10000 unless
+    given, here or as ``scaling``'s ``rope_theta``.  ``scaling`` is a model config's entry:
+    ``rope_type`` ``"default"``, ``"linear"`` (``factor``), ``"yarn"`` (``factor``,
     ``original_max_position_embeddings``, optional ``beta_fast``, ``beta_slow``, ``truncate``,
     ``attention_factor``) or ``"llama3"`` (``factor``, ``original_max_position_embeddings``,
     ``low_freq_factor``, ``high_freq_factor``)."""
     if dim < 0 or dim % 2:
         raise ValueError("the rotated channels must be an even number")
-    if base <= 0:
-        raise ValueError("base must be positive")
-    w = [float(base) ** (-2.0 * i / dim) for i in range(dim // 2)]
     scaling = dict(scaling or {})
+    theta = scaling.get("rope_theta")
+    if base is not None and theta is not None and base != theta:
+        raise ValueError(f"base {base} is not scaling's rope_theta {theta}")
+    base = float(base if base is not None else 10000.0 if theta is None else theta)
+    if not 0 < base < math.inf:
+        raise ValueError("base must be positive")
+    w = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
+        _known(scaling)
         return w, 1.0
     if kind == "linear":
         _known(scaling, "factor")
@@ -68,6 +74,8 @@ def rotary_frequencies(dim, *, base=10000.0, scaling=None):
         _known(scaling, "factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate",
                "attention_factor")
         s, context = float(scaling["factor"]), scaling["original_max_position_embeddings"]
+        if base <= 1:
+            raise ValueError("'yarn' needs a base above 1")
 
         def pair(turns):
             return dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -94,7 +102,7 @@ def rotary_frequencies(dim, *, base=10000.0, scaling=None):
     raise ValueError(f"unknown rope_type {kind!r}: 'default', 'linear', 'yarn' or 'llama3', or pass inv_freq")
 
 
-def rotary_plan(dim, *, base=10000.0, scaling=None, inv_freq=None, factor=None, layout="half", device="cuda"):
+def rotary_plan(dim, *, base=None, scaling=None, inv_freq=None, factor=None, layout="half", device="cuda"):
     """A ``RotaryPlan`` of ``dim`` channels: frequencies from ``base`` and ``scaling`` (see
     ``rotary_frequencies``), or ``inv_freq``, radians per position of each pair (numbers or a
     tensor).  ``factor`` multiplies the rotated channels (by default what ``scaling`` asks for).
@@ -104,8 +112,8 @@ def rotary_plan(dim, *, base=10000.0, scaling=None, inv_freq=None, factor=None, 
     if inv_freq is None:
         w, amplitude = rotary_frequencies(dim, base=base, scaling=scaling)
     else:
-        if scaling is not None:
-            raise ValueError("scaling is for frequencies made from base: inv_freq holds them already")
+        if scaling is not None or base is not None:
+            raise ValueError("base and scaling make frequencies: inv_freq holds them already")
         w, amplitude = [float(x) for x in inv_freq], 1.0
         if 2 * len(w) != dim:
             raise ValueError("inv_freq must hold a frequency for each of dim / 2 pairs")

@@ -76,8 +76,22 @@ def test_turns_are_whole_numbers_of_the_circle():
     assert ia.rotary_plan(8, scaling=yarn, factor=2.0, device="cpu").factor == 2.0
 
 
+def test_base_may_stand_in_the_scaling():
+    theta = {"rope_type": "default", "rope_theta": 500000.0}
+    want = ia.rotary_frequencies(16, base=500000.0)
+    assert ia.rotary_frequencies(16, scaling=theta) == want == ia.rotary_frequencies(16, base=500000, scaling=theta)
+    assert ia.rotary_frequencies(16) == ia.rotary_frequencies(16, base=10000.0)
+    assert ia.rotary_frequencies(16, scaling={"rope_type": "linear", "factor": 2.0, "rope_theta": 500000.0})[0] \
+        == [x / 2 for x in want[0]]
+
+
 @pytest.mark.parametrize("kw,text", [
     (dict(dim=7), "even"),
+    (dict(dim=8, base=10000.0, scaling={"rope_type": "default", "rope_theta": 500000.0}), "rope_theta"),
+    (dict(dim=8, scaling={"rope_type": "default", "factor": 2.0}), "factor"),
+    (dict(dim=8, base=math.inf), "base"),
+    (dict(dim=4, base=100.0, inv_freq=[1.0, 2.0]), "inv_freq"),
+    (dict(dim=4, base=1.0, scaling={"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 64}), "above 1"),
     (dict(dim=-2), "even"),
     (dict(dim=8, base=0.0), "base"),
     (dict(dim=8, layout="columns"), "layout"),
