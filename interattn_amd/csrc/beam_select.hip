@@ -516,7 +516,7 @@ BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
 }
 
 bool beam_sizes(int64_t batch, int beams, int vocab, int n, int dtype) {
-  return batch >= 0 && batch <= (1 << 20) && beams >= 1 && beams <= kMaxBeams && n >= 1 && n <= kMaxBest && vocab >= 1 &&
+  return batch >= 0 && batch <= (1 << 20) && batch * beams <= 1 << 24 && beams >= 1 && beams <= kMaxBeams && n >= 1 && n <= kMaxBest && vocab >= 1 &&
          vocab <= 1 << 30 && n <= (int64_t)beams * vocab && (dtype == IA_F32 || dtype == IA_BF16);
 }
 

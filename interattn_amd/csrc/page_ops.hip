@@ -702,7 +702,7 @@ int ia_reorder_sequences(const ia_page_state* state, const ia_page_tensor* tenso
   hipStream_t st = static_cast<hipStream_t>(stream);
   // (a row's length and counts are written even where the table has no column)
   const int span = 4 * kPlanThreads, spans = std::max(1, (t.cols + span - 1) / span);
-  if (spans > 65535) return fail(IA_ERR_UNSUPPORTED, "the table has too many columns");
+  if (spans > 65535 || (int64_t)t.rows * spans >= 1 << 22) return fail(IA_ERR_UNSUPPORTED, "the table has too many columns");
   hipLaunchKernelGGL(ia_reorder_take, dim3(t.rows, spans), dim3(kPlanThreads), 0, st, t, r, span);
   rc = check_launch("reorder");
   for (int at = 0; !rc && (at == 0 || at < n_tensors); at += kMaxTensors) {

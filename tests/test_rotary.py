@@ -306,6 +306,8 @@ def test_beam_select_of_nothing_and_its_workspace():
     size = N.lib().ia_beam_select_workspace_size
     assert size(1, 65, 100, 4, N.IA_F32) == size(1, 4, 100, 65, N.IA_F32) == 0
     assert 0 < size(1, 4, 32000, 8, N.IA_F32) <= size(4, 4, 32000, 8, N.IA_F32)
+    # (a launch holds 2^32 threads)
+    assert size(1 << 20, 16, 1000, 4, N.IA_F32) > 0 == size(1 << 20, 17, 1000, 4, N.IA_F32)
 
 
 STATE = dict(block_table=P, bt_stride=4, rows=3, cols=4, seq_lens=P, refs=P, n_pages=20, page_size=16)
@@ -323,6 +325,7 @@ def reorder_call(state={}, tensor=None, parents=P, ok=P, ws=P, nbytes=BIG):
     (dict(state=dict(seq_lens=None)), N.IA_ERR_INVALID, "null"),
     (dict(state=dict(rows=8193)), N.IA_ERR_UNSUPPORTED, "8192"),
     (dict(state=dict(page_size=0)), N.IA_ERR_INVALID, "page_size"),
+    (dict(state=dict(rows=8192, cols=1 << 22, bt_stride=1 << 22), nbytes=1 << 40), N.IA_ERR_UNSUPPORTED, "columns"),
     (dict(tensor=N.PageTensor(None, 64, 0, 0, 1, 1, 64, 16)), N.IA_ERR_INVALID, "non-null"),
     (dict(nbytes=8), N.IA_ERR_WORKSPACE, "workspace"),
     (dict(ws=None), N.IA_ERR_WORKSPACE, "workspace"),
