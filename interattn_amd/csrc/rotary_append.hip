@@ -16,7 +16,10 @@
 // for values that turn subnormal: a cache written token by token holds what one written at once
 // does.  Codes are rounded from float32, without a rounding to bf16 between.
 //
-// Bound by HBM for prompts, by its round trips (length, page, rows, scale) for single tokens.
+// Bound by HBM for prompts: 38k tokens of 8 kv heads of 128 and groups of 4, bf16 rows, are read
+// and written in 162 us into fp8 pages (856 MB, 5.3 TB/s) and 164 us into bf16 ones (5.7 TB/s);
+// 3.5k tokens of 4 heads of 64 in 11.5 us.  Bound by its round trips (length, page, rows, scale)
+// for single tokens: 32 sequences in 8.5 us, 6.6 without scales.
 #include <algorithm>
 
 #include "packed_rows.hpp"
@@ -29,7 +32,7 @@ int check_kv(const ia_paged_kv* kv, int d);
 namespace {
 
 constexpr int kWriteThreads = 256, kWriteMaxThreads = 512;
-constexpr int kWriteBytes = 96 << 10;
+constexpr int kWriteBytes = 48 << 10, kWriteBytesFp8 = 96 << 10;
 constexpr int kSub = 16;  // rows of a page taken at a time
 constexpr float kLargestCode = 448.f;
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
@@ -56,7 +59,7 @@ struct WriteParams {
   const int32_t* seq_lens;
   int32_t* new_lens;
   const int32_t* positions;  // null: the place in the sequence
-  int32_t n_seq, n_tokens, n_kv_heads, group, kv_heads_per_wg;
+  int32_t n_seq, n_tokens, n_kv_heads, group, kv_heads_per_wg, slices;
   RotaryArgs rot;
   bool stream;  // the queries' rows are written past the caches
 };
@@ -285,23 +288,26 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   __shared__ float parts[2][kWriteMaxThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = blockDim.x >> 6;
+  // slices of a tile are neighbours, as their rows are in memory (with one slice of every tile
+  // behind another, pages of 64 took 207 us instead of 164, pages of 16 165 instead of 162)
+  const int tile = blockIdx.x / p.slices, slice = blockIdx.x - tile * p.slices;
   int b, first, count;
   int64_t local;
   if (p.cu) {
-    const PackedTile t = packed_tile(p.cu, p.n_seq, p.n_tokens, p.page_rows, blockIdx.x, lane, 2);
+    const PackedTile t = packed_tile(p.cu, p.n_seq, p.n_tokens, p.page_rows, tile, lane, 2);
     b = t.b;
     first = t.first;
     count = t.count;
     local = t.local;
   } else {
-    b = blockIdx.x;
+    b = tile;
     first = b;
     count = 1;
     local = 0;
   }
   if (local < 0) return;
   const int64_t past = p.seq_lens[b];
-  if (local == 0 && blockIdx.y == 0) {
+  if (local == 0 && slice == 0) {
     // the length: up to the first position without a page
     if (tid == 0) first_gap = INT32_MAX;
     __syncthreads();  // (and every thread has read the length, which may be written in place)
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   w.lo = (int)(start > base ? start - base : 0);
   w.hi = (int)(start + count - base < p.page_rows ? start + count - base : p.page_rows);
   const int64_t shift = past - first;  // a token's position less its packed row
-  const int kv0 = blockIdx.y * p.kv_heads_per_wg, n_kv = min(kv0 + p.kv_heads_per_wg, p.n_kv_heads) - kv0;
+  const int kv0 = slice * p.kv_heads_per_wg, n_kv = min(kv0 + p.kv_heads_per_wg, p.n_kv_heads) - kv0;
   const int n_q = p.q ? n_kv * p.group : 0;
 
   // parts with new rows: 1, 2 or up to 4 waves share a head's page, each with a part of its own;
@@ -391,7 +397,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
         const typename Rows::Turns& turns = t.value ? rows.none : rows.turns;
         typename Rows::Values y;
         float a = 0.f;
-        for (int k = 0; k < turns_each; ++k) {
+        for (int k = 0; k < turns_each && i < 2 * n_kv; ++k) {
           if (turns_each > 1) {
             rows.load(x[f], t.from, t.from_tok, sub0 + part + k * share);
             rows.angles(sub0 + part + k * share, shift);
@@ -538,22 +544,25 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
                      rotary ? rotary->dim : 0, rotary ? rotary->factor : 1.f, 1.f};
   const int64_t tiles = cu_seqlens ? (int64_t)n_tokens / p.page_rows + 2 * (int64_t)n_seq : n_seq;
   if (tiles >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
-  // A workgroup takes about kWriteBytes of rows: with 8 kv heads of 128 bf16 and groups of 4,
-  // pages of 16 (36k tokens into fp8) took 193 us with all heads to a workgroup, 183 with half
-  // of them and 220 with a quarter; pages of 64 227, 217 and 210; heads of 64 99, 119 and 176.
+  // A workgroup takes about kWriteBytes of rows, into 8 bits about as many K and V rows as its
+  // waves have in flight: 38k tokens of 8 kv heads of 128 bf16 and groups of 4 into pages of 16
+  // took 162 us with half of the heads to a workgroup, 177 with all and 177 with a quarter; into
+  // bf16 pages 176 with half, 190 with all, 164 with a quarter and 212 with one.
   // Few tiles: a workgroup for each kv head.  Lengths that advance in place are read by one
   // workgroup only, of as many waves as it has tasks.
   int threads = kWriteThreads;
   const int64_t head_rows = (int64_t)p.page_rows * (2 + (q ? p.group : 0)) * head_dim * eb;
-  const int64_t slices = tiles >= 2 * device_cus() ? std::max<int64_t>(1, n_kv_heads * head_rows / kWriteBytes) : n_kv_heads;
-  p.kv_heads_per_wg = (int)((n_kv_heads + std::min<int64_t>(slices, n_kv_heads) - 1) / std::min<int64_t>(slices, n_kv_heads));
+  int64_t slices = n_kv_heads;
+  if (tiles >= 2 * device_cus())
+    slices = std::clamp<int64_t>(n_kv_heads * head_rows / (fp8 ? kWriteBytesFp8 : kWriteBytes), 1, n_kv_heads);
+  p.kv_heads_per_wg = (int)((n_kv_heads + slices - 1) / slices);
   if (in_place) {
     p.kv_heads_per_wg = n_kv_heads;
     threads = (2 + (q ? p.group : 0)) * n_kv_heads > 4 ? kWriteMaxThreads : kWriteThreads;
   }
-  const int64_t ny = (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg;
-  if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
-  const dim3 grid((unsigned)tiles, (unsigned)ny), block((unsigned)threads);
+  p.slices = (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg;
+  if (tiles * p.slices >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  const dim3 grid((unsigned)(tiles * p.slices)), block((unsigned)threads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int layout = rotary_layout(rotary, eb);
   p.stream = stream_rows(rotary, layout, (int64_t)n_tokens * p.group * n_kv_heads * head_dim * eb, eb);
