@@ -229,7 +229,7 @@ inline int rotary_layout(const ia_rotary* r, int elem_bytes) {
 
 // Whether rows of this size are better written past the caches: more than the L2s hold (dirty
 // lines are written back when the kernel ends: 24,001 tokens of 36 heads 93 us, past them 86),
-// and no chunk that ends inside a 64-byte sector (halves of 96 bytes: 108 us, past them 144).
+// and no chunk that ends inside a 64-byte sector (halves of 96 bytes: 103 us, past them 143).
 inline bool stream_rows(const ia_rotary* r, int layout, int64_t bytes, int elem_bytes) {
   return bytes > (32 << 20) && !(layout != kRowsInterleaved && r && r->dim / 2 * elem_bytes % 64);
 }
