@@ -5,16 +5,17 @@
 // ia_beam_scan, one launch, one pass over the logits.  A wave takes a slice of a row, groups of
 // four 16-byte loads a lane, and keeps sum exp(x - M) against a reference M near its running
 // maximum, and the slice's n best logits (the order inside a row is that of the keys).  What is
-// below the n-th largest of the lanes' running maxima (found bit by bit with ballots) cannot be
-// among them, so a group is one comparison unless it holds something better; candidates wait in
-// LDS and are cut to the n best when they fill up.  The workgroup that ends last of a batch entry
+// below the n-th largest of the lanes' running maxima (found bit by bit with ballots, and over
+// the slices of a row that a workgroup holds) cannot be among them, so a group is one comparison
+// unless it holds something better; candidates wait in LDS and are cut to the n best when they
+// fill up.  The workgroup that ends last of a batch entry
 // joins the slices' sums, forms the candidates' keys in 64 bits (float32 keys of magnitude 10
 // would order equal what differs by 10^-6) and ranks those above a threshold.  Slices are handed
 // over through memory at the device's coherence point (ia_common.hpp).
 //
 // Equal keys go to the lower beam * vocabulary + token.
 //
-// 512 rows of 128,000 bf16 logits take 42 us (131 MB; 26 us at the rate of a copy): the vector
+// 512 rows of 128,000 bf16 logits take 39 us (131 MB; 26 us at the rate of a copy): the vector
 // units issue for about two thirds of the time (an exp is four instructions' worth, and takes as
 // long as all else of an element together) and the merge behind the last row is 7 us of waiting.
 // Short calls are a chain of round trips: the scan 7 us (its first loads 3, the cut of the
@@ -31,12 +32,13 @@ constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kFly = 4;              // chunks of a group, and in flight
 constexpr int kHeld = 640;           // candidates a wave holds: a chunk's 512 and some
 constexpr int kTrim = 128;           // candidates at which they are cut to the n best
-constexpr int kWorthFloor = 8;       // lanes with something better for which the floor is raised
+constexpr int kWorthFloor = 2;       // lanes with something better for which the floor is raised
 constexpr int kMaxSlices = 64;       // of a row: a lane each in the merge
 constexpr int kMaxBeams = 64, kMaxBest = 64;
 constexpr int kOwn = 8;              // candidates a merging thread keeps in registers
 constexpr int kMaxCandidates = kOwn * kScanThreads;  // of a batch entry, where a slice a row is fewer
 constexpr int kNear = 1024;          // of those above the threshold, in LDS; more go through memory
+constexpr u32 kLowest = 0x00800000u; // the key of the lowest finite float
 constexpr int kWaves = 2048;         // of a call, where slices are long
 
 // Floats as integers of the same order (-0 before +0).
@@ -161,10 +163,11 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // 16 bytes at any e
   u32x4_t w;
 };
 
-// One slice of one row: its candidates and sum, handed over.
+// One slice of one row: its candidates and sum, handed over.  shares[w0 .. w1): the workgroup's
+// slices of the row, each with the order_key that its part of n values reach (`wave` this one).
 template <typename T>
-__device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held, int64_t row, int slice, int64_t id,
-                                           int lane) {
+__device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held, u32* shares, int w0, int w1, int wave,
+                                           int64_t row, int slice, int64_t id, int lane) {
   constexpr int kVec = RowVec<T>::kVec, kChunk = 64 * kVec;
   const T* x0 = reinterpret_cast<const T*>(p.logits + row * p.row_stride);
   const int chunks = (p.vocab + kChunk - 1) / kChunk;
@@ -191,7 +194,19 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
   auto load = [&](int c) {
     return __builtin_nontemporal_load(&reinterpret_cast<const Loose<T>*>(x0 + (c * kChunk + lane * kVec))->w);
   };
+  const int part_of_n = (n + w1 - w0 - 1) / (w1 - w0);
+  // n of the row's values reach the least of the shares
+  auto joint = [&]() {
+    u32 k = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+      const u32 x = __hip_atomic_load(shares + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (w >= w0 && w < w1) k = min(k, x);
+    }
+    return k;
+  };
   auto take = [&](const u32x4_t* w, int c) {
+    const u32 reached = joint();
     float most[kFly], all = kNegInf;
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
@@ -229,14 +244,24 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
       }
     }
     sum += (double)part;
+    // (equal ones stay: theirs may be the lower place)
+    lo = fmaxf(lo, order_value(reached));
     const unsigned long long hits = __ballot(all >= lo);
     if (!hits) return;
     seen = fmaxf(seen, all);
-    // n values of n lanes reach the floor; a few better values are not worth a new one
+    // n values of n lanes reach the floor; a single better value is not worth a new one.  The
+    // row's n values are sought over all of its slices here: four waves that share them meet a
+    // third of the candidates (512 rows of 128,000, n of 16: 39 us, each for itself 44; 64 x 8 of
+    // 16,384: 17 and 20; slices of two groups with n of 5 lose half a microsecond)
     u32 floor_ = 0;
     if (__popcll(hits) >= kWorthFloor) {
-      floor_ = nth_of_lanes<16>(order_key(seen + 0.f), n);
-      lo = fmaxf(lo, order_value(floor_));
+      const u32 mine = order_key(seen + 0.f);
+      if (w1 - w0 > 1) {
+        const u32 share = nth_of_lanes<16>(mine, part_of_n);
+        if (lane == 0) __hip_atomic_store(shares + wave, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+      if (reached == kLowest) floor_ = nth_of_lanes<16>(mine, n);  // (not every slice has a share yet)
+      lo = fmaxf(lo, order_value(max(floor_, joint())));
     }
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
@@ -260,7 +285,7 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
       }
     }
     // n values at lower places reach the floor: from here on only what is above it counts
-    if (floor_ > order_key(-3.402823466e38f)) lo = fmaxf(lo, above(floor_));
+    if (floor_ > kLowest) lo = fmaxf(lo, above(floor_));
   };
 
   // whole groups, one ahead (the last is loaded twice: a load under a condition would make every
@@ -470,13 +495,18 @@ __global__ __launch_bounds__(kScanThreads) void ia_beam_scan(BeamParams p) {
     Candidate held[kScanWaves][kHeld];
     MergeLds merge;
   } lds;
-  __shared__ u32 before;
+  __shared__ u32 before, shares[kScanWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x / p.groups, local = (blockIdx.x - b * p.groups) * kScanWaves + wave;
+  if (threadIdx.x < kScanWaves) shares[threadIdx.x] = kLowest;
+  __syncthreads();
   if (local < p.beams * p.slices) {
     const int j = local / p.slices, slice = local - j * p.slices;
     const int64_t row = (int64_t)b * p.beams + j;
-    if (!p.done || !p.done[row]) scan_slice<T>(p, lds.held[wave], row, slice, row * p.slices + slice, lane);
+    if (!p.done || !p.done[row]) {
+      const int w0 = max(wave - slice, 0), w1 = min(wave - slice + p.slices, kScanWaves);
+      scan_slice<T>(p, lds.held[wave], shares, w0, w1, wave, row, slice, row * p.slices + slice, lane);
+    }
   }
   // the workgroup that ends last merges
   wait_memory();
@@ -495,18 +525,20 @@ struct BeamPlan {
 };
 
 // Slices of a row: up to kWaves waves in all with two groups a slice, up to half as many with
-// one, and no more candidates for a batch entry than a merging workgroup holds in registers.  A
-// wave's first group and its last cut of the candidates cost about 4 us, so that more waves are
-// not faster: 512 rows of 128,000 take 42 us in 2,048 waves, 43 in 4,096, 55 in 8,192 and 69 in
-// 1,024, where too few loads are in flight; 512 of 16,384 19 in 2,048 and 4,096, 22 in 8,192; 80
-// of 50,021 14.8 with two groups a slice and 16.6 with one.
+// one, as many as fill a batch entry's workgroup, and no more candidates for a batch entry than a
+// merging workgroup holds in registers.  A wave's first group and its last cut of the candidates
+// cost about 4 us, so that more waves are not faster: 512 rows of 128,000 take 39 us in 2,048
+// waves, 41 in 4,096, 51 in 8,192 and 50 in 1,024, where too few loads are in flight; 512 of
+// 16,384 17.5 in 2,048 and 4,096, 20.7 in 8,192; 80 of 50,021 15.4 with two groups a slice and
+// 16.7 with one.  4,096 entries of one beam of 32,000 take 84 us with a workgroup's four waves on
+// the row, 149 with one of them.
 BeamPlan beam_plan(int64_t batch, int beams, int vocab, int n, int elem_bytes) {
   BeamPlan r{};
   const int64_t rows = batch * beams;
   const int64_t chunk = 64 * (16 / elem_bytes), chunks = (vocab + chunk - 1) / chunk;
   const int64_t per_row = kWaves / std::max<int64_t>(rows, 1);
   int64_t s = std::max(std::min(per_row, chunks / (2 * kFly)), std::min(per_row / 2, (chunks + kFly - 1) / kFly));
-  s = std::max<int64_t>(s, 1);
+  s = std::max({s, std::min<int64_t>((kScanWaves + beams - 1) / beams, chunks / kFly), (int64_t)1});
   s = std::min<int64_t>(s, std::max(1, std::min(kMaxSlices, kMaxCandidates / (beams * n))));
   r.slice_chunks = (int)align_up((chunks + s - 1) / s, kFly);
   r.slices = (int)((chunks + r.slice_chunks - 1) / r.slice_chunks);
