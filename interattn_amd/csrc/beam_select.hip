@@ -16,10 +16,11 @@
 // Equal keys go to the lower beam * vocabulary + token.
 //
 // 512 rows of 128,000 bf16 logits take 39 us (131 MB; 26 us at the rate of a copy): the vector
-// units issue for about two thirds of the time (an exp is four instructions' worth, and takes as
-// long as all else of an element together) and the merge behind the last row is 7 us of waiting.
-// Short calls are a chain of round trips: the scan 7 us (its first loads 3, the cut of the
-// candidates 4), handing over 2.5, the merge 6: 80 rows of 50,021 take 15 us, 4 of 32,000 10.
+// units are busy for half of the time (an exp takes as long as four other instructions, as much as
+// all else of an element), with two waves a SIMD to cover the branches of the candidates, and the
+// merge behind the last row is 7 us of waiting.  Short calls are a chain of round trips: the scan
+// 7 us (its first loads 3, the cut of the candidates 4), handing over 2.5, the merge 6: 80 rows
+// of 50,021 take 15 us, 4 of 32,000 10.
 #include <algorithm>
 
 #include "rotary.hpp"
