@@ -54,6 +54,7 @@ def check(got, logits, scores, n, done=None, pad=0):
 @pytest.mark.parametrize("batch,beams,vocab,n,pad_cols", [
     (1, 1, 1, 1, 0), (1, 1, 7, 7, 0), (3, 2, 5, 10, 1), (1, 4, 32000, 8, 0), (2, 5, 50021, 5, 3), (2, 1, 513, 64, 7),
     (1, 64, 1000, 64, 0), (5, 3, 511, 3, 0), (40, 8, 2049, 16, 1), (1, 2, 131072, 33, 0),
+    (2100, 1, 4100, 5, 0), (800, 3, 5001, 7, 2), (300, 1, 20000, 16, 0), (24, 7, 30000, 64, 0),
 ])
 def test_best_continuations(device, dtype, batch, beams, vocab, n, pad_cols):
     """Odd vocabularies, rows that begin at any element."""
@@ -104,6 +105,27 @@ def test_more_equal_keys_than_fit(device):
     row = torch.randn((1, 3000), device=device, generator=g)
     for logits in (row.expand(128, 3000), torch.zeros((128, 3000), device=device), row.bfloat16().repeat(128, 1)):
         check(ia.beam_select(logits, scores, 64), logits, scores, 64)
+
+
+@pytest.mark.parametrize("n", [1, 3, 16])
+def test_best_that_lie_in_one_slice(device, n):
+    """All of a row's best at its end, at its start, and one equal value in every stretch: what the
+    slices of a row learn of each other must not cost a candidate."""
+    announce(f"beam select, uneven slices, {n} best")
+    g = torch.Generator(device=device)
+    g.manual_seed(n)
+    logits = torch.randn((4 * 3, 60000), device=device, generator=g)
+    logits[0, -40:] += 30
+    logits[1, :40] += 30
+    logits[2, 5::997] = 9.0
+    logits[3] = logits[3].sort().values
+    logits[4] = logits[4].sort(descending=True).values
+    logits[5, 30000:30040] = 20.0
+    logits[6:9] = logits[2] + torch.tensor([[0.0], [1.0], [-2.0]], device=device)
+    logits[9, ::2] = -1e30
+    scores = torch.zeros((4, 3), device=device)
+    for x in (logits, logits.bfloat16()):
+        check(ia.beam_select(x, scores, n), x, scores, n)
 
 
 def test_what_offers_nothing(device):
