@@ -400,7 +400,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
         for (int k = 0; k < turns_each && i < 2 * n_kv; ++k) {
           if (turns_each > 1) {
             rows.load(x[f], t.from, t.from_tok, sub0 + part + k * share);
-            rows.angles(sub0 + part + k * share, shift);
+            if (!t.value) rows.angles(sub0 + part + k * share, shift);
           }
           rows.turn(x[f], turns, y);
           a = fmaxf(a, rows.largest(y));
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
           const int sub = sub0 + part + k * share;
           if (turns_each > 1) {
             rows.load(x[f], t.from, t.from_tok, sub);
-            rows.angles(sub, shift);
+            if (!t.value) rows.angles(sub, shift);
             rows.turn(x[f], turns, y);
             rows.largest(y);  // (what is not finite)
           }
