@@ -1,10 +1,11 @@
 // Keys rotated into the paged pool, values into the pool, queries rotated out, for gfx950:
 // the write side of a serving step, into bf16, f32 and fp8 pages.
 //
-// A workgroup per (sequence, page its new tokens touch, slice of heads).  A wave takes one
+// Packed rows: a workgroup per (sequence, page its new tokens touch, slice of heads).  A wave takes one
 // head's rows of the page, 16 at a time (a part), as units of VEC pairs: lane = (row, unit), so
 // that the angles of its rows are computed once and serve every head, and a pair turns inside a
-// lane.  Pages of up to four parts give each part a wave of its own.
+// lane.  Pages of up to four parts give each part a wave of its own.  Single tokens: a workgroup
+// per sequence, several rows a wave.
 //
 // fp8 pages have one float32 scale per (page, kv head).  The waves that hold the page's new
 // rows take the largest magnitude a of its finite values (a reduction inside a wave, and over
@@ -19,7 +20,8 @@
 // Bound by HBM for prompts: 38k tokens of 8 kv heads of 128 and groups of 4, bf16 rows, are read
 // and written in 162 us into fp8 pages (856 MB, 5.3 TB/s) and 164 us into bf16 ones (5.7 TB/s);
 // 3.5k tokens of 4 heads of 64 in 11.5 us.  Bound by its round trips (length, page, rows, scale)
-// for single tokens: 32 sequences in 8.5 us, 6.6 without scales.
+// for single tokens: 1 to 256 sequences of 48 heads into fp8 pages in 4.4 to 5.1 us, 2,048 in 23
+// (through the packed rows' kernel 8.2 to 25 and 71).
 #include <algorithm>
 
 #include "packed_rows.hpp"
@@ -31,7 +33,8 @@ int check_kv(const ia_paged_kv* kv, int d);
 
 namespace {
 
-constexpr int kWriteThreads = 256, kWriteMaxThreads = 512;
+constexpr int kWriteThreads = 256, kWaves = kWriteThreads / 64;
+constexpr int kTokenThreads = 1024;  // at most, of a workgroup for one token
 constexpr int kWriteBytes = 48 << 10, kWriteBytesFp8 = 96 << 10;
 constexpr int kSub = 16;  // rows of a page taken at a time
 constexpr float kLargestCode = 448.f;
@@ -55,7 +58,7 @@ struct WriteParams {
   int64_t bt_stride, bt_cols, n_pages;
   int32_t page_rows;
   // batch
-  const int32_t* cu;  // null: one token per sequence
+  const int32_t* cu;
   const int32_t* seq_lens;
   int32_t* new_lens;
   const int32_t* positions;  // null: the place in the sequence
@@ -90,13 +93,13 @@ __device__ __forceinline__ u32 fp8_codes(const float* x) {
 // Not finite: NaN, which has a code (infinity has none).
 __device__ __forceinline__ float or_nan(float x) { return finite(x) ? x : __uint_as_float(0x7fc00000u); }
 
-// The earlier rows [0, n) of one head's page from scale s0 to s.
-template <int D>
+// The earlier rows [0, n) of one head's page from scale s0 to s, by LANES lanes.
+template <int D, int LANES>
 __device__ void recode(char* rows, int64_t tok_stride, int n, float s0, float s, int lane) {
   const float ratio = s0 / s;
-  constexpr int kLanes = D / 16;
-  for (int r = lane / kLanes; r < n; r += 64 / kLanes) {
-    u32x4_t* at = reinterpret_cast<u32x4_t*>(rows + r * tok_stride + lane % kLanes * 16);
+  constexpr int kChunks = D / 16;
+  for (int i = lane; i < n * kChunks; i += LANES) {
+    u32x4_t* at = reinterpret_cast<u32x4_t*>(rows + i / kChunks * tok_stride + i % kChunks * 16);
     u32x4_t w = *at;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -108,6 +111,43 @@ __device__ void recode(char* rows, int64_t tok_stride, int n, float s0, float s,
     }
     *at = w;
   }
+}
+
+// A unit's elements y as codes over the scale s, inv its reciprocal where that is exact (0 where
+// not).
+template <int LAYOUT, int VEC>
+__device__ __forceinline__ void put_unit_codes(char* to, int u, int rot, int d, const float* y, float s, float inv) {
+  int a, b;
+  unit_chunks<LAYOUT, VEC>(u, rot, d, &a, &b);
+  float z[2 * VEC < 4 ? 4 : 2 * VEC] = {};
+  if (inv != 0.f) {
+#pragma unroll
+    for (int j = 0; j < 2 * VEC; ++j) z[j] = y[j] * inv;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2 * VEC; ++j) z[j] = y[j] / s;
+  }
+  if constexpr (VEC == 8) {
+    *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(z), fp8_codes(z + 4)};
+    *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(z + 8), fp8_codes(z + 12)};
+  } else if constexpr (VEC == 4) {
+    *reinterpret_cast<u32*>(to + a) = fp8_codes(z);
+    *reinterpret_cast<u32*>(to + b) = fp8_codes(z + 4);
+  } else {
+    const u32 c = fp8_codes(z);
+    to[a] = (char)(c & 0xff);
+    to[b] = (char)(c >> 8 & 0xff);
+  }
+}
+
+// (a power of two is divided by exactly through its reciprocal)
+__device__ __forceinline__ float exact_inverse(float s) { return (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f; }
+
+// The scale for new values of magnitude a of a page whose scale was s0; keeps: the earlier
+// codes stay as they are.
+__device__ __forceinline__ float settle(float a, bool begun, float s0, bool* keeps) {
+  *keeps = begun && finite(s0) && s0 >= kLeastScale && a <= kLargestCode * s0;
+  return *keeps ? s0 : page_scale(a);
 }
 
 // One page of one sequence, as all of its tasks see it.
@@ -217,34 +257,11 @@ struct PageRows {
 
   // as e4m3 codes over the scale s
   __device__ __forceinline__ void put_codes(const Values& y, char* rows, int64_t tok_stride, int sub, float s) const {
-    // (a power of two is divided by exactly through its reciprocal)
-    const float inv = (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
-    int a, b;
-    unit_chunks<LAYOUT, kVec>(unit, p.rot.rot, D, &a, &b);
+    const float inv = exact_inverse(s);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int at = place(sub, g);
-      float z[2 * kVec < 4 ? 4 : 2 * kVec] = {};
-      if (inv != 0.f) {
-#pragma unroll
-        for (int j = 0; j < 2 * kVec; ++j) z[j] = y[g][j] * inv;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2 * kVec; ++j) z[j] = y[g][j] / s;
-      }
-      if (!mine(at)) continue;
-      char* to = rows + at * tok_stride;
-      if constexpr (kVec == 8) {
-        *reinterpret_cast<u32x2_t*>(to + a) = u32x2_t{fp8_codes(z), fp8_codes(z + 4)};
-        *reinterpret_cast<u32x2_t*>(to + b) = u32x2_t{fp8_codes(z + 8), fp8_codes(z + 12)};
-      } else if constexpr (kVec == 4) {
-        *reinterpret_cast<u32*>(to + a) = fp8_codes(z);
-        *reinterpret_cast<u32*>(to + b) = fp8_codes(z + 4);
-      } else {
-        const u32 c = fp8_codes(z);
-        to[a] = (char)(c & 0xff);
-        to[b] = (char)(c >> 8 & 0xff);
-      }
+      if (mine(at)) put_unit_codes<LAYOUT, kVec>(rows + at * tok_stride, unit, p.rot.rot, D, y[g], s, inv);
     }
   }
 };
@@ -272,45 +289,26 @@ __device__ __forceinline__ WriteTask kv_task(const WriteParams& p, int64_t page,
   return t;
 }
 
-// The scale for new values of magnitude a of a page whose scale was s0; keeps: the earlier
-// codes stay as they are.
-__device__ __forceinline__ float settle(float a, bool begun, float s0, bool* keeps) {
-  *keeps = begun && finite(s0) && s0 >= kLeastScale && a <= kLargestCode * s0;
-  return *keeps ? s0 : page_scale(a);
-}
-
 template <typename T, bool FP8, int D, int LAYOUT>
-__global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p) {
+__global__ __launch_bounds__(kWriteThreads) void ia_write_pages(WriteParams p) {
   using Rows = PageRows<T, D, LAYOUT>;
   using Unit = typename Rows::Unit;
   constexpr int kFly = Rows::kFly, kGroups = Rows::kGroups;
   __shared__ int first_gap;
-  __shared__ float parts[2][kWriteMaxThreads / 64];
+  __shared__ float parts[2][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int waves = blockDim.x >> 6;
   // slices of a tile are neighbours, as their rows are in memory (with one slice of every tile
   // behind another, pages of 64 took 207 us instead of 164, pages of 16 165 instead of 162)
   const int tile = blockIdx.x / p.slices, slice = blockIdx.x - tile * p.slices;
-  int b, first, count;
-  int64_t local;
-  if (p.cu) {
-    const PackedTile t = packed_tile(p.cu, p.n_seq, p.n_tokens, p.page_rows, tile, lane, 2);
-    b = t.b;
-    first = t.first;
-    count = t.count;
-    local = t.local;
-  } else {
-    b = tile;
-    first = b;
-    count = 1;
-    local = 0;
-  }
+  const PackedTile own = packed_tile(p.cu, p.n_seq, p.n_tokens, p.page_rows, tile, lane, 2);
+  const int b = own.b, first = own.first, count = own.count;
+  const int64_t local = own.local;
   if (local < 0) return;
   const int64_t past = p.seq_lens[b];
   if (local == 0 && slice == 0) {
     // the length: up to the first position without a page
     if (tid == 0) first_gap = INT32_MAX;
-    __syncthreads();  // (and every thread has read the length, which may be written in place)
+    __syncthreads();
     const int64_t end = past + count;
     if (past >= 0 && count > 0)
       for (int64_t lp = past / p.page_rows + tid; lp * p.page_rows < end; lp += blockDim.x)
@@ -343,8 +341,8 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   // parts with new rows: 1, 2 or up to 4 waves share a head's page, each with a part of its own;
   // with more parts each wave goes through several
   const int sub0 = w.lo / kSub, subs = (w.hi + kSub - 1) / kSub - sub0;
-  const int share = subs == 1 || waves < 2 ? 1 : subs == 2 || waves < 4 ? 2 : 4;
-  const int step = waves / share, slot = wave / share, part = wave % share;
+  const int share = subs == 1 ? 1 : subs == 2 ? 2 : 4;
+  const int step = kWaves / share, slot = wave / share, part = wave % share;
   const int turns_each = (subs + share - 1) / share;
   Rows rows(p, w, lane);
   for (int k = 0; k < turns_each; ++k) {
@@ -415,7 +413,7 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
         bool keeps;
         const float s = settle(a, w.lo > 0, s0[f], &keeps);
         if (part == 0) {
-          if (w.lo > 0 && !keeps) recode<D>(t.rows, t.tok, w.lo, s0[f], s, lane);
+          if (w.lo > 0 && !keeps) recode<D, 64>(t.rows, t.tok, w.lo, s0[f], s, lane);
           if (lane == 0) *t.scale = s;
         }
         for (int k = 0; k < turns_each; ++k) {
@@ -433,22 +431,94 @@ __global__ __launch_bounds__(kWriteMaxThreads) void ia_write_pages(WriteParams p
   }
 }
 
+// One token of one sequence by a workgroup: a unit of a row (a query, key or value head) a lane,
+// several rows a wave, so that the call is the chain length -> page -> scale and everything else
+// (rows, frequencies) is loaded beside it.
+template <typename T, bool FP8, int D, int LAYOUT>
+__global__ __launch_bounds__(kTokenThreads) void ia_write_tokens(WriteParams p) {
+  using Unit = RowUnit<T, LAYOUT>;
+  constexpr int kVec = Unit::kVec, kUnits = D / (2 * kVec);
+  const int b = blockIdx.x, tid = threadIdx.x, unit = tid % kUnits;
+  const int64_t past = p.seq_lens[b];
+  const int n_q = p.q ? p.group * p.n_kv_heads : 0, n_rows = n_q + 2 * p.n_kv_heads, step = blockDim.x / kUnits;
+  int64_t page = -1, lp = 0;
+  float cs[kVec], sn[kVec];
+  for (int r = tid / kUnits; r < n_rows; r += step) {
+    const bool query = r < n_q, value = r >= n_q + p.n_kv_heads;
+    const int64_t h = query ? r : value ? r - n_q - p.n_kv_heads : r - n_q;
+    const char* from = query ? p.q + b * p.q_tok + h * p.q_head
+                             : value ? p.v_new + b * p.vn_tok + h * p.vn_head : p.k_new + b * p.kn_tok + h * p.kn_head;
+    Unit x;
+    x.template load<false>(reinterpret_cast<const T*>(from), unit, p.rot.rot, D);
+    if (r < step) {  // (the first of the lane's rows: behind its load)
+      if (past >= 0) {
+        lp = past / p.page_rows;
+        page = write_page(p, b, lp);
+      }
+      unit_angles<LAYOUT, kVec>(p.rot, p.positions ? p.positions[b] : (int)past,
+                                typename Unit::Turns(unit, p.rot.rot, D), cs, sn);
+    }
+    const int lo = (int)(past - lp * p.page_rows);
+    char* rows = value ? p.v + page * p.v_page + h * p.v_head : p.k + page * p.k_page + h * p.k_head;
+    const int64_t tok = value ? p.v_tok : p.k_tok;
+    float* scale = (value ? p.v_scale : p.k_scale) + page * p.scale_page + h;
+    const bool writes = !query && page >= 0;
+    float s0 = 0.f;
+    if (FP8 && writes && lo > 0) s0 = *scale;
+    float y[2 * kVec];
+    x.turned(cs, sn, typename Unit::Turns(unit, value ? 0 : p.rot.rot, D), y);
+    if (query || (!FP8 && writes)) {
+      char* to = query ? p.q_out + b * p.qo_tok + h * p.qo_head : rows + lo * tok;
+      store_unit<T, LAYOUT, false>(reinterpret_cast<T*>(to), unit, p.rot.rot, D, y);
+    }
+    if constexpr (FP8) {
+      float a = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2 * kVec; ++j) {
+        y[j] = or_nan(y[j]);
+        a = fmaxf(a, fabsf(y[j]));  // (a maximum passes over NaN)
+      }
+#pragma unroll
+      for (int m = 1; m < kUnits; m <<= 1) a = fmaxf(a, __shfl_xor(a, m, 64));
+      if (!writes) continue;
+      bool keeps;
+      const float s = settle(a, lo > 0, s0, &keeps);
+      if (lo > 0 && !keeps) recode<D, kUnits>(rows, tok, lo, s0, s, unit);
+      put_unit_codes<LAYOUT, kVec>(rows + lo * tok, unit, p.rot.rot, D, y, s, exact_inverse(s));
+      if (unit == 0) *scale = s;
+    }
+  }
+  __syncthreads();  // (every thread has read the length, which may be written in place)
+  if (tid == 0) p.new_lens[b] = (int)(page >= 0 ? past + 1 : past);
+}
+
+template <typename T, bool FP8, int D, int LAYOUT>
+void launch_layout(dim3 grid, hipStream_t st, const WriteParams& p) {
+  if (p.cu) {
+    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, LAYOUT>), grid, dim3(kWriteThreads), 0, st, p);
+    return;
+  }
+  const int64_t lanes = (int64_t)p.n_kv_heads * (2 + (p.q ? p.group : 0)) * (D / (2 * RowVec<T, LAYOUT>::kVec));
+  const unsigned threads = (unsigned)std::min<int64_t>((lanes + 63) / 64 * 64, kTokenThreads);
+  hipLaunchKernelGGL((ia_write_tokens<T, FP8, D, LAYOUT>), grid, dim3(threads), 0, st, p);
+}
+
 template <typename T, bool FP8, int D>
-void launch_write(int layout, dim3 grid, dim3 block, hipStream_t st, const WriteParams& p) {
+void launch_write(int layout, dim3 grid, hipStream_t st, const WriteParams& p) {
   if (layout == kRowsHalf)
-    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalf>), grid, block, 0, st, p);
+    launch_layout<T, FP8, D, kRowsHalf>(grid, st, p);
   else if (layout == kRowsInterleaved)
-    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsInterleaved>), grid, block, 0, st, p);
+    launch_layout<T, FP8, D, kRowsInterleaved>(grid, st, p);
   else
-    hipLaunchKernelGGL((ia_write_pages<T, FP8, D, kRowsHalfOdd>), grid, block, 0, st, p);
+    launch_layout<T, FP8, D, kRowsHalfOdd>(grid, st, p);
 }
 
 template <typename T, bool FP8>
-void launch_write_d(int d, int layout, dim3 grid, dim3 block, hipStream_t st, const WriteParams& p) {
+void launch_write_d(int d, int layout, dim3 grid, hipStream_t st, const WriteParams& p) {
   if (d == 64)
-    launch_write<T, FP8, 64>(layout, grid, block, st, p);
+    launch_write<T, FP8, 64>(layout, grid, st, p);
   else
-    launch_write<T, FP8, 128>(layout, grid, block, st, p);
+    launch_write<T, FP8, 128>(layout, grid, st, p);
 }
 
 }  // namespace
@@ -548,29 +618,24 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   // waves have in flight: 38k tokens of 8 kv heads of 128 bf16 and groups of 4 into pages of 16
   // took 162 us with half of the heads to a workgroup, 177 with all and 177 with a quarter; into
   // bf16 pages 176 with half, 190 with all, 164 with a quarter and 212 with one.
-  // Few tiles: a workgroup for each kv head.  Lengths that advance in place are read by one
-  // workgroup only, of as many waves as it has tasks.
-  int threads = kWriteThreads;
+  // Few tiles: a workgroup for each kv head.
   const int64_t head_rows = (int64_t)p.page_rows * (2 + (q ? p.group : 0)) * head_dim * eb;
   int64_t slices = n_kv_heads;
   if (tiles >= 2 * device_cus())
     slices = std::clamp<int64_t>(n_kv_heads * head_rows / (fp8 ? kWriteBytesFp8 : kWriteBytes), 1, n_kv_heads);
   p.kv_heads_per_wg = (int)((n_kv_heads + slices - 1) / slices);
-  if (in_place) {
-    p.kv_heads_per_wg = n_kv_heads;
-    threads = (2 + (q ? p.group : 0)) * n_kv_heads > 4 ? kWriteMaxThreads : kWriteThreads;
-  }
-  p.slices = (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg;
-  if (tiles * p.slices >= (int64_t)1 << 23) return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
-  const dim3 grid((unsigned)(tiles * p.slices)), block((unsigned)threads);
+  p.slices = cu_seqlens ? (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg : 1;
+  if (tiles * p.slices >= (int64_t)1 << (cu_seqlens ? 23 : 22))
+    return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  const dim3 grid((unsigned)(tiles * p.slices));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int layout = rotary_layout(rotary, eb);
   p.stream = stream_rows(rotary, layout, (int64_t)n_tokens * p.group * n_kv_heads * head_dim * eb, eb);
   if (rows->dtype == IA_BF16)
-    fp8 ? launch_write_d<bf16_t, true>(head_dim, layout, grid, block, st, p)
-        : launch_write_d<bf16_t, false>(head_dim, layout, grid, block, st, p);
+    fp8 ? launch_write_d<bf16_t, true>(head_dim, layout, grid, st, p)
+        : launch_write_d<bf16_t, false>(head_dim, layout, grid, st, p);
   else
-    fp8 ? launch_write_d<float, true>(head_dim, layout, grid, block, st, p)
-        : launch_write_d<float, false>(head_dim, layout, grid, block, st, p);
+    fp8 ? launch_write_d<float, true>(head_dim, layout, grid, st, p)
+        : launch_write_d<float, false>(head_dim, layout, grid, st, p);
   return check_launch("rotary append kv");
 }

@@ -297,6 +297,51 @@ def test_single_tokens_with_and_without_cu(device, kv):
         assert all(torch.equal(x, y) for x, y in zip(r, results[0]))
 
 
+@pytest.mark.parametrize("kv,dtype", [("bf16", BF16), ("f32", F32), ("fp8", BF16), ("fp8", F32)],
+                         ids=["bf16", "f32", "fp8-bf16", "fp8-f32"])
+@pytest.mark.parametrize("d,page,rot,layout,hq,hkv,paired", [
+    (128, 16, 128, "half", 128, 8, False),         # more rows than a workgroup has places for
+    (64, 32, 32, "interleaved", 32, 32, True),
+    (128, 16, 70, "half", 12, 4, True),            # a pair a lane
+    (64, 48, 10, "half", 5, 1, False),
+    (64, 256, 0, "half", 40, 8, False),
+    (128, 64, 96, "interleaved", 0, 2, False),     # no queries
+])
+def test_single_tokens_of_many_heads(device, kv, dtype, d, page, rot, layout, hq, hkv, paired):
+    """The form for single tokens writes what the packed form does, bit for bit: scales that stay
+    and that rise, pages that begin, end and are missing, explicit positions."""
+    announce(f"single tokens of many heads {kv} {dtype} {d} {page} {rot} {layout} {hq}+{hkv}")
+    past = [0, 3, page - 1, page, 2 * page - 1, 2 * page, -1, 7, 2 * page + 9, page + 2]
+    n = len(past)
+    g, pk, pv, table, scales = setup(device, rot + hq, n, hkv, page, d, 3, paired,
+                                     {"bf16": BF16, "f32": F32, "fp8": FP8}[kv])
+    table[7, 0] = -1
+    mag = torch.exp2(torch.randint(-6, 8, (n, hq + 2 * hkv, 1), device=device, generator=g).float())
+    buf = (torch.randn((n, hq + 2 * hkv, d), device=device, generator=g) * mag).to(dtype)
+    buf[5, hq, 3], buf[9, hq + hkv, d - 1] = float("inf"), float("nan")
+    q, k, v = buf.split([hq, hkv, hkv], 1)
+    plan = ia.rotary_plan(rot, base=300.0, layout=layout, factor=0.75, device=device)
+    cu = torch.arange(n + 1, device=device, dtype=torch.int32)
+    where = torch.randint(-5, 9000, (n,), device=device, generator=g, dtype=torch.int32)
+    for positions in (None, where):
+        results = []
+        for form in range(3):
+            a, b = pk.clone(), pv.clone()
+            sc = None if scales is None else tuple(s.clone() for s in scales)
+            lens = torch.tensor(past, device=device, dtype=torch.int32)
+            out = None if not hq else torch.empty_like(q) if form < 2 else buf.clone()[:, :hq]
+            qo, new = ia.rotary_append_kv(q if hq else None, k, v, plan, a, b, table, lens, cu if form == 0 else None,
+                                          positions=positions, scales=sc, q_out=out,
+                                          new_seq_lens=torch.empty_like(lens) if form == 1 else None)
+            torch.cuda.synchronize()
+            assert (new is lens) == (form == 2)
+            assert new.tolist() == [p + (p >= 0 and i != 7) for i, p in enumerate(past)]
+            results.append((new, a.view(torch.uint8), b.view(torch.uint8), *(sc or ()), *([qo.contiguous().view(torch.uint8)] if hq else [])))
+        assert any(not torch.equal(x, y) for x, y in zip(results[0][1:], (pk.view(torch.uint8),)))
+        for r in results[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(r, results[0]))
+
+
 @pytest.mark.parametrize("kv", ["bf16", "fp8"])
 def test_sequences_without_new_rows(device, kv):
     """A begun page of a sequence that gets no rows keeps its codes and its scale, whatever the
