@@ -23,9 +23,10 @@ def beam_select(logits, scores, n=None, *, done=None, pad_token=0, workspace=Non
     row that holds +inf offers nothing.  Where fewer than ``n`` are offered the rest score -inf.
 
     Returns ``(scores [batch, n] float32, tokens [batch, n] int32, parents [batch, n] int32)``,
-    new tensors; parents are rows ``b * beams + j``, as ``reorder_sequences`` takes them.  Sums
-    and the order are kept in 64 bits, so results do not depend on how rows are cut.  Launches
-    on the current stream, never synchronises, can be captured."""
+    new tensors; parents are rows ``b * beams + j``, as ``reorder_sequences`` takes them.  Keys
+    are compared in 64 bits, their logs of sums good to 2^-21; the same call gives the same bits
+    (how rows are cut, and with it a sum's last bits, follows from the sizes).  Launches on the
+    current stream, never synchronises, can be captured."""
     device_of(logits, scores, done)
     if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError("scores must be contiguous float32 [batch, beams]")
