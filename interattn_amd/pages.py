@@ -4,7 +4,7 @@
 ``refs [n_pages] int32``, the number of table entries that hold each page.  A page is free
 where its count is 0, and allocation takes the lowest free pages, so the state after a call
 is a function of the state before it.  ``tensors`` is every tensor whose pages the table
-names, as a list of ``[n_pages, ...]``: the K and V pools of all layers and, for fp8, their
+names, as any iterable of ``[n_pages, ...]``: the K and V pools of all layers and, for fp8, their
 scales; they need not be contiguous.
 
 Calls launch on the current stream of the tensors' device, never synchronise and can be
@@ -63,6 +63,7 @@ def _struct_tail(shape, stride, dtype, word):
 
 def _page_tensors(tensors, n_pages, ref):
     """C array of page tensors; ``n_pages`` None takes the first tensor's."""
+    tensors = tuple(tensors)  # (walked twice: an iterator would be at its end)
     dev, at = ref.get_device(), [t.data_ptr() for t in tensors]
     if not at:
         return None, 0, 0
