@@ -24,9 +24,11 @@ def beam_select(logits, scores, n=None, *, done=None, pad_token=0, workspace=Non
 
     Returns ``(scores [batch, n] float32, tokens [batch, n] int32, parents [batch, n] int32)``,
     new tensors; parents are rows ``b * beams + j``, as ``reorder_sequences`` takes them.  Keys
-    are compared in 64 bits, their logs of sums good to 2^-21; the same call gives the same bits
-    (how rows are cut, and with it a sum's last bits, follows from the sizes).  Launches on the
-    current stream, never synchronises, can be captured."""
+    are compared in 64 bits, their logs of sums (of float32 exponentials) off by at most
+    2^-24 (14 + 2.3 d), d how far a row's tokens lie under its largest logit on average, by their
+    probability (less than log vocab); the same call gives the same bits (how rows are cut, and
+    with it a sum's last bits, follows from the sizes).  Launches on the current stream, never
+    synchronises, can be captured."""
     device_of(logits, scores, done)
     if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError("scores must be contiguous float32 [batch, beams]")

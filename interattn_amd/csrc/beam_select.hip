@@ -3,7 +3,7 @@
 //   key(j, v) = scores[j] + logits[j, v] - logsumexp(logits[j])
 //
 // ia_beam_scan, one launch, one pass over the logits.  A wave takes a slice of a row, groups of
-// four 16-byte loads a lane, and keeps sum exp(x - M) against a reference M near its running
+// four 16-byte loads a lane, and keeps sum exp(x - M) against a reference M within 1 of its running
 // maximum, and the slice's n best logits (the order inside a row is that of the keys).  What is
 // below the n-th largest of the lanes' running maxima (found bit by bit with ballots, and over
 // the slices of a row that a workgroup holds) cannot be among them, so a group is one comparison
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kScanThreads = 256;
 constexpr int kScanWaves = kScanThreads / 64;
-constexpr int kFly = 4;              // chunks of a group, and in flight
+constexpr int kFly = 4;              // chunks of a group, and in flight (group_sum joins four)
 constexpr int kHeld = 640;           // candidates a wave holds: a chunk's 512 and some
 constexpr int kTrim = 128;           // candidates at which they are cut to the n best
 constexpr int kWorthFloor = 2;       // lanes with something better for which the floor is raised
@@ -164,6 +164,26 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // 16 bytes at any e
   u32x4_t w;
 };
 
+// The sum of `term` over a lane's elements of a group, joined in pairs.
+template <typename T, typename F>
+__device__ __forceinline__ float group_sum(const u32x4_t* w, F term) {
+  constexpr int kVec = RowVec<T>::kVec;
+  float part[kFly];
+#pragma unroll
+  for (int i = 0; i < kFly; ++i) {
+    float x[kVec];
+    widen(w[i], x, T{});
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = term(x[j]);
+#pragma unroll
+    for (int m = kVec / 2; m > 0; m /= 2)
+#pragma unroll
+      for (int j = 0; j < m; ++j) x[j] += x[j + m];
+    part[i] = x[0];
+  }
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
 // One slice of one row: its candidates and sum, handed over.  shares[w0 .. w1): the workgroup's
 // slices of the row, each with the order_key that its part of n values reach (`wave` this one).
 template <typename T>
@@ -218,32 +238,20 @@ __device__ __forceinline__ void scan_slice(const BeamParams& p, Candidate* held,
       for (int j = 0; j < kVec; ++j) most[i] = fmaxf(most[i], x[j]);
       all = fmaxf(all, most[i]);
     }
-    // (the reference is the maximum of a group that is well above the one before: exp stays
-    // below e^8 and few groups pay for a new one)
-    if (__ballot(all > ref + 8.f)) {
+    // The reference follows the maximum to within 1: a term's argument, whose roundings are a part
+    // of its size, is then no larger than the term lies under the maximum, or 1 (a reference that
+    // lagged by 8 put the log of a sum off by 2^-20.5 where one token is most of it).  Most groups
+    // raise nothing.  (As a difference, which a constant added to the row does not change.)
+    if (__ballot(all - ref > 1.f)) {
       const float to = wave_max(all);
       if (ref != kNegInf) sum *= (double)__builtin_amdgcn_exp2f((ref - to) * kLog2e);
       ref = to;
     }
     const float base = ref == kNegInf ? 0.f : ref;
-    float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < kFly; ++i) {
-      float x[kVec];
-      widen(w[i], x, T{});
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) part += __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
-    }
-    if (part != part) {  // NaN adds nothing; +infinity leaves the sum NaN: the row offers nothing
-      part = 0.f;
-#pragma unroll
-      for (int i = 0; i < kFly; ++i) {
-        float x[kVec];
-        widen(w[i], x, T{});
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) part += x[j] == x[j] ? __builtin_amdgcn_exp2f((x[j] - base) * kLog2e) : 0.f;
-      }
-    }
+    // (a tree of additions: 32 equal small terms in a row behind a large one were off by 2^-19.4)
+    float part = group_sum<T>(w, [&](float x) { return __builtin_amdgcn_exp2f((x - base) * kLog2e); });
+    if (part != part)  // NaN adds nothing; +infinity leaves the sum NaN: the row offers nothing
+      part = group_sum<T>(w, [&](float x) { return x == x ? __builtin_amdgcn_exp2f((x - base) * kLog2e) : 0.f; });
     sum += (double)part;
     // (equal ones stay: theirs may be the lower place)
     lo = fmaxf(lo, order_value(reached));
