@@ -1,9 +1,11 @@
 // Rotary positions: angles from whole positions, and rows of a head as pairs.
 //
 // Pair p of a head at position t turns by t * w[p].  w is held as turns of a circle in 64-bit
-// fixed point, so that t * w modulo one turn is an integer product that drops what overflows:
-// every position of 31 bits and sign has its angle to 2^-32 turns (1.5e-9), with no table and
-// no range reduction in floating point (in float32, t * w at t = 10^6 is off by 0.03).
+// fixed point, rounded once from the model's float64 frequencies, so that t * w modulo one turn
+// is an integer product that drops what overflows: every position of 31 bits and sign has its
+// frequency's angle to 1.25 * 2^-32 turns (1.8e-9 radians: 2^-32 cut off and 2^31 roundings of
+// 2^-65), with no table and no range reduction in floating point (in float32, t * w at t = 10^6
+// is off by 0.03).
 #pragma once
 
 #include "ia_common.hpp"

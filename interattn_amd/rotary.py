@@ -22,6 +22,19 @@ LAYOUTS = ("half", "interleaved")
 _TWO_ROWS = N.RotaryRows * 2
 
 
+# 2 pi in units of 10^-62: with the 53 bits of a float64 pi, the angle of position 2^31 would be
+# 150 units of 2^-32 turns off
+_TWO_PI = 628318530717958647692528676655900576839433879875021164194988918
+
+
+def _turns(w):
+    """``w`` radians as turns in units of 2^-64: the nearest whole number.  (Whole turns a position,
+    which no model has, are first taken off in float64.)"""
+    num, den = math.fmod(w, 2 * math.pi).as_integer_ratio()
+    num, den = num * (10 ** 62 << 64), den * _TWO_PI
+    return (2 * num + den) // (2 * den) % (1 << 64)
+
+
 class RotaryPlan:
     """Frequencies of a rotation on one device: ``dim`` channels in pairs, ``layout`` ``"half"``
     (channel i with i + dim / 2) or ``"interleaved"`` (2 i with 2 i + 1), ``factor`` the amplitude,
@@ -119,7 +132,7 @@ def rotary_plan(dim, *, base=None, scaling=None, inv_freq=None, factor=None, lay
             raise ValueError("inv_freq must hold a frequency for each of dim / 2 pairs")
     if not all(math.isfinite(x) for x in w) or (factor is not None and not math.isfinite(factor)):
         raise ValueError("frequencies and factor must be finite")
-    fixed = [int(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for x in w]
+    fixed = [_turns(x) for x in w]
     turns = torch.tensor([x - (1 << 64) if x >> 63 else x for x in fixed], dtype=torch.int64).to(device)
     return RotaryPlan(turns, layout, amplitude if factor is None else factor)
 
