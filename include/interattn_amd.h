@@ -613,8 +613,10 @@ typedef struct ia_rotary {
   float factor;
 } ia_rotary;
 
-/* Rows to rotate: in[t, h, :] and out[t, h, :] (strides in elements, 16-byte multiples; out
- * may be in). */
+/* Rows to rotate: in[t, h, :] and out[t, h, :] (strides in elements, 16-byte multiples).  out may
+ * be in, with the same strides; else it shares no memory with any row that the call reads or
+ * writes.  Rows that interleave in one buffer without a common period of their strides are
+ * taken to share. */
 typedef struct ia_rotary_rows {
   const void* in;
   void* out;

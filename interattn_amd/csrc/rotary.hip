@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "rotary.hpp"
+#include "row_spans.hpp"
 
 namespace ia {
 
@@ -110,6 +111,7 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
   if (!positions) return fail(IA_ERR_INVALID, "null pointer argument");
   const int eb = dtype == IA_F32 ? 4 : 2;
   RotParams p{};
+  RowSpan in[2] = {{nullptr, 0, 0, 0, 0, 0}, {nullptr, 0, 0, 0, 0, 0}}, out[2] = {in[0], in[0]};
   for (int i = 0; i < n_tensors; ++i) {
     const ia_rotary_rows& x = rows[i];
     if (x.n_heads < 0) return fail(IA_ERR_INVALID, "head counts");
@@ -118,8 +120,9 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
     const int64_t strides[4] = {x.in_token_stride, x.in_head_stride, x.out_token_stride, x.out_head_stride};
     for (int64_t s : strides)
       if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
-    if ((n_tokens > 1 && x.out_token_stride < head_dim) || (x.n_heads > 1 && x.out_head_stride < head_dim))
-      return fail(IA_ERR_INVALID, "output rows must not overlap");
+    in[i] = RowSpan(x.in, n_tokens, x.n_heads, x.in_token_stride * eb, x.in_head_stride * eb, head_dim * eb);
+    out[i] = RowSpan(x.out, n_tokens, x.n_heads, x.out_token_stride * eb, x.out_head_stride * eb, head_dim * eb);
+    if (!out[i].rows_apart()) return fail(IA_ERR_INVALID, "output rows must not overlap");
     if ((reinterpret_cast<uintptr_t>(x.in) | reinterpret_cast<uintptr_t>(x.out)) % 16)
       return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
     p.t[i] = RotTensor{static_cast<const char*>(x.in), static_cast<char*>(x.out), x.in_token_stride * eb,
@@ -145,6 +148,11 @@ extern "C" int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* ro
   p.heads_per_wg = (int)((all + slices - 1) / slices);
   const int64_t ny = (all + p.heads_per_wg - 1) / p.heads_per_wg;
   if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
+  // (a thread reads what it writes itself, and nothing else of an output)
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
+      if ((may_meet(out[i], in[j]) && !(i == j && out[i].same(in[j]))) || (i < j && may_meet(out[i], out[j])))
+        return fail(IA_ERR_INVALID, "an output must be its input itself, or overlap no input and no other output");
   const dim3 grid((unsigned)tiles, (unsigned)ny);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool stream_them = stream_rows(rotary, layout, n_tokens * all * head_dim * eb, eb);

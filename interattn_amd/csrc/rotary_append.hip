@@ -26,6 +26,7 @@
 
 #include "packed_rows.hpp"
 #include "rotary.hpp"
+#include "row_spans.hpp"
 
 namespace ia {
 
@@ -568,8 +569,8 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
     const int64_t qs[4] = {q->in_token_stride, q->in_head_stride, q->out_token_stride, q->out_head_stride};
     for (int64_t s : qs)
       if (s < 0 || (s * eb) % 16) return fail(IA_ERR_INVALID, "row strides must be non-negative 16-byte multiples");
-    if ((n_tokens > 1 && q->out_token_stride < head_dim) || (q->n_heads > 1 && q->out_head_stride < head_dim))
-      return fail(IA_ERR_INVALID, "output rows must not overlap");
+    const RowSpan out(q->out, n_tokens, q->n_heads, q->out_token_stride * eb, q->out_head_stride * eb, head_dim * eb);
+    if (!out.rows_apart()) return fail(IA_ERR_INVALID, "output rows must not overlap");
     if ((reinterpret_cast<uintptr_t>(q->in) | reinterpret_cast<uintptr_t>(q->out)) % 16)
       return fail(IA_ERR_INVALID, "rows must be 16-byte aligned");
     p.q = static_cast<const char*>(q->in);
@@ -627,6 +628,15 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   p.slices = cu_seqlens ? (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg : 1;
   if (tiles * p.slices >= (int64_t)1 << (cu_seqlens ? 23 : 22))
     return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  if (q) {
+    // (a lane reads the queries that it writes itself, and nothing else of the output)
+    const RowSpan out(p.q_out, n_tokens, q->n_heads, p.qo_tok, p.qo_head, head_dim * eb),
+        in(p.q, n_tokens, q->n_heads, p.q_tok, p.q_head, head_dim * eb),
+        k(p.k_new, n_tokens, n_kv_heads, p.kn_tok, p.kn_head, head_dim * eb),
+        v(p.v_new, n_tokens, n_kv_heads, p.vn_tok, p.vn_head, head_dim * eb);
+    if ((may_meet(out, in) && !out.same(in)) || may_meet(out, k) || may_meet(out, v))
+      return fail(IA_ERR_INVALID, "the turned queries must be the queries themselves, or overlap no input");
+  }
   const dim3 grid((unsigned)(tiles * p.slices));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int layout = rotary_layout(rotary, eb);

@@ -167,8 +167,9 @@ def apply_rotary(q, k, positions, plan, *, inverse=False, q_out=None, k_out=None
     """Turn packed rows ``q [tokens, Hq, D]`` and ``k [tokens, Hkv, D]`` (or None) to
     ``positions [tokens] int32`` (any, negative ones too): one launch, sums in float32, rounded
     once.  D is a multiple of 16 up to 256; channels past ``plan.dim`` are copied as they are.
-    Returns ``(q, k)`` turned: new tensors, or ``q_out`` / ``k_out``, which may be the inputs
-    themselves.  ``inverse``: angles negated (the gradient; a rotation by position differences
+    Returns ``(q, k)`` turned: new tensors, or ``q_out`` / ``k_out``, each of which may be its
+    input itself and has to lie apart from the inputs and the other output else (views of one
+    buffer do where their rows do).  ``inverse``: angles negated (the gradient; a rotation by position differences
     moves cached keys)."""
     device_of(q, k, positions, plan.turns if plan.dim else None, q_out, k_out)
     shape = q.shape
@@ -200,7 +201,8 @@ def rotary_append_kv(q, k_new, v_new, plan, pool_k, pool_v, block_table, seq_len
     ``q [tokens, Hq, D]`` (or None), ``k_new, v_new [tokens, Hkv, D]`` packed; sequence b's rows
     ``cu_seqlens[b] ..`` are the positions ``seq_lens[b], seq_lens[b] + 1, ...`` of the pool, and
     what they are turned to, unless ``positions [tokens] int32`` (not the tensor the lengths are
-    written to) says otherwise.  ``plan`` None turns nothing.  Pools are bf16 or float32 as the rows are, or fp8 with ``scales=(k_scale,
+    written to) says otherwise.  ``plan`` None turns nothing.  ``q_out`` may be ``q`` itself and has
+    to lie apart from the inputs else.  Pools are bf16 or float32 as the rows are, or fp8 with ``scales=(k_scale,
     v_scale)``, which the call sets: every page gets the least power of two that brings its
     largest finite magnitude down to 448; a page with earlier tokens keeps its scale while that
     is enough, else its codes are rewritten with it (exact, but for what turns subnormal).  A
