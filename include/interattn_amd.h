@@ -591,7 +591,7 @@ IA_API int ia_shared_prefix_decode(const ia_decode_shape* shape, const void* q, 
  * cu_seqlens[b + 1] - 1 (a device array [n_seq + 1] as for ia_prompt_attention) are
  * written at positions seq_lens[b], seq_lens[b] + 1, ... through the block table, and
  * new_seq_lens[b] (another array than seq_lens, so that ia_update_block_summaries can
- * have both) receives the length after them.  The many-token form of ia_append_kv: bf16
+ * have both, and apart from cu_seqlens) receives the length after them.  The many-token form of ia_append_kv: bf16
  * and f32 pools; a position whose page is not mapped (or past the table) is skipped, and
  * the length counts up to the first such position.
  */
@@ -640,7 +640,8 @@ IA_API int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* rows, 
  * where given) rotated to their positions in the sequence, or to positions[t] (device array
  * [n_tokens]) where that is given.  rotary null: nothing is turned.  q's dtype is rows->dtype;
  * its rows are written where the pool has no page too.  cu_seqlens null: one token per
- * sequence (n_tokens = n_seq); then, and only then, new_seq_lens may be seq_lens.
+ * sequence (n_tokens = n_seq); then, and only then, new_seq_lens may be seq_lens.  Else it shares
+ * no memory with seq_lens, cu_seqlens or positions.
  *
  * IA_FP8_E4M3 pools take f32 or bf16 rows and set k_scale / v_scale of the pages they write.
  * With a the largest finite magnitude of the call's rows in a (page, kv head), the scale is

@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "packed_rows.hpp"
+#include "row_spans.hpp"
 
 namespace ia {
 
@@ -157,6 +158,11 @@ extern "C" int ia_append_prompt_kv(const ia_paged_kv* kv, const ia_packed_kv* ro
   // few tiles: a workgroup per head, so that a short prompt is one round trip
   p.heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
   const dim3 grid((unsigned)tiles, (unsigned)((n_kv_heads + p.heads_per_wg - 1) / p.heads_per_wg));
+  // (a sequence's length is written while other workgroups still read theirs, and where they begin)
+  if (ints_meet(new_seq_lens, n_seq, seq_lens, n_seq))
+    return fail(IA_ERR_INVALID, "new_seq_lens must not overlap seq_lens");
+  if (ints_meet(new_seq_lens, n_seq, cu_seqlens, (int64_t)n_seq + 1))
+    return fail(IA_ERR_INVALID, "new_seq_lens must not overlap cu_seqlens");
   hipLaunchKernelGGL(ia_append_prompt_rows, grid, dim3(kAppendThreads), 0, static_cast<hipStream_t>(stream), p);
   return check_launch("append prompt kv");
 }

@@ -554,12 +554,9 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   const bool in_place = n_seq > 0 && new_seq_lens == seq_lens;
   if (in_place && cu_seqlens)
     return fail(IA_ERR_INVALID, "lengths advance in place for single tokens only (cu_seqlens null)");
-  if (n_seq > 0 && positions) {
-    // (lengths are written while other waves still look for their positions)
-    const uintptr_t a = reinterpret_cast<uintptr_t>(positions), b = reinterpret_cast<uintptr_t>(new_seq_lens);
-    if (a < b + 4 * (uintptr_t)n_seq && b < a + 4 * (uintptr_t)n_tokens)
-      return fail(IA_ERR_INVALID, "positions must not overlap new_seq_lens");
-  }
+  // (lengths are written while other waves still look for their positions)
+  if (positions && ints_meet(positions, n_tokens, new_seq_lens, n_seq))
+    return fail(IA_ERR_INVALID, "positions must not overlap new_seq_lens");
   WriteParams p{};
   p.group = 1;
   if (q) {
@@ -628,6 +625,11 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
   p.slices = cu_seqlens ? (n_kv_heads + p.kv_heads_per_wg - 1) / p.kv_heads_per_wg : 1;
   if (tiles * p.slices >= (int64_t)1 << (cu_seqlens ? 23 : 22))
     return fail(IA_ERR_UNSUPPORTED, "too many tokens for one launch");
+  // (a sequence's length is written while other workgroups still read theirs, and where they begin)
+  if (!in_place && ints_meet(new_seq_lens, n_seq, seq_lens, n_seq))
+    return fail(IA_ERR_INVALID, "new_seq_lens must not overlap seq_lens");
+  if (cu_seqlens && ints_meet(new_seq_lens, n_seq, cu_seqlens, (int64_t)n_seq + 1))
+    return fail(IA_ERR_INVALID, "new_seq_lens must not overlap cu_seqlens");
   if (q) {
     // (a lane reads the queries that it writes itself, and nothing else of the output)
     const RowSpan out(p.q_out, n_tokens, q->n_heads, p.qo_tok, p.qo_head, head_dim * eb),

@@ -63,4 +63,10 @@ inline bool may_meet(const RowSpan& a, const RowSpan& b) {
            apart_modulo(a, b, head, a.head_bytes(), b.head_bytes()));
 }
 
+// The same of two vectors of int32.
+inline bool ints_meet(const int32_t* a, int64_t n, const int32_t* b, int64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return n > 0 && m > 0 && x < y + 4 * (uintptr_t)m && y < x + 4 * (uintptr_t)n;
+}
+
 }  // namespace ia
