@@ -649,7 +649,8 @@ IA_API int ia_apply_rotary(const ia_rotary* rotary, const ia_rotary_rows* rows, 
  * sequence (its first one) keeps its scale s0 (finite, at least 2^-126) where a <= 448 s0, else
  * the earlier rows' codes c become e4m3(c * s0 / s).  Codes are x / s rounded to nearest even;
  * values that are not finite become NaN codes.  Rows of a page past the sequence's tokens keep
- * their codes.  A page must not be written by two sequences of a call.  kv->seq_scale must be
+ * their codes.  A page must not be written by two sequences of a call; k_scale and v_scale share
+ * no memory (k and v neither, for any pool).  kv->seq_scale must be
  * null: such copies of the scales have to be gathered again.
  */
 IA_API int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows* q, const ia_packed_kv* rows,

@@ -630,6 +630,11 @@ extern "C" int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows
     return fail(IA_ERR_INVALID, "new_seq_lens must not overlap seq_lens");
   if (cu_seqlens && ints_meet(new_seq_lens, n_seq, cu_seqlens, (int64_t)n_seq + 1))
     return fail(IA_ERR_INVALID, "new_seq_lens must not overlap cu_seqlens");
+  // (keys and values are written by different waves)
+  if (kv->k == kv->v) return fail(IA_ERR_INVALID, "the K and V pools must not be one");
+  if (fp8 && may_meet(RowSpan(kv->k_scale, kv->n_pages, 1, kv->scale_page_stride * 4, 0, (int64_t)n_kv_heads * 4),
+                      RowSpan(kv->v_scale, kv->n_pages, 1, kv->scale_page_stride * 4, 0, (int64_t)n_kv_heads * 4)))
+    return fail(IA_ERR_INVALID, "k_scale and v_scale must not share memory: the call sets both");
   if (q) {
     // (a lane reads the queries that it writes itself, and nothing else of the output)
     const RowSpan out(p.q_out, n_tokens, q->n_heads, p.qo_tok, p.qo_head, head_dim * eb),

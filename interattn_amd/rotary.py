@@ -203,7 +203,7 @@ def rotary_append_kv(q, k_new, v_new, plan, pool_k, pool_v, block_table, seq_len
     what they are turned to, unless ``positions [tokens] int32`` (not the tensor the lengths are
     written to) says otherwise.  ``plan`` None turns nothing.  ``q_out`` may be ``q`` itself and has
     to lie apart from the inputs else.  Pools are bf16 or float32 as the rows are, or fp8 with ``scales=(k_scale,
-    v_scale)``, which the call sets: every page gets the least power of two that brings its
+    v_scale)`` (two tensors, or views that lie apart), which the call sets: every page gets the least power of two that brings its
     largest finite magnitude down to 448; a page with earlier tokens keeps its scale while that
     is enough, else its codes are rewritten with it (exact, but for what turns subnormal).  A
     value that is not finite becomes NaN and sets no scale.  What else holds scales
