@@ -663,7 +663,7 @@ IA_API int ia_rotary_append_kv(const ia_rotary* rotary, const ia_rotary_rows* q,
  * v_out ([n_tokens, n_kv_heads, head_dim], contiguous, out_dtype IA_F32 or IA_BF16) are the
  * positions starts[b], starts[b] + 1, ... (device array [n_seq]) of sequence b in the pool,
  * fp8 codes times their page's scale.  Positions without a page give zeros; rows of no
- * sequence are left as they were.
+ * sequence are left as they were.  k_out and v_out must not overlap.
  */
 IA_API int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32_t out_dtype, const int32_t* starts,
                       const int32_t* cu_seqlens, int32_t n_seq, int32_t n_tokens, int32_t n_kv_heads,

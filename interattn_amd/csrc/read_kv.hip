@@ -10,6 +10,7 @@
 
 #include "packed_rows.hpp"
 #include "rotary.hpp"
+#include "row_spans.hpp"
 
 namespace ia {
 
@@ -217,6 +218,9 @@ extern "C" int ia_read_kv(const ia_paged_kv* kv, void* k_out, void* v_out, int32
   p.heads_per_wg = tiles >= 2 * device_cus() ? n_kv_heads : 1;
   const int64_t ny = (n_kv_heads + p.heads_per_wg - 1) / p.heads_per_wg;
   if (ny > 65535) return fail(IA_ERR_UNSUPPORTED, "too many heads");
+  const int64_t row_bytes = (int64_t)n_kv_heads * head_dim * ob;
+  if (may_meet(RowSpan(k_out, n_tokens, 1, row_bytes, 0, row_bytes), RowSpan(v_out, n_tokens, 1, row_bytes, 0, row_bytes)))
+    return fail(IA_ERR_INVALID, "k_out and v_out must not overlap");
   const dim3 grid((unsigned)tiles, (unsigned)ny);
   hipStream_t st = static_cast<hipStream_t>(stream);
   // outputs larger than the L2s are written past them, as stream_rows says
