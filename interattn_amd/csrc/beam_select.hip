@@ -8,10 +8,10 @@
 // below the n-th largest of the lanes' running maxima (found bit by bit with ballots, and over
 // the slices of a row that a workgroup holds) cannot be among them, so a group is one comparison
 // unless it holds something better; candidates wait in LDS and are cut to the n best when they
-// fill up.  The workgroup that ends last of a batch entry
-// joins the slices' sums, forms the candidates' keys in 64 bits (float32 keys of magnitude 10
-// would order equal what differs by 10^-6) and ranks those above a threshold.  Slices are handed
-// over through memory at the device's coherence point (ia_common.hpp).
+// fill up.  The workgroup that ends last of a batch entry joins the slices' sums, forms the
+// candidates' keys in 64 bits (float32 keys of magnitude 10 would order equal what differs by
+// 10^-6) and ranks those above a threshold, after cutting them to the n best where they are more
+// than 128.  Slices are handed over through memory at the device's coherence point (ia_common.hpp).
 //
 // Equal keys go to the lower beam * vocabulary + token.
 //
@@ -39,6 +39,7 @@ constexpr int kMaxBeams = 64, kMaxBest = 64;
 constexpr int kOwn = 8;              // candidates a merging thread keeps in registers
 constexpr int kMaxCandidates = kOwn * kScanThreads;  // of a batch entry, where a slice a row is fewer
 constexpr int kNear = 1024;          // of those above the threshold, in LDS; more go through memory
+constexpr int kRanked = 128;         // of those, as many as are ranked at once; more are cut first
 constexpr u32 kLowest = 0x00800000u; // the key of the lowest finite float
 constexpr int kWaves = 2048;         // of a call, where slices are long
 
@@ -338,7 +339,79 @@ struct MergeLds {
   int ended[kMaxBeams];
   u32 least[2][kScanWaves];
   int stay;
+  unsigned long long cut_keys[kMaxBest], cut_places[kMaxBest];  // of more than kRanked, the n best
+  int digits[256];                                              // how many have each value
+  int cut;
 };
+
+// The *want-th largest of the workgroup's values below 2^BITS, eight bits at a time: how many of
+// those that agree so far have each next digit.  value(o, &v): whether o counts, and its value.
+// *want becomes the number of those equal to the result that belong to the largest *want.
+template <int BITS, typename F>
+__device__ unsigned long long nth_largest(int count, int* want, int* digits, F value) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  unsigned long long edge = 0;
+  for (int shift = BITS - 8; shift >= 0; shift -= 8) {
+    digits[tid] = 0;
+    __syncthreads();
+    for (int o = tid; o < count; o += kScanThreads) {
+      unsigned long long v;
+      if (value(o, &v) && ((v ^ edge) >> shift) < 256) atomicAdd(&digits[v >> shift & 255], 1);
+    }
+    __syncthreads();
+    int n[4], mine = 0;  // a lane's four digits, the largest first
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine += n[j] = digits[255 - 4 * lane - j];
+    const int upto = wave_inclusive_scan(mine);
+    const int first = __builtin_ctzll(__ballot(upto >= *want));
+    int before = __builtin_amdgcn_readlane(upto - mine, first), digit = 4 * first;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int c = __builtin_amdgcn_readlane(n[j], first);
+      if (digit == 4 * first + j && before + c < *want) {
+        before += c;
+        ++digit;
+      }
+    }
+    *want -= before;
+    edge |= (unsigned long long)(255 - digit) << shift;
+    __syncthreads();  // (every wave has read the digits)
+  }
+  return edge;
+}
+
+// The n best of `count` candidates (more than n, in LDS and behind kNear in memory) to cut_keys and
+// cut_places, in any order.  Candidates are many where keys are equal: beams that hold the same, rows
+// that a mask leaves at the type's lowest value.  Ranked each against all, 64 equal beams (n of 64, 4,096
+// candidates) took 895 us a call, 12,000 where all keys were equal, and 8 flat rows of 32,000 (n of
+// 16) 2,700; cut first 163, 163 and 95.
+__device__ void cut_to_best(MergeLds& l, const unsigned long long* far_keys, const unsigned long long* far_places,
+                            int count, int n) {
+  auto key_at = [&](int o) { return o < kNear ? l.keys[o] : far_keys[o]; };
+  // (a beam below 64 and a token below 2^30: 40 bits; lower places are better)
+  auto lowness_at = [&](int o) { return ~(o < kNear ? l.places[o] : far_places[o]) & 0xffffffffffull; };
+  int want = n;
+  const unsigned long long key = nth_largest<64>(count, &want, l.digits, [&](int o, unsigned long long* v) {
+    *v = key_at(o);
+    return true;
+  });
+  const unsigned long long low = nth_largest<40>(count, &want, l.digits, [&](int o, unsigned long long* v) {
+    if (key_at(o) != key) return false;
+    *v = lowness_at(o);
+    return true;
+  });
+  if (threadIdx.x == 0) l.cut = 0;
+  __syncthreads();
+  for (int o = threadIdx.x; o < count; o += kScanThreads) {
+    const unsigned long long k = key_at(o);
+    if (k > key || (k == key && lowness_at(o) >= low)) {
+      const int to = atomicAdd(&l.cut, 1);
+      l.cut_keys[to] = k;
+      l.cut_places[to] = o < kNear ? l.places[o] : far_places[o];
+    }
+  }
+  __syncthreads();
+}
 
 // The n best of a batch entry's candidates, by the whole workgroup.
 __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
@@ -450,45 +523,41 @@ __device__ void merge_entry(const BeamParams& p, MergeLds& l, int b) {
   __threadfence_block();
   __syncthreads();
   // ranks: better keys, and equal ones at lower places
-  const int count = l.stay;
-  auto put = [&](int rank, double score, unsigned long long place) {
-    const int64_t to = (int64_t)b * p.n + rank;
-    p.out_scores[to] = (float)score;
-    p.out_tokens[to] = (int32_t)(u32)place;
-    p.out_rows[to] = (int)(row0 + (int64_t)(place >> 32));
-  };
-  if (count <= 128) {  // a candidate a lane, the others read across the wave
-    const int i = tid;
-    const unsigned long long k = i < count ? l.keys[i] : 0ull, at = i < count ? l.places[i] : 0ull;
-    int rank = 0;
-    for (int o0 = 0; o0 < count && wave * 64 < count; o0 += 64) {
-      const unsigned long long ok = o0 + lane < count ? l.keys[o0 + lane] : 0ull;
-      const unsigned long long oa = o0 + lane < count ? l.places[o0 + lane] : 0ull;
-      const int many = min(count - o0, 64);
+  int count = l.stay;
+  const unsigned long long *keys = l.keys, *places = l.places;
+  if (count > kRanked) {
+    cut_to_best(l, far_keys, far_places, count, p.n);
+    keys = l.cut_keys;
+    places = l.cut_places;
+    count = p.n;
+  }
+  // a candidate a lane, the others read across the wave
+  const unsigned long long k = tid < count ? keys[tid] : 0ull, at = tid < count ? places[tid] : 0ull;
+  int rank = 0;
+  for (int o0 = 0; o0 < count && wave * 64 < count; o0 += 64) {
+    const unsigned long long ok = o0 + lane < count ? keys[o0 + lane] : 0ull;
+    const unsigned long long oa = o0 + lane < count ? places[o0 + lane] : 0ull;
+    const int many = min(count - o0, 64);
 #pragma unroll 8
-      for (int o = 0; o < many; ++o) {
-        const unsigned long long x = of_lane(ok, o), y = of_lane(oa, o);
-        rank += x > k || (x == k && y < at);
-      }
-    }
-    if (i < count && rank < p.n) put(rank, order_value64(k), at);
-  } else {
-    auto key_at = [&](int o) { return o < kNear ? l.keys[o] : far_keys[o]; };
-    auto place_at = [&](int o) { return o < kNear ? l.places[o] : far_places[o]; };
-    for (int i = tid; i < count; i += kScanThreads) {
-      const unsigned long long k = key_at(i), at = place_at(i);
-      int rank = 0;
-      for (int o = 0; o < count; ++o) rank += key_at(o) > k || (key_at(o) == k && place_at(o) < at);
-      if (rank < p.n) put(rank, order_value64(k), at);
+    for (int o = 0; o < many; ++o) {
+      const unsigned long long x = of_lane(ok, o), y = of_lane(oa, o);
+      rank += x > k || (x == k && y < at);
     }
   }
+  auto put = [&](int to, double score, unsigned long long place) {
+    const int64_t i = (int64_t)b * p.n + to;
+    p.out_scores[i] = (float)score;
+    p.out_tokens[i] = (int32_t)(u32)place;
+    p.out_rows[i] = (int)(row0 + (int64_t)(place >> 32));
+  };
+  if (tid < count && rank < p.n) put(rank, order_value64(k), at);
   // fewer candidates than places: -infinity, the lowest ones that are none
   if (count < p.n && tid == 0) {
     int j = 0, v = 0;
     for (int r = count; r < p.n;) {
       const unsigned long long place = (unsigned long long)j << 32 | (u32)v;
       bool is = false;
-      for (int o = 0; o < count; ++o) is |= l.places[o] == place;
+      for (int o = 0; o < count; ++o) is |= places[o] == place;
       if (!is) put(r++, (double)kNegInf, place);
       if (++v == p.vocab) {
         v = 0;
