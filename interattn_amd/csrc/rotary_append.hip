@@ -19,9 +19,12 @@
 //
 // Bound by HBM for prompts: 38k tokens of 8 kv heads of 128 and groups of 4, bf16 rows, are read
 // and written in 162 us into fp8 pages (856 MB, 5.3 TB/s) and 164 us into bf16 ones (5.7 TB/s);
-// 3.5k tokens of 4 heads of 64 in 11.5 us.  Bound by its round trips (length, page, rows, scale)
-// for single tokens: 1 to 256 sequences of 48 heads into fp8 pages in 4.4 to 5.1 us, 2,048 in 23
-// (through the packed rows' kernel 8.2 to 25 and 71).
+// 3.5k tokens of 4 heads of 64 in 11.5 us.  Single tokens, up to what the device holds at once, are
+// bound by their round trips (length, page, rows, scale): 1 to 256 sequences of 48 heads into fp8
+// pages in 4.4 to 5.1 us.  More are bound by how many run together: the fp8 kernel holds 102
+// registers, a CU two of its workgroups of 6 waves, the device 512, so that 2,048 sequences are
+// four rounds, 23 us, where their bytes would take 9.  (Through the packed rows' kernel 8.2 to 25
+// and 71.)
 #include <algorithm>
 
 #include "packed_rows.hpp"

@@ -274,7 +274,8 @@ def read_kv(pool_k, pool_v, block_table, starts, cu_seqlens, n_tokens, *, scales
     ``out_dtype`` bf16 or float32 (the pool's by default, bf16 of fp8 pools).  For what a
     quantised cache really holds, sequences that move elsewhere, attention that wants packed
     K/V.  Positions without a page give zeros; rows of no sequence are left as ``k_out`` /
-    ``v_out``, which must not overlap, had them.  Any pool, capturable."""
+    ``v_out``, which must not overlap, had them (new tensors' are not set).  Any pool, capturable.
+    Forward only."""
     device_of(pool_k, pool_v, block_table, starts, cu_seqlens, k_out, v_out, *(scales or ()))
     n_seq = _n_seq(cu_seqlens)
     check_ints(starts, "starts", n_seq)

@@ -169,8 +169,9 @@ def apply_rotary(q, k, positions, plan, *, inverse=False, q_out=None, k_out=None
     once.  D is a multiple of 16 up to 256; channels past ``plan.dim`` are copied as they are.
     Returns ``(q, k)`` turned: new tensors, or ``q_out`` / ``k_out``, each of which may be its
     input itself and has to lie apart from the inputs and the other output else (views of one
-    buffer do where their rows do).  ``inverse``: angles negated (the gradient; a rotation by position differences
-    moves cached keys)."""
+    buffer do where their rows do).  ``inverse``: angles negated (the gradient; a rotation by
+    position differences moves cached keys).  Forward only: the outputs carry no gradient back to
+    the inputs; a backward pass calls it with the outputs' gradients and ``inverse``."""
     device_of(q, k, positions, plan.turns if plan.dim else None, q_out, k_out)
     shape = q.shape
     tokens = check_ints(positions, "positions", shape[0] if len(shape) else None)
@@ -212,7 +213,8 @@ def rotary_append_kv(q, k_new, v_new, plan, pool_k, pool_v, block_table, seq_len
     Without ``cu_seqlens`` every sequence has one token (a decode step) and ``seq_lens`` advances
     in place unless ``new_seq_lens`` is given.  Returns ``(q turned, lengths after it)``; a
     position without a page is skipped and the length counts up to the first of them, as in
-    ``append_prompt_kv``."""
+    ``append_prompt_kv``.  Rows of no sequence are left as ``q_out`` had them (a new tensor's are
+    not set).  Forward only."""
     device_of(k_new, pool_k, pool_v, block_table, seq_lens, v_new, cu_seqlens, q, q_out, positions, new_seq_lens,
               plan.turns if plan is not None and plan.dim else None, *(scales or ()))
     n_seq = check_ints(seq_lens, "seq_lens")
